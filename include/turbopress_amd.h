@@ -33,8 +33,12 @@ enum tp_status {
   TP_ERR_BAD_BLOCK = 6,           /* Hadamard block not a power of 2 dividing d, or too large */
   TP_ERR_HIP = 7,                 /* a HIP launch or query failed */
   TP_ERR_WORKSPACE = 8,           /* workspace missing or too small */
-  TP_ERR_BAD_LAYOUT = 9           /* device-layout descriptor inconsistent with the call */
+  TP_ERR_BAD_LAYOUT = 9,          /* device-layout descriptor inconsistent with the call */
+  TP_ERR_BAD_TYPE = 10            /* element type outside what the entry point supports */
 };
+
+/* Element types of the decoder operators' tensors. */
+enum tp_dtype { TP_F16 = 0, TP_BF16 = 1, TP_F32 = 2 };
 
 /* ABI version of the loaded library (TP_ABI_VERSION when headers match). */
 int tp_abi_version(void);
@@ -371,6 +375,102 @@ int tp_tcq_viterbi(const float* z, int64_t ldz, int64_t n, int64_t d, const floa
                    int n_states, const int32_t* start_state, uint8_t* level_codes, uint8_t* path_bits,
                    uint8_t* member_codes, int32_t* end_state, void* workspace, int64_t workspace_bytes,
                    void* stream);
+
+/* ---------------------------------------------------------------------------
+ * Decoder operators between the packed projections (no reference counterpart:
+ * the reference leaves them to the HF decoder it replays,
+ * scripts/graph_decode_bench.py:70-118)
+ * ------------------------------------------------------------------------- */
+
+/* y = h / sqrt(mean(h^2) + eps) * weight over rows of d elements, with
+ * h = x + residual (residual may be NULL: h = x).  Row r of x starts at
+ * element (r / inner) * x_outer + (r % inner) * x_inner (inner >= 1: rows of a
+ * slice of a wider tensor), of residual likewise; a row's elements are
+ * contiguous.  y and, when given, h_out are contiguous [rows, d] and alias
+ * neither input.  All tensors are of `dtype` and aligned to it.  Sums, mean
+ * and products are fp32; h enters the norm unrounded, y and h_out are rounded
+ * once.  rows = 0 does nothing. */
+int tp_rms_norm(int dtype, int64_t rows, int64_t inner, int64_t d, const void* x, int64_t x_outer, int64_t x_inner,
+                const void* residual, int64_t r_outer, int64_t r_inner, const void* weight, float eps,
+                void* y, void* h_out, void* stream);
+
+/* tp_rms_norm with its output in 8-bit floating point (OCP e4m3): codes
+ * uint8 [rows, ldc] (ldc >= d a multiple of 16, codes 16-byte aligned, columns
+ * [d, ldc) of a row may be written with zeros) and fp32 scales [rows, ceil(d /
+ * block)] for blocks of `block` columns (128, or 0: one scale per row);
+ * y = code * scale with scale = max(largest |y| of the block / 448, 2^-126).
+ * A block that holds a NaN has scale and codes NaN. */
+int tp_rms_norm_fp8(int dtype, int64_t rows, int64_t inner, int64_t d, const void* x, int64_t x_outer,
+                    int64_t x_inner, const void* residual, int64_t r_outer, int64_t r_inner, const void* weight,
+                    float eps, int block, uint8_t* codes, int64_t ldc, float* scales, void* h_out, void* stream);
+
+/* y[i, j] = sum over 128-column blocks b of a_scales[i, b] * w_scales[j / 128, b]
+ * * sum_{c in b} a[i, c] * w[j, c], plus bias[j]: a e4m3 [m, lda], a_scales
+ * fp32 [m, ceil(k / 128)], w e4m3 [n, ldw], w_scales fp32 [ceil(n / 128),
+ * ceil(k / 128)], bias (may be NULL) and y of `dtype`, y [m, ldy].  lda and
+ * ldw are at least k; rows of any alignment are taken, 16-byte aligned ones
+ * (pointers, lda and ldw) load faster.  Columns [k, ld) are not used, whatever
+ * they hold.  Sums are fp32, added in a fixed order; y rounds once.
+ * The workspace (tp_fp8_workspace_bytes, 16-byte aligned; NULL when that is 0)
+ * may hold anything.  m = 0 or n = 0 does nothing. */
+int tp_fp8_linear(int dtype, int64_t m, int64_t n, int64_t k, const uint8_t* a, int64_t lda, const float* a_scales,
+                  const uint8_t* w, int64_t ldw, const float* w_scales, const void* bias, void* y, int64_t ldy,
+                  void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Bytes of workspace of a tp_fp8_linear call on the current device (0: none
+ * needed; -1: sizes it does not take). */
+int64_t tp_fp8_workspace_bytes(int64_t m, int64_t n, int64_t k);
+
+/* Rotary positions: for each token t and head, with c, s the two halves of
+ * row positions[t] of `table` (fp32 [n_positions, rotary_dim]: cosines, then
+ * sines, of the position's rotary_dim / 2 angles), the pair (a, b) of index i
+ * becomes (a c_i - b s_i, b c_i + a s_i): elements (i, i + rotary_dim / 2) of
+ * the head, or (2 i, 2 i + 1) where `interleaved`; elements [rotary_dim, d)
+ * are copied.  q [tokens, hq, d] and k [tokens, hk, d] have token and head
+ * strides in elements (an element's neighbours are contiguous); hk may be 0.
+ * q_out is contiguous [tokens, hq, d].
+ *
+ * With k_cache NULL k_out is contiguous [tokens, hk, d].  Otherwise k_out is
+ * NULL, v is given, and the rotated k and the v of a token are written into
+ * the paged caches [n_pages, page_size, hk, d] (strides of page, slot and head
+ * in elements, kc[3] and vc[3]) at position p = positions[t] of sequence
+ * sequences[t] (NULL: sequence t): slot p % page_size of page
+ * block_table[sequence * table_width + p / page_size].  Two tokens of one
+ * position of one sequence in a call race.
+ *
+ * A token of a negative position is padding: its outputs are zero and nothing
+ * is written into the caches.  A position >= n_positions gives NaN outputs and
+ * writes nothing; a sequence outside [0, n_sequences), a position past
+ * table_width pages and a page outside [0, n_pages) write nothing. */
+int tp_rotary(int dtype, int64_t tokens, int64_t hq, int64_t hk, int64_t d, int64_t rotary_dim, int interleaved,
+              const void* q, int64_t q_token, int64_t q_head, const void* k, int64_t k_token, int64_t k_head,
+              const float* table, int64_t n_positions, const int64_t* positions, void* q_out, void* k_out,
+              const void* v, int64_t v_token, int64_t v_head, void* k_cache, const int64_t* kc, void* v_cache,
+              const int64_t* vc, int64_t n_pages, int64_t page_size, const int32_t* block_table,
+              int64_t table_width, int64_t n_sequences, const int32_t* sequences, void* stream);
+
+/* Attention of one new token per sequence over a paged cache: out[b, h] =
+ * sum_t p_t v_t with p = softmax(scale * q[b, h] . k_t) over the cached tokens
+ * t in [max(0, lengths[b] - window), lengths[b]) (window 0: from 0), head h
+ * reading cache head h / (hq / hkv).  q [batch, hq, d] (strides in elements),
+ * out contiguous [batch, hq, d]; caches as in tp_rotary; token t of sequence b
+ * is slot t % page_size of page block_table[b * table_width + t / page_size].
+ * d is a multiple of 8 up to 256, rows of q and of the caches are 16-byte
+ * aligned (pointers and strides); dtype is TP_F16 or TP_BF16.  A length of 0
+ * or below gives zeros.  Lengths past table_width pages are cut there; a page
+ * outside [0, n_pages) is skipped like a masked one.  What the caches hold
+ * outside the tokens read does not matter (NaN and infinity included).
+ * The workspace (tp_paged_attention_workspace_bytes, 256-byte aligned) may
+ * hold anything. */
+int tp_paged_attention(int dtype, int64_t batch, int64_t hq, int64_t hkv, int64_t d, const void* q, int64_t q_batch,
+                       int64_t q_head, const void* k_cache, const int64_t* kc, const void* v_cache,
+                       const int64_t* vc, int64_t n_pages, int64_t page_size, const int32_t* block_table,
+                       int64_t table_width, const int32_t* lengths, float scale, int64_t window, void* out,
+                       void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Bytes of workspace of a tp_paged_attention call on the current device (-1:
+ * sizes it does not take).  Depends on no length. */
+int64_t tp_paged_attention_workspace_bytes(int64_t batch, int64_t hq, int64_t hkv, int64_t d);
 
 #ifdef __cplusplus
 }

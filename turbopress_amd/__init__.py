@@ -24,6 +24,14 @@ _LAZY = {
     "pack_model": ("turbopress_amd.pack", "pack_model"),
     "load_packed_model": ("turbopress_amd.artifact", "load_packed_model"),
     "tcq_quantize_rows": ("turbopress_amd.encoder", "tcq_quantize_rows"),
+    "rms_norm": ("turbopress_amd.norm", "rms_norm"),
+    "rms_norm_fp8": ("turbopress_amd.norm", "rms_norm_fp8"),
+    "fp8_linear": ("turbopress_amd.fp8", "fp8_linear"),
+    "quantize_fp8_weight": ("turbopress_amd.fp8", "quantize_fp8_weight"),
+    "rotary_table": ("turbopress_amd.paged", "rotary_table"),
+    "rotary": ("turbopress_amd.paged", "rotary"),
+    "rotary_append": ("turbopress_amd.paged", "rotary_append"),
+    "paged_attention": ("turbopress_amd.paged", "paged_attention"),
 }
 
 __all__ = list(_LAZY)

@@ -8,7 +8,7 @@ operation on the packed path.
 from __future__ import annotations
 
 import ctypes
-from ctypes import c_int, c_int64, c_void_p, c_char_p, POINTER, c_uint8
+from ctypes import c_float, c_int, c_int64, c_void_p, c_char_p, POINTER, c_uint8
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "libturbopress_amd.so"
@@ -24,6 +24,10 @@ TP_ERR_BAD_BLOCK = 6
 TP_ERR_HIP = 7
 TP_ERR_WORKSPACE = 8
 TP_ERR_BAD_LAYOUT = 9
+TP_ERR_BAD_TYPE = 10
+
+# tp_dtype
+TP_F16, TP_BF16, TP_F32 = 0, 1, 2
 
 # Every exported symbol with its (restype, argtypes).
 _P = c_void_p
@@ -80,6 +84,22 @@ SIGNATURES.update({
     "tp_stack_gemv": (c_int, [_P, _I64, _P, c_int, c_int, c_int, _I64, _P]),
     "tp_stack_plan_blocks": (c_int64, [POINTER(c_int64), c_int]),
     "tp_stack_error": (c_int, [_P, POINTER(c_int)]),
+})
+
+# The decoder operators between the packed projections.
+SIGNATURES.update({
+    "tp_rms_norm": (c_int, [c_int, _I64, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _P, c_float, _P, _P, _P]),
+    "tp_rms_norm_fp8": (c_int, [c_int, _I64, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _P, c_float, c_int,
+                                _P, _I64, _P, _P, _P]),
+    "tp_fp8_linear": (c_int, [c_int, _I64, _I64, _I64, _P, _I64, _P, _P, _I64, _P, _P, _P, _I64, _P, _I64, _P]),
+    "tp_fp8_workspace_bytes": (_I64, [_I64, _I64, _I64]),
+    "tp_rotary": (c_int, [c_int, _I64, _I64, _I64, _I64, _I64, c_int, _P, _I64, _I64, _P, _I64, _I64,
+                          _P, _I64, _P, _P, _P, _P, _I64, _I64, _P, POINTER(c_int64), _P, POINTER(c_int64),
+                          _I64, _I64, _P, _I64, _I64, _P, _P]),
+    "tp_paged_attention": (c_int, [c_int, _I64, _I64, _I64, _I64, _P, _I64, _I64, _P, POINTER(c_int64),
+                                   _P, POINTER(c_int64), _I64, _I64, _P, _I64, _P, c_float, _I64, _P,
+                                   _P, _I64, _P]),
+    "tp_paged_attention_workspace_bytes": (_I64, [_I64, _I64, _I64, _I64]),
 })
 
 _LIB: ctypes.CDLL | None = None

@@ -15,6 +15,7 @@ extern "C" const char* tp_status_string(int status) {
     case TP_ERR_HIP: return "HIP launch or runtime error";
     case TP_ERR_WORKSPACE: return "workspace missing or too small";
     case TP_ERR_BAD_LAYOUT: return "device layout does not match the call";
+    case TP_ERR_BAD_TYPE: return "unsupported element type";
     default: return "unknown status";
   }
 }

@@ -1,0 +1,81 @@
+// What the decoder operators (norm, rotary positions, 8-bit product, paged
+// attention) share: element types, unaligned vectors, reductions across lanes.
+#pragma once
+
+#include "tp_common.h"
+
+namespace tp {
+
+typedef _Float16 f16_t;
+typedef __bf16 bf16_t;
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+
+// Casts between element types and fp32; f32 -> f16 / bf16 round to nearest even.
+template <typename T>
+struct Vec {
+  T v[8];
+};
+
+// 8 elements at any element-aligned address (gfx950 takes global accesses of
+// any byte alignment; the compiler makes one 16-byte access of a 2-byte type).
+template <typename T>
+__device__ __forceinline__ Vec<T> load8(const T* p) {
+  Vec<T> r;
+  __builtin_memcpy(&r, p, sizeof(r));
+  return r;
+}
+
+template <typename T>
+__device__ __forceinline__ void store8(T* p, const Vec<T>& r) {
+  __builtin_memcpy(p, &r, sizeof(r));
+}
+
+template <int CTRL>
+__device__ __forceinline__ float dpp(float v) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), CTRL, 0xF, 0xF, false));
+}
+
+struct AddOp {
+  __device__ __forceinline__ static float of(float a, float b) { return a + b; }
+};
+// The larger of two; NaN where either is (v_max_f32 drops a NaN).
+struct MaxNanOp {
+  __device__ __forceinline__ static float of(float a, float b) { return a > b || a != a ? a : b; }
+};
+
+// Over the 16 lanes of a row, in every lane: lane xor 1, xor 2, then (the
+// values being equal within groups) the half-row and the row mirror.
+template <typename Op>
+__device__ __forceinline__ float reduce16(float v) {
+  v = Op::of(v, dpp<0xB1>(v));
+  v = Op::of(v, dpp<0x4E>(v));
+  v = Op::of(v, dpp<0x141>(v));
+  return Op::of(v, dpp<0x140>(v));
+}
+
+// The value of the lane 16 (or 32) away, combined: both results of a permlane
+// swap of v with itself hold one of the two rows (halves) in every lane.
+template <typename Op>
+__device__ __forceinline__ float combine16(float v) {
+  const uint32_t x = __builtin_bit_cast(uint32_t, v);
+  const auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+  return Op::of(__builtin_bit_cast(float, (uint32_t)r[0]), __builtin_bit_cast(float, (uint32_t)r[1]));
+}
+template <typename Op>
+__device__ __forceinline__ float combine32(float v) {
+  const uint32_t x = __builtin_bit_cast(uint32_t, v);
+  const auto r = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+  return Op::of(__builtin_bit_cast(float, (uint32_t)r[0]), __builtin_bit_cast(float, (uint32_t)r[1]));
+}
+
+// Over the 64 lanes of a wave, in every lane.
+template <typename Op>
+__device__ __forceinline__ float reduce64(float v) {
+  return combine32<Op>(combine16<Op>(reduce16<Op>(v)));
+}
+
+inline bool dtype_ok(int dtype) { return dtype == TP_F16 || dtype == TP_BF16 || dtype == TP_F32; }
+inline int dtype_bytes(int dtype) { return dtype == TP_F32 ? 4 : 2; }
+
+}  // namespace tp
