@@ -460,17 +460,22 @@ int tp_rotary(int dtype, int64_t tokens, int64_t hq, int64_t hk, int64_t d, int6
  * or below gives zeros.  Lengths past table_width pages are cut there; a page
  * outside [0, n_pages) is skipped like a masked one.  What the caches hold
  * outside the tokens read does not matter (NaN and infinity included).
- * The workspace (tp_paged_attention_workspace_bytes, 256-byte aligned) may
- * hold anything. */
+ * page_size is at most 2^24.  The workspace (tp_paged_attention_workspace_bytes,
+ * 16-byte aligned) may hold anything; the counters
+ * (tp_paged_attention_counter_bytes, 4-byte aligned) are zero before the first
+ * call and after every call, so calls of any sizes share them in stream order;
+ * calls that overlap on one workspace or on one counter array race. */
 int tp_paged_attention(int dtype, int64_t batch, int64_t hq, int64_t hkv, int64_t d, const void* q, int64_t q_batch,
                        int64_t q_head, const void* k_cache, const int64_t* kc, const void* v_cache,
                        const int64_t* vc, int64_t n_pages, int64_t page_size, const int32_t* block_table,
                        int64_t table_width, const int32_t* lengths, float scale, int64_t window, void* out,
-                       void* workspace, int64_t workspace_bytes, void* stream);
+                       void* workspace, int64_t workspace_bytes, void* counters, int64_t counter_bytes,
+                       void* stream);
 
 /* Bytes of workspace of a tp_paged_attention call on the current device (-1:
- * sizes it does not take).  Depends on no length. */
+ * sizes it does not take), and of its counters.  Neither depends on a length. */
 int64_t tp_paged_attention_workspace_bytes(int64_t batch, int64_t hq, int64_t hkv, int64_t d);
+int64_t tp_paged_attention_counter_bytes(int64_t batch, int64_t hq, int64_t hkv, int64_t d);
 
 #ifdef __cplusplus
 }

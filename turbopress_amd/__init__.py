@@ -41,5 +41,6 @@ def __getattr__(name):
     if name in _LAZY:
         import importlib
         mod, attr = _LAZY[name]
-        return getattr(importlib.import_module(mod), attr)
+        value = globals()[name] = getattr(importlib.import_module(mod), attr)
+        return value  # (found without this function from now on: it took 3 us per use)
     raise AttributeError(f"module 'turbopress_amd' has no attribute {name!r}")

@@ -98,8 +98,9 @@ SIGNATURES.update({
                           _I64, _I64, _P, _I64, _I64, _P, _P]),
     "tp_paged_attention": (c_int, [c_int, _I64, _I64, _I64, _I64, _P, _I64, _I64, _P, POINTER(c_int64),
                                    _P, POINTER(c_int64), _I64, _I64, _P, _I64, _P, c_float, _I64, _P,
-                                   _P, _I64, _P]),
+                                   _P, _I64, _P, _I64, _P]),
     "tp_paged_attention_workspace_bytes": (_I64, [_I64, _I64, _I64, _I64]),
+    "tp_paged_attention_counter_bytes": (_I64, [_I64, _I64, _I64, _I64]),
 })
 
 _LIB: ctypes.CDLL | None = None

@@ -244,13 +244,17 @@ def paged_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, block_table: Te
     lengths = lengths.contiguous()
     out = torch.empty(b, hq, d, dtype=q.dtype, device=dev)
     lib = _lib.lib()
+    if b == 0:
+        return out
     need = lib.tp_paged_attention_workspace_bytes(b, hq, hkv, d)
-    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need > 0 else None
+    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    count = lib.tp_paged_attention_counter_bytes(b, hq, hkv, d)
+    counters = hk.shared_workspace(dev, count)  # zero between launches, as the split-K sums' counters
     st = lib.tp_paged_attention(
         DTYPE_CODES[q.dtype], b, hq, hkv, d, q.data_ptr(), q.stride(0), q.stride(1), k_cache.data_ptr(),
         _strides(k_cache), v_cache.data_ptr(), _strides(v_cache), k_cache.shape[0], k_cache.shape[1],
         block_table.data_ptr(), block_table.shape[1], lengths.data_ptr(),
         1.0 / math.sqrt(d) if scale is None else scale, window, out.data_ptr(),
-        0 if ws is None else ws.data_ptr(), max(need, 0), hk.current_stream_ptr(dev))
+        ws.data_ptr(), need, counters.data_ptr(), count, hk.current_stream_ptr(dev))
     _lib.check(st, "paged_attention")
     return out
