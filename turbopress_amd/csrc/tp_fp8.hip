@@ -1,11 +1,32 @@
 // Product of e4m3 activations and weights with scales per 128 columns:
 //
 //   y[i, j] = sum_b a_scales[i, b] w_scales[j / 128, b] sum_{c in block b} a[i, c] w[j, c]  (+ bias[j])
+//
+// A block's inner sum is one matrix instruction (16 x 16 x 128) from zero, and
+// one FMA per output multiplies it into fp32 sums; the weights are the
+// instructions' rows and the activations their columns, so that a lane's
+// outputs share an activation row: one product of scales per lane and block.
+// The K order inside a block is the instructions' own for both operands; sums
+// over blocks are in a fixed order.
+//
+// Few rows (fp8_takes_rows): every weight is read once, straight into operand
+// registers (bound by HBM: 151936 x 2560, 1 row, 66.8 us = 5.8 TB/s).  More:
+// tiles of both operands are staged in LDS by loads that bypass the registers
+// (bound by the matrix cores and LDS: 4096 x 8192 x 8192 257 us = 2.1 PFLOP/s,
+// where the instructions alone, without staging, sums and LDS reads, ran at
+// 3.6; or by the chain of a tile's blocks, 0.5 us each: 199 x 4096 x 2560
+// 11.6 us).
 #include "tp_ops_common.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace tp {
+
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef f16_t f16x2 __attribute__((ext_vector_type(2)));
+typedef f16_t f16x8 __attribute__((ext_vector_type(8)));
 
 struct Fp8Args {
   const uint8_t *a, *w;
@@ -14,42 +35,571 @@ struct Fp8Args {
   void* y;
   int64_t lda, ldw, ldy, m, n;
   int k, kb;
+  int tiles_m, tiles_n;
 };
 
-template <typename T>
-__global__ void __launch_bounds__(256) fp8_linear_kernel(const Fp8Args a) {
-  const int64_t j = (int64_t)blockIdx.x * 64 + (threadIdx.x & 63);
-  const int64_t i = (int64_t)blockIdx.y * 4 + (threadIdx.x >> 6);
-  if (i >= a.m || j >= a.n) return;
-  const uint8_t* ar = a.a + i * a.lda;
-  const uint8_t* wr = a.w + j * a.ldw;
-  float y = 0.0f;
-  for (int b = 0; b < a.kb; ++b) {
-    float part = 0.0f;
-    for (int c = 128 * b; c < min(a.k, 128 * b + 128); ++c)
-      part = fmaf(__builtin_amdgcn_cvt_f32_fp8(ar[c], 0), __builtin_amdgcn_cvt_f32_fp8(wr[c], 0), part);
-    y = fmaf(part, a.sa[i * a.kb + b] * a.sw[(j >> 7) * a.kb + b], y);
-  }
-  if (a.bias) y += (float)static_cast<const T*>(a.bias)[j];
-  static_cast<T*>(a.y)[i * a.ldy + j] = (T)y;
+// (cbsz = blgp = 0: both operands e4m3; scale operands 0: the unscaled form)
+__device__ __forceinline__ f32x4 mma16(i32x8 w, i32x8 a, f32x4 c) {
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, a, c, 0, 0, 0, 0, 0, 0);
 }
 
 template <typename T>
-int launch_fp8(const Fp8Args& a, hipStream_t s) {
-  hipLaunchKernelGGL((fp8_linear_kernel<T>), dim3((uint32_t)((a.n + 63) / 64), (uint32_t)((a.m + 3) / 4)), dim3(256), 0, s, a);
-  return launch_status();
+__device__ __forceinline__ void store4(const Fp8Args& g, int64_t i, int64_t j, f32x4 v) {
+  if (j >= g.n) return;
+  T* y = static_cast<T*>(g.y) + i * g.ldy + j;
+  const T* bias = static_cast<const T*>(g.bias) + j;
+  if (j + 4 <= g.n) {
+    if (g.bias)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] += (float)bias[e];
+    struct {
+      T v[4];
+    } r;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) r.v[e] = (T)v[e];
+    __builtin_memcpy(y, &r, sizeof(r));
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (j + e < g.n) y[e] = (T)(v[e] + (g.bias ? (float)bias[e] : 0.0f));
+  }
+}
+
+// Operands of a block of 16 rows x 128 columns.  fp16 and bf16 outputs take the
+// 8-bit instructions, whose inner sums are good to about 2^-16 of the result
+// (measured 1.3e-5 rms, and the same for both of their widths); fp32 outputs
+// convert the codes to fp16, exactly, for instructions with fp32 inner sums
+// (6e-9), at a quarter of the rate.
+template <bool F32>
+struct Operand;
+template <>
+struct Operand<false> {
+  i32x8 v;
+  __device__ __forceinline__ void set(i32x8 x) { v = x; }
+  __device__ __forceinline__ static f32x4 mul(const Operand& w, const Operand& a) {
+    return mma16(w.v, a.v, f32x4{0, 0, 0, 0});
+  }
+};
+template <>
+struct Operand<true> {
+  f16x8 v[4];
+  __device__ __forceinline__ void set(i32x8 x) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const f16x2 p0 = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x[2 * q], 1.0f, false);
+      const f16x2 p1 = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x[2 * q], 1.0f, true);
+      const f16x2 p2 = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x[2 * q + 1], 1.0f, false);
+      const f16x2 p3 = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x[2 * q + 1], 1.0f, true);
+      v[q] = f16x8{p0[0], p0[1], p1[0], p1[1], p2[0], p2[1], p3[0], p3[1]};
+    }
+  }
+  __device__ __forceinline__ static f32x4 mul(const Operand& w, const Operand& a) {
+    f32x4 d{0, 0, 0, 0};
+#pragma unroll
+    for (int q = 0; q < 4; ++q) d = __builtin_amdgcn_mfma_f32_16x16x32_f16(w.v[q], a.v[q], d, 0, 0, 0);
+    return d;
+  }
+};
+
+// ---------------------------------------------------------------------------
+// few rows
+// ---------------------------------------------------------------------------
+// The first `left` of 32 bytes at any alignment, then zeros.
+__device__ __forceinline__ i32x8 load_rest(const uint8_t* p, int left) {
+  i32x8 r = {0, 0, 0, 0, 0, 0, 0, 0};
+  if (left >= 32) {
+    __builtin_memcpy(&r, p, 32);
+  } else {
+#pragma unroll
+    for (int x = 0; x < 8; ++x) {
+      uint32_t v = 0;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (4 * x + e < left) v |= (uint32_t)p[4 * x + e] << (8 * e);
+      r[x] = (int)v;
+    }
+  }
+  return r;
+}
+
+// A workgroup takes RT tiles of 16 weight rows and all (up to 16 NC)
+// activation rows; its waves take every waves-th block of columns, the loads
+// of the next one in flight, and their sums are joined through LDS.
+template <typename T, int NC, int RT>
+__global__ void __launch_bounds__(NC == 1 ? 1024 : 512) fp8_rows_kernel(const Fp8Args g) {
+  using Op = Operand<sizeof(T) == 4>;
+  extern __shared__ __attribute__((aligned(16))) char fp8_lds[];
+  f32x4* const sums = reinterpret_cast<f32x4*>(fp8_lds);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int waves = blockDim.x >> 6;
+  const int lr = lane & 15, lg = lane >> 4;
+  const int64_t row0 = (int64_t)blockIdx.x * (16 * RT);
+  const uint8_t *wp[RT], *ap[NC];
+  const float *swp[RT], *sap[NC];
+#pragma unroll
+  for (int t = 0; t < RT; ++t) {
+    const int64_t r = min(row0 + 16 * t + lr, g.n - 1);  // (rows past the end: not stored)
+    wp[t] = g.w + r * g.ldw + 32 * lg;
+    swp[t] = g.sw + min((row0 + 16 * t) >> 7, (g.n - 1) >> 7) * g.kb;
+  }
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    const int64_t i = min((int64_t)(16 * c + lr), g.m - 1);
+    ap[c] = g.a + i * g.lda + 32 * lg;
+    sap[c] = g.sa + i * g.kb;
+  }
+  f32x4 acc[RT][NC];
+#pragma unroll
+  for (int t = 0; t < RT; ++t)
+#pragma unroll
+    for (int c = 0; c < NC; ++c) acc[t][c] = f32x4{0, 0, 0, 0};
+
+  struct Block {
+    i32x8 w[RT], a[NC];
+    float fa[NC], fw[RT];
+  };
+  auto load = [&](Block& x, int b) __attribute__((always_inline)) {
+#pragma unroll
+    for (int t = 0; t < RT; ++t) __builtin_memcpy(&x.w[t], wp[t] + 128 * b, 32);
+#pragma unroll
+    for (int c = 0; c < NC; ++c) __builtin_memcpy(&x.a[c], ap[c] + 128 * b, 32), x.fa[c] = sap[c][b];
+#pragma unroll
+    for (int t = 0; t < RT; ++t) x.fw[t] = swp[t][b];
+  };
+  auto add = [&](const Block& x) __attribute__((always_inline)) {
+    Op a[NC];
+#pragma unroll
+    for (int c = 0; c < NC; ++c) a[c].set(x.a[c]);
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+      Op w;
+      w.set(x.w[t]);
+#pragma unroll
+      for (int c = 0; c < NC; ++c) acc[t][c] += Op::mul(w, a[c]) * (x.fa[c] * x.fw[t]);
+    }
+  };
+  const int whole = g.k >> 7;  // blocks without a tail
+  if (wave < whole) {
+    Block x, y;
+    load(x, wave);
+    for (int b = wave; b < whole; b += waves) {
+      // (past the last: the first again, not used)
+      load(y, b + waves < whole ? b + waves : wave);
+      add(x);
+      x = y;
+    }
+  }
+  if (whole < g.kb && wave == whole % waves) {
+    const int left = g.k - 128 * whole - 32 * lg;  // columns of this lane's 32
+    Block x;
+#pragma unroll
+    for (int t = 0; t < RT; ++t) x.w[t] = load_rest(wp[t] + 128 * whole, left), x.fw[t] = swp[t][whole];
+#pragma unroll
+    for (int c = 0; c < NC; ++c) x.a[c] = load_rest(ap[c] + 128 * whole, left), x.fa[c] = sap[c][whole];
+    add(x);
+  }
+
+#pragma unroll
+  for (int t = 0; t < RT; ++t)
+#pragma unroll
+    for (int c = 0; c < NC; ++c) sums[(wave * RT * NC + t * NC + c) * 64 + lane] = acc[t][c];
+  __syncthreads();
+  for (int p = wave; p < RT * NC; p += waves) {
+    f32x4 y = sums[p * 64 + lane];
+    for (int x = 1; x < waves; ++x) y += sums[(x * RT * NC + p) * 64 + lane];
+    const int t = p / NC, c = p - t * NC;
+    const int64_t i = 16 * c + lr;
+    if (i < g.m) store4<T>(g, i, row0 + 16 * t + 4 * lg, y);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// more rows
+// ---------------------------------------------------------------------------
+// A workgroup of WN x WM waves, a wave TN x TM blocks of 16 weight rows x 16
+// activation rows.  LDS holds kBufs stages of 128 columns; a row's eight 16-byte
+// chunks are stored in the order c ^ (row & 7), so that the rows that a lane
+// group reads at one chunk fall on distinct banks (a load to LDS writes lane
+// after lane, so the lanes' global addresses are permuted).
+template <int WN, int WM, int TN, int TM>
+struct TileShape {
+  static constexpr int kWaves = WN * WM;
+  static constexpr int kBN = 16 * WN * TN, kBM = 16 * WM * TM;
+  static constexpr int kStage = (kBN + kBM) * 128;
+  static constexpr int kBufs = 4 * kStage <= 64 * 1024 ? 4 : 3 * kStage <= 72 * 1024 ? 3 : 2;
+  // scales of 8 stages, [row][8] activations' and [8][8] weights': of those in
+  // use, those arriving, and those that stages ahead of the block call for
+  static constexpr int kScales = kBufs * kStage, kScaleBuf = (kBM + 8) * 8 * 4;
+  static constexpr int kLds = kScales + 3 * kScaleBuf;
+  static constexpr int kWLoads = kBN / 8 / kWaves, kALoads = kBM / 8 / kWaves;  // 1 KB pieces (8 rows) of a wave
+  static constexpr int kLoads = kWLoads + kALoads + 2;
+  static_assert(kBN % (8 * kWaves) == 0 && kBM % (8 * kWaves) == 0 && kBM % 64 == 0 && 64 * kWaves >= kBM && kLds <= 160 * 1024, "");
+};
+
+template <int N>
+__device__ __forceinline__ void wait_vm() {
+  __asm__ volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_rsrc(const void* p, int64_t bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, (uint32_t)std::min<int64_t>(bytes, 0xfffffff0), 0x00020000);
+}
+
+template <typename T, int WN, int WM, int TN, int TM>
+__global__ void __launch_bounds__(64 * WN * WM, 2) fp8_tile_kernel(const Fp8Args g) {
+  using S = TileShape<WN, WM, TN, TM>;
+  using Op = Operand<sizeof(T) == 4>;
+  constexpr int BN = S::kBN, BM = S::kBM, NBUF = S::kBufs;
+  extern __shared__ __attribute__((aligned(16))) char fp8_lds[];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wn = wave % WN, wm = wave / WN;
+
+  // each XCD (blockIdx % 8) takes a contiguous run of tiles, activation tiles
+  // fastest: they share a weight tile in its L2
+  const int total = (int)gridDim.x, q8 = total >> 3, r8 = total & 7, xcd = (int)blockIdx.x & 7;
+  const int tile = xcd * q8 + min(xcd, r8) + ((int)blockIdx.x >> 3);
+  const int tn = tile / g.tiles_m, tm = tile - tn * g.tiles_m;
+  const int64_t n0 = (int64_t)tn * BN, m0 = (int64_t)tm * BM;
+
+  // Reads past the last row's columns, rounded up to 16, return zero (its
+  // 16-byte chunks hold a byte of the row each, so none is outside memory).
+  // The scalar offset is the column's alone, below the record count: the range
+  // check subtracts it.
+  const int64_t kr = (g.k + 15) & ~15;
+  const __amdgpu_buffer_rsrc_t wrs = rows_rsrc(g.w + n0 * g.ldw, (std::min<int64_t>(BN, g.n - n0) - 1) * g.ldw + kr);
+  const __amdgpu_buffer_rsrc_t ars = rows_rsrc(g.a + m0 * g.lda, (std::min<int64_t>(BM, g.m - m0) - 1) * g.lda + kr);
+  const __amdgpu_buffer_rsrc_t sars = rows_rsrc(g.sa + m0 * g.kb, std::min<int64_t>(BM, g.m - m0) * g.kb * 4);
+  const int64_t nb0 = n0 >> 7;  // weight blocks of the tile
+  const __amdgpu_buffer_rsrc_t swrs = rows_rsrc(g.sw + nb0 * g.kb, (((g.n - 1) >> 7) - nb0 + 1) * g.kb * 4);
+  const uint32_t lrow = lane >> 3, chunk = ((lane & 7) ^ lrow) * 16;  // of an 8-row piece
+  const uint32_t wv = (uint32_t)(8 * wave * S::kWLoads + lrow) * (uint32_t)g.ldw + chunk;
+  const uint32_t av = (uint32_t)(8 * wave * S::kALoads + lrow) * (uint32_t)g.lda + chunk;
+  // Scales go to LDS too (a scalar load would make every LDS wait a full one),
+  // those of 8 blocks together: a load takes 8 rows x 8 blocks, 32 bytes of a
+  // row (64 rows x 1 block at a time, 64 pieces of memory in one load, took as
+  // long as all operands).  With stage 8 q + j goes the j-th eighth of the
+  // scales of blocks 8 q + 8 .. + 15.
+  const uint32_t srow = 8 * (wave % (BM / 64)) + (lane >> 3);  // in an eighth
+  const uint32_t sav = srow * (uint32_t)g.kb * 4u + (lane & 7) * 4u, swv = (lane >> 3) * (uint32_t)g.kb * 4u + (lane & 7) * 4u;
+  auto stage_scales = [&](int j, int b, int ring) __attribute__((always_inline)) {  // blocks b .. b + 7
+    char* p = fp8_lds + S::kScales + ring * S::kScaleBuf;
+    // (blocks past the last: not loaded, nor used)
+    const uint32_t past = b + (int)(lane & 7) >= g.kb ? 0x80000000u : 0u;
+    const uint32_t soff = 4u * min(b, g.kb - 1);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(
+        sars, (__attribute__((address_space(3))) void*)(p + (j * (BM / 8) + 8 * (wave % (BM / 64))) * 32), 4,
+        (sav | past) + (uint32_t)(j * (BM / 8)) * (uint32_t)g.kb * 4u, soff, 0, 0);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(swrs, (__attribute__((address_space(3))) void*)(p + BM * 32), 4, swv | past, soff,
+                                             0, 0);
+  };
+  int ring = 1;  // where the next scales go
+  auto stage = [&](int b, int buf) __attribute__((always_inline)) {
+    char* p = fp8_lds + buf * S::kStage;
+    const int bc = min(b, g.kb - 1);
+    // chunks past the columns, and stages past the last, load nothing: zeros
+    const uint32_t past = 128 * b + (int)chunk >= kr ? 0x80000000u : 0u;
+    stage_scales(b & 7, (b & ~7) + 8, ring);
+    ring = (b & 7) == 7 ? (ring == 2 ? 0 : ring + 1) : ring;
+#pragma unroll
+    for (int x = 0; x < S::kWLoads; ++x)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(
+          wrs, (__attribute__((address_space(3))) void*)(p + (wave * S::kWLoads + x) * 1024), 16,
+          (wv | past) + (uint32_t)(8 * x) * (uint32_t)g.ldw, 128u * bc, 0, 0);
+#pragma unroll
+    for (int x = 0; x < S::kALoads; ++x)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(
+          ars, (__attribute__((address_space(3))) void*)(p + BN * 128 + (wave * S::kALoads + x) * 1024), 16,
+          (av | past) + (uint32_t)(8 * x) * (uint32_t)g.lda, 128u * bc, 0, 0);
+  };
+  // The bytes past the columns of the last stage's last chunk, which hold
+  // anything, are zeroed (by the wave that loaded them).
+  auto zero_rest = [&](int buf) __attribute__((always_inline)) {
+    const int in = g.k - (128 * (g.kb - 1) + (int)chunk);  // columns of this lane's chunk
+    if (in > 0 && in < 16) {
+      char* p = fp8_lds + buf * S::kStage + lane * 16;
+#pragma nounroll
+      for (int x = 0; x < S::kWLoads + S::kALoads; ++x) {
+        char* at = p + (x < S::kWLoads ? (wave * S::kWLoads + x) * 1024
+                                       : BN * 128 + (wave * S::kALoads + x - S::kWLoads) * 1024);
+#pragma nounroll
+        for (int e = in; e < 16; ++e) at[e] = 0;
+      }
+    }
+  };
+
+  // operand: columns 32 lg .. + 31 of row lr of 16
+  const int lr = lane & 15, lg = lane >> 4;
+  const uint32_t o0 = lr * 128 + (((2 * lg) ^ (lr & 7)) << 4), o1 = lr * 128 + (((2 * lg + 1) ^ (lr & 7)) << 4);
+  auto operand = [&](const char* rows) __attribute__((always_inline)) {
+    const u32x4 lo = *reinterpret_cast<const u32x4*>(rows + o0), hi = *reinterpret_cast<const u32x4*>(rows + o1);
+    Op op;
+    op.set(i32x8{(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], (int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]});
+    return op;
+  };
+  f32x4 acc[TN][TM], d[2][TM];
+  float f[TM], fa[TM], fw;  // scales of the products in d; of the current block, apart
+#pragma unroll
+  for (int t = 0; t < TN; ++t)
+#pragma unroll
+    for (int c = 0; c < TM; ++c) acc[t][c] = f32x4{0, 0, 0, 0};
+#pragma unroll
+  for (int c = 0; c < TM; ++c) d[1][c] = f32x4{0, 0, 0, 0}, f[c] = 0.0f;
+  constexpr int kAhead = TN < 4 ? TN : 4;  // weight operands in registers: read three groups ahead
+  Op a[TM], w[kAhead];
+  // what a block's first products need
+  auto first = [&](int b, int buf, int ring) __attribute__((always_inline)) {
+    const char* p = fp8_lds + buf * S::kStage;
+    const float* sl = reinterpret_cast<const float*>(fp8_lds + S::kScales + ring * S::kScaleBuf) + (b & 7);
+    // (the order of their use; the scales' product is formed where it is used)
+    w[0] = operand(p + wn * 16 * TN * 128);
+#pragma unroll
+    for (int c = 0; c < TM; ++c) a[c] = operand(p + BN * 128 + (wm * TM + c) * 16 * 128);
+#pragma unroll
+    for (int t = 1; t < kAhead - 1; ++t) w[t] = operand(p + (wn * TN + t) * 16 * 128);
+    fw = sl[(BM + (wn * 16 * TN) / 128) * 8];
+#pragma unroll
+    for (int c = 0; c < TM; ++c) fa[c] = sl[(wm * 16 * TM + 16 * c + lr) * 8];
+  };
+  auto sums = [&](int t, int c) __attribute__((always_inline)) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[t][c][e] = fmaf(d[t & 1][c][e], f[c], acc[t][c][e]);
+  };
+  static_assert(TN % 2 == 0, "a block's last products are in d[1], its first weights in w[0]");
+
+  // A block of 128 columns: TN groups of TM products, and under each product
+  // the sums of the group before it (of the last block's last group under the
+  // first).  sched_barrier keeps that order: left alone the scheduler gathers
+  // the reads, and waits for each group's products.
+  auto block = [&](int buf) __attribute__((always_inline)) {
+    const char* wl = fp8_lds + buf * S::kStage + wn * 16 * TN * 128;
+#pragma unroll
+    for (int t = 0; t < TN; ++t) {
+      if (t + kAhead - 1 < TN) w[(t + kAhead - 1) % kAhead] = operand(wl + (t + kAhead - 1) * 16 * 128);
+#pragma unroll
+      for (int c = 0; c < TM; ++c) {
+        d[t & 1][c] = Op::mul(w[t % kAhead], a[c]);
+        sums((t + TN - 1) % TN, c);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      if (t == 0) {
+#pragma unroll
+        for (int c = 0; c < TM; ++c) f[c] = fa[c] * fw;
+      }
+    }
+  };
+  auto meet = [&]() __attribute__((always_inline)) {
+    __builtin_amdgcn_s_barrier();
+    __asm__ volatile("" ::: "memory");
+  };
+
+#pragma unroll
+  for (int j = 0; j < 8; ++j) stage_scales(j, 0, 0);
+#pragma unroll
+  for (int s = 0; s < NBUF; ++s) stage(s, s);
+  wait_vm<(NBUF - 1) * S::kLoads>();
+  meet();
+  first(0, 0, 0);
+  int buf = 0, used = 0;  // used: where the block's scales are
+  for (int b = 0; b + 1 < g.kb; ++b) {
+    block(buf);
+    // With the last products under way the next stage is complete (its loads
+    // were issued a block ago) and every wave has read this one: its buffer
+    // takes the next loads, and the next block's first operands are read.
+    wait_vm<(NBUF - 2) * S::kLoads>();
+    meet();
+    stage(b + NBUF, buf);
+    buf = buf + 1 == NBUF ? 0 : buf + 1;
+    used = (b & 7) == 7 ? (used == 2 ? 0 : used + 1) : used;
+    first(b + 1, buf, used);
+  }
+  if (g.k & 15) {
+    zero_rest(buf);
+    __asm__ volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    meet();
+    first(g.kb - 1, buf, used);
+  }
+  block(buf);
+  wait_vm<0>();  // (no load to LDS may be in flight when the workgroup ends)
+#pragma unroll
+  for (int c = 0; c < TM; ++c) sums(TN - 1, c);
+  // (the sums end here: sunk into the stores' branches they spill)
+#pragma unroll
+  for (int t = 0; t < TN; ++t)
+#pragma unroll
+    for (int c = 0; c < TM; ++c) __asm__ volatile("" : "+v"(acc[t][c]));
+
+  // Out through LDS, 16 activation rows of a wave at a time (a lane holds row lr
+  // and weight rows 4 lg .. + 3 of a block): whole rows of the wave's 16 TN
+  // columns in 16-byte stores.  Stored as they lie, 8 bytes a lane over 16 rows,
+  // a tile of 256 x 256 took about 15 us more.
+  meet();
+  constexpr int kPer = 16 / sizeof(T);                   // elements of a store
+  constexpr int kPitch = 16 * TN * (int)sizeof(T) + 16;  // of a row in LDS
+  constexpr int kChunks = 16 * TN / kPer;                // stores of a row
+  static_assert(S::kWaves * 16 * kPitch <= S::kLds, "");
+  struct Out {
+    T v[kPer];
+  };
+  char* const ol = fp8_lds + wave * 16 * kPitch;
+  const int64_t j0 = n0 + wn * 16 * TN;
+  const T* bias = static_cast<const T*>(g.bias);
+#pragma unroll
+  for (int c = 0; c < TM; ++c) {
+#pragma unroll
+    for (int t = 0; t < TN; ++t) {
+      struct {
+        T v[4];
+      } o;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int64_t j = j0 + 16 * t + 4 * lg + e;
+        o.v[e] = (T)(acc[t][c][e] + (bias && j < g.n ? (float)bias[j] : 0.0f));
+      }
+      __builtin_memcpy(ol + lr * kPitch + (16 * t + 4 * lg) * (int)sizeof(T), &o, sizeof(o));
+    }
+    wave_lds_fence();
+    const int64_t i0 = m0 + wm * 16 * TM + 16 * c;
+    T* y = static_cast<T*>(g.y) + i0 * g.ldy + j0;
+#pragma unroll
+    for (int x = 0; x < 16 * kChunks / 64; ++x) {
+      const int id = 64 * x + lane, row = id / kChunks, j = (id - row * kChunks) * kPer;
+      Out o;
+      __builtin_memcpy(&o, __builtin_assume_aligned(ol + row * kPitch + j * (int)sizeof(T), 16), 16);
+      if (i0 + row < g.m) {
+        if (j0 + j + kPer <= g.n) {
+          __builtin_memcpy(y + (int64_t)row * g.ldy + j, &o, 16);
+        } else {
+#pragma unroll
+          for (int e = 0; e < kPer; ++e)
+            if (j0 + j + e < g.n) y[(int64_t)row * g.ldy + j + e] = o.v[e];
+        }
+      }
+    }
+    wave_lds_fence();
+  }
+}
+
+// Rows of any alignment copied to rows of `ld` bytes (a multiple of 16).
+__global__ void __launch_bounds__(256) fp8_align_kernel(const uint8_t* __restrict__ src, int64_t lds, uint8_t* __restrict__ dst,
+                                                        int64_t ldd, int64_t rows, int k) {
+  const int64_t chunks = ldd / 16, all = rows * chunks;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (int64_t)gridDim.x * 256) {
+    const int64_t r = i / chunks;
+    const int c = (int)(i - r * chunks) * 16;
+    const uint8_t* p = src + r * lds + c;
+    u32x4 v = {0, 0, 0, 0};
+    if (c + 16 <= k) {
+      __builtin_memcpy(&v, p, 16);
+    } else {
+#pragma unroll
+      for (int x = 0; x < 16; ++x)
+        if (c + x < k) v[x >> 2] |= (uint32_t)p[x] << (8 * (x & 3));
+    }
+    *reinterpret_cast<u32x4*>(dst + r * ldd + c) = v;
+  }
 }
 
 bool fp8_sizes_ok(int64_t m, int64_t n, int64_t k) {
-  return m >= 0 && n >= 0 && k >= 1 && m <= 65535 * 4 && n <= (1 << 28) && k <= (1 << 20);
+  return m >= 0 && n >= 0 && k >= 1 && m <= (1 << 24) && n <= (1 << 28) && k <= (1 << 20);
 }
+
+bool fp8_rows_aligned(const void* p, int64_t ld) { return ((ld | (int64_t)(uintptr_t)p) & 15) == 0; }
+
+template <typename T, int NC, int RT>
+void launch_rows(const Fp8Args& g, int waves, hipStream_t s) {
+  const int64_t groups = (g.n + 16 * RT - 1) / (16 * RT);
+  const int lds = waves * RT * NC * 64 * 16;
+  if (lds > 64 * 1024) allow_dynamic_lds(reinterpret_cast<const void*>(&fp8_rows_kernel<T, NC, RT>), 0);
+  hipLaunchKernelGGL((fp8_rows_kernel<T, NC, RT>), dim3((uint32_t)groups), dim3(64 * waves), lds, s, g);
+}
+
+// Whether a call takes the rows kernel.  us at (n, k), rows kernel against the
+// fastest tiles:
+//   32 rows  4096, 2560: 7.0 / 10.7   2560, 9728: 17.8 / 30.5   9728, 2560: 13.7 / 11.0   16384, 1000: 9.4 / 8.3
+//   64 rows  4096, 2560: 10.3 / 11.1  2560, 9728: 28.8 / 30.7   9728, 2560: 20.2 / 11.5   1024, 1024: 6.0 / 6.4
+// so 17..32 rows take it for up to 6144 weight rows (the tiles' time is their
+// chain of blocks until their count fills the GPU), more rows never.
+bool fp8_takes_rows(int64_t m, int64_t n) { return m <= 16 || (m <= 32 && n <= 6144); }
+
+template <typename T>
+int launch_rows_for(const Fp8Args& g, hipStream_t s) {
+  // 8 waves share a tile's columns (4 / 8 / 16 waves, 1 row: 4096 x 2560 5.5 /
+  // 4.6 / 4.9 us, 2560 x 9728 12.6 / 8.4 / 8.3); two tiles per workgroup where
+  // that leaves two workgroups per CU (1 / 2 tiles, 1 row: 151936 x 2560 76.9 /
+  // 66.8 us, 16384 x 1000 8.5 / 7.4, 9728 x 2560 7.8 / 8.5)
+  int waves = 8;
+  while (waves > 1 && waves > g.kb) waves /= 2;
+  const bool two = (g.n + 15) / 16 >= 4 * (int64_t)device_cu_count();
+  if (g.m <= 16) {
+    if (two) launch_rows<T, 1, 2>(g, waves, s);
+    else launch_rows<T, 1, 1>(g, waves, s);
+  } else {
+    launch_rows<T, 2, 1>(g, waves, s);
+  }
+  return launch_status();
+}
+
+template <typename T, int WN, int WM, int TN, int TM>
+int launch_tiles(Fp8Args g, hipStream_t s) {
+  using S = TileShape<WN, WM, TN, TM>;
+  g.tiles_m = (int)((g.m + S::kBM - 1) / S::kBM), g.tiles_n = (int)((g.n + S::kBN - 1) / S::kBN);
+  const int64_t total = (int64_t)g.tiles_m * g.tiles_n;
+  if (total > 0x7fffffff) return TP_ERR_BAD_DIMS;
+  if (S::kLds > 64 * 1024) allow_dynamic_lds(reinterpret_cast<const void*>(&fp8_tile_kernel<T, WN, WM, TN, TM>), 0);
+  hipLaunchKernelGGL((fp8_tile_kernel<T, WN, WM, TN, TM>), dim3((uint32_t)total), dim3(64 * S::kWaves), S::kLds, s, g);
+  return launch_status();
+}
+
+// Rounds of workgroups over the GPU times what a round takes, us: per block of
+// 128 columns, with one workgroup on a CU and with as many as it holds, and 4 to
+// begin and end.  Times of these picks, and of the other shapes in this order:
+//   2048 x 9728 x 2560 (rows, weight rows, columns)  81 (256 x 192)  88, -, 83, 95, 140
+//   4096 x 8192 x 8192  257 (256 x 256)  -, 300, 330, 410, 652
+//   512 x 4096 x 2560   15.7 (128 x 64)  40, 33, 21, -, 15.5
+//   199 x 4096 x 2560   11.6 (64 x 64)  40, 33, 20, 15, -
+template <typename T>
+int launch_tiles_for(const Fp8Args& g, hipStream_t s) {
+  struct Shape {
+    int n, m, per_cu;
+    double one, full;
+  };
+  static const Shape shapes[] = {
+      {256, 256, 1, 1.9, 1.9}, {256, 192, 1, 1.5, 1.5}, {128, 128, 2, 1.0, 1.3}, {128, 64, 2, 0.7, 1.0}, {64, 64, 2, 0.5, 0.75}};
+  const int64_t cus = device_cu_count();
+  // (fp32 outputs: the operands of the largest, converted, do not fit the registers)
+  int best = sizeof(T) == 4 ? 2 : 0;
+  double least = 0;
+  for (int x = best, first = best; x < 5; ++x) {
+    const Shape& p = shapes[x];
+    const int64_t t = ((g.m + p.m - 1) / p.m) * ((g.n + p.n - 1) / p.n);
+    const double c = t <= cus ? g.kb * p.one + 4 : (double)((t + cus * p.per_cu - 1) / (cus * p.per_cu)) * (g.kb * p.full + 4);
+    if (x == first || c < least) best = x, least = c;
+  }
+  if constexpr (sizeof(T) != 4) {
+    if (best == 0) return launch_tiles<T, 2, 4, 8, 4>(g, s);
+    if (best == 1) return launch_tiles<T, 2, 4, 8, 3>(g, s);
+  }
+  if (best == 2) return launch_tiles<T, 2, 2, 4, 4>(g, s);
+  if (best == 3) return launch_tiles<T, 2, 2, 4, 2>(g, s);
+  return launch_tiles<T, 2, 2, 2, 2>(g, s);
+}
+
+template <typename T>
+int launch_fp8(const Fp8Args& g, hipStream_t s) {
+  return fp8_takes_rows(g.m, g.n) ? launch_rows_for<T>(g, s) : launch_tiles_for<T>(g, s);
+}
+
+int64_t align_bytes(int64_t rows, int64_t k) { return rows * ((k + 15) & ~(int64_t)15); }
 
 }  // namespace tp
 
 using namespace tp;
 
-extern "C" int64_t tp_fp8_workspace_bytes(int64_t m, int64_t n, int64_t k) {
-  return fp8_sizes_ok(m, n, k) ? 0 : -1;
+extern "C" int64_t tp_fp8_workspace_bytes(int64_t m, int64_t n, int64_t k, const uint8_t* a, int64_t lda,
+                                          const uint8_t* w, int64_t ldw) {
+  if (!fp8_sizes_ok(m, n, k)) return -1;
+  if (m == 0 || n == 0 || fp8_takes_rows(m, n)) return 0;
+  return (fp8_rows_aligned(a, lda) ? 0 : align_bytes(m, k)) + (fp8_rows_aligned(w, ldw) ? 0 : align_bytes(n, k));
 }
 
 extern "C" int tp_fp8_linear(int dtype, int64_t m, int64_t n, int64_t k, const uint8_t* a, int64_t lda,
@@ -57,16 +607,29 @@ extern "C" int tp_fp8_linear(int dtype, int64_t m, int64_t n, int64_t k, const u
                              const void* bias, void* y, int64_t ldy, void* workspace, int64_t workspace_bytes,
                              void* stream) {
   if (!dtype_ok(dtype)) return TP_ERR_BAD_TYPE;
-  if (!fp8_sizes_ok(m, n, k) || lda < k || ldw < k || ldy < n) return TP_ERR_BAD_DIMS;
+  if (!fp8_sizes_ok(m, n, k) || lda < k || ldw < k || ldy < n || lda > (1 << 22) || ldw > (1 << 22)) return TP_ERR_BAD_DIMS;
   if (m == 0 || n == 0) return TP_OK;
   if (!a || !a_scales || !w || !w_scales || !y) return TP_ERR_NULL_POINTER;
   const uintptr_t mask = dtype_bytes(dtype) - 1;
-  if ((((uintptr_t)a_scales | (uintptr_t)w_scales) & 3) || (((uintptr_t)bias | (uintptr_t)y) & mask))
-    return TP_ERR_MISALIGNED;
-  const int64_t need = tp_fp8_workspace_bytes(m, n, k);
+  if ((((uintptr_t)a_scales | (uintptr_t)w_scales) & 3) || (((uintptr_t)bias | (uintptr_t)y) & mask)) return TP_ERR_MISALIGNED;
+  const int64_t need = tp_fp8_workspace_bytes(m, n, k, a, lda, w, ldw);
   if (need > 0 && (!workspace || workspace_bytes < need)) return TP_ERR_WORKSPACE;
-  Fp8Args g{a, w, a_scales, w_scales, bias, y, lda, ldw, ldy, m, n, (int)k, (int)((k + 127) / 128)};
+  if (need > 0 && ((uintptr_t)workspace & 15)) return TP_ERR_MISALIGNED;
   hipStream_t s = (hipStream_t)stream;
+  if (need > 0) {
+    const int64_t ld = (k + 15) & ~(int64_t)15;
+    uint8_t* free = static_cast<uint8_t*>(workspace);
+    auto align = [&](const uint8_t*& p, int64_t& from, int64_t rows) {
+      if (fp8_rows_aligned(p, from)) return;
+      const int64_t blocks = std::min<int64_t>((rows * (ld / 16) + 255) / 256, 16 * device_cu_count());
+      hipLaunchKernelGGL(fp8_align_kernel, dim3((uint32_t)blocks), dim3(256), 0, s, p, from, free, ld, rows, (int)k);
+      p = free, from = ld;
+      free += rows * ld;
+    };
+    align(a, lda, m);
+    align(w, ldw, n);
+  }
+  Fp8Args g{a, w, a_scales, w_scales, bias, y, lda, ldw, ldy, m, n, (int)k, (int)((k + 127) / 128), 0, 0};
   if (dtype == TP_F16) return launch_fp8<f16_t>(g, s);
   if (dtype == TP_BF16) return launch_fp8<bf16_t>(g, s);
   return launch_fp8<float>(g, s);

@@ -81,7 +81,7 @@ def fp8_linear(a: Tensor, a_scales: Tensor, w: Tensor, w_scales: Tensor, bias: T
     m = flat.shape[0]
     y = torch.empty(*a.shape[:-1], n, dtype=out_dtype, device=dev)
     lib = _lib.lib()
-    need = lib.tp_fp8_workspace_bytes(m, n, k)
+    need = lib.tp_fp8_workspace_bytes(m, n, k, flat.data_ptr(), flat.stride(0), w.data_ptr(), w.stride(0))
     ws = torch.empty(need, dtype=torch.uint8, device=dev) if need > 0 else None
     st = lib.tp_fp8_linear(code, m, n, k, flat.data_ptr(), flat.stride(0), a_scales.contiguous().data_ptr(),
                            w.data_ptr(), w.stride(0), w_scales.contiguous().data_ptr(),
