@@ -497,7 +497,8 @@ extern "C" int tp_paged_attention(int dtype, int64_t batch, int64_t hq, int64_t 
       table_width < 0 || table_width > (1 << 30) || window < 0)
     return TP_ERR_BAD_DIMS;
   if (batch == 0) return TP_OK;
-  if (!q || !k_cache || !kc || !v_cache || !vc || !block_table || !lengths || !out) return TP_ERR_NULL_POINTER;
+  if (!q || !kc || !vc || !lengths || !out || (n_pages > 0 && (!k_cache || !v_cache)) || (table_width > 0 && !block_table))
+    return TP_ERR_NULL_POINTER;  // (empty tensors have no address)
   if (((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)out) & 15) return TP_ERR_MISALIGNED;
   if ((q_batch | q_head | kc[0] | kc[1] | kc[2] | vc[0] | vc[1] | vc[2]) & 7) return TP_ERR_MISALIGNED;
   if (((uintptr_t)block_table | (uintptr_t)lengths) & 3) return TP_ERR_MISALIGNED;

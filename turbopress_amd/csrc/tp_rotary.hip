@@ -141,7 +141,7 @@ extern "C" int tp_rotary(int dtype, int64_t tokens, int64_t hq, int64_t hk, int6
   RotaryArgs a{};
   if (k_cache) {
     if (!hk || n_pages < 0 || page_size < 1 || table_width < 0 || n_sequences < 0) return TP_ERR_BAD_DIMS;
-    if (!k || !v || !v_cache || !kc || !vc || !block_table) return TP_ERR_NULL_POINTER;
+    if (!k || !v || !v_cache || !kc || !vc || (table_width > 0 && n_sequences > 0 && !block_table)) return TP_ERR_NULL_POINTER;
     a.hv = (int)hk;
     a.kc_page = kc[0], a.kc_slot = kc[1], a.kc_head = kc[2], a.vc_page = vc[0], a.vc_slot = vc[1], a.vc_head = vc[2];
   } else if (hk && (!k || !k_out)) {
