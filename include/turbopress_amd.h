@@ -46,6 +46,10 @@ int tp_abi_version(void);
 /* Static, human-readable name of a status code. */
 const char* tp_status_string(int status);
 
+/* The id of the graph capture that `stream` is part of (above 0, another for
+ * every capture), or 0 where it is not being captured. */
+int64_t tp_stream_capture_id(void* stream);
+
 /* Read `bytes` (a multiple of 16, 16-byte aligned) of device memory once
  * with a plain streaming-read kernel (each wave streams a contiguous slice
  * with 16-byte loads, 2 workgroups of 8 waves per CU); `sink` (one device

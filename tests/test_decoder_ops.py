@@ -563,6 +563,25 @@ def test_operators_in_a_graph(cuda):
 
 
 @pytest.mark.gpu
+def test_a_graph_stands_without_the_one_captured_before(cuda):
+    """Two graphs captured in a row, the second replayed alone: its counters'
+    zeros are its own, not the first one's."""
+    _, run = _step(_gen(21))
+    want = [t.clone() for t in run()]
+    graphs = []
+    for _ in range(2):
+        junk = torch.full((1 << 24,), 255, dtype=torch.uint8, device="cuda")  # (what memory may hold)
+        del junk
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs = run()
+        graphs.append((graph, outs))
+    for i in (1, 1, 0, 1):
+        graphs[i][0].replay()
+        assert all(torch.equal(a, b) for a, b in zip(graphs[i][1], want))
+
+
+@pytest.mark.gpu
 def test_operators_on_two_streams(cuda):
     """The same calls on two streams at once, each with workspaces of its own."""
     steps = [_step(_gen(30 + i)) for i in range(2)]

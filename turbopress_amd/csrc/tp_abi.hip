@@ -38,6 +38,14 @@ extern "C" int tp_subset_lut(int n_states, uint8_t* lut_out, int lut_len) {
   return TP_OK;
 }
 
+extern "C" int64_t tp_stream_capture_id(void* stream) {
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  if (hipStreamGetCaptureInfo((hipStream_t)stream, &status, &id) != hipSuccess || status != hipStreamCaptureStatusActive)
+    return 0;
+  return (int64_t)id;
+}
+
 // Streaming read of `n16` 16-byte words.  Every wave streams its own
 // contiguous slice (a multiple of 64 words), eight 1 KiB loads in flight
 // (short slices too: the loads past the slice are masked off):

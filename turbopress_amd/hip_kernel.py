@@ -201,19 +201,35 @@ def _aligned(nbytes: int) -> int:
     return (nbytes + _WS_ALIGN - 1) // _WS_ALIGN * _WS_ALIGN
 
 
+# Workspaces made while a graph was being captured, by (device, stream): the
+# capture's id and its buffers.  Their zeros are nodes of that graph, so only
+# that capture may share them: another graph replayed before it would find
+# whatever the memory held.
+_CAPTURED_WORKSPACES: dict = {}
+
+
 def shared_workspace(device, nbytes: int) -> Tensor:
     """The zeroed split-K workspace of `device` and its current stream, at
     least `nbytes` long (allocated or grown on first need)."""
     dev = torch.device(device)
     index = dev.index if dev.index is not None else torch.cuda.current_device()
-    key = (index, current_stream_ptr(torch.device("cuda", index)))
+    stream = torch._C._cuda_getCurrentRawStream(index)
+    key = (index, stream)
     ws = _WORKSPACES.get(key)
-    if ws is None or ws.numel() < nbytes:
-        if ws is not None:
-            _RETIRED_WORKSPACES.append(ws)
-        ws = torch.zeros(max(_aligned(nbytes), _WS_ALIGN), dtype=torch.uint8,
-                         device=torch.device("cuda", index))
-        _WORKSPACES[key] = ws
+    if ws is not None and ws.numel() >= nbytes:
+        return ws
+    new = max(_aligned(nbytes), _WS_ALIGN)
+    if torch.cuda.is_current_stream_capturing():
+        capture = _lib.lib().tp_stream_capture_id(stream)
+        held = _CAPTURED_WORKSPACES.get(key)
+        if held is None or held[0] != capture:
+            held = _CAPTURED_WORKSPACES[key] = (capture, [])
+        if not held[1] or held[1][-1].numel() < nbytes:
+            held[1].append(torch.zeros(new, dtype=torch.uint8, device=torch.device("cuda", index)))
+        return held[1][-1]
+    if ws is not None:
+        _RETIRED_WORKSPACES.append(ws)
+    ws = _WORKSPACES[key] = torch.zeros(new, dtype=torch.uint8, device=torch.device("cuda", index))
     return ws
 
 
