@@ -32,6 +32,7 @@ _LAZY = {
     "rotary": ("turbopress_amd.paged", "rotary"),
     "rotary_append": ("turbopress_amd.paged", "rotary_append"),
     "paged_attention": ("turbopress_amd.paged", "paged_attention"),
+    "PagedDecoder": ("turbopress_amd.paged_decode", "PagedDecoder"),
 }
 
 __all__ = list(_LAZY)
