@@ -39,6 +39,9 @@ __device__ __forceinline__ float dpp(float v) {
 struct AddOp {
   __device__ __forceinline__ static float of(float a, float b) { return a + b; }
 };
+struct MaxOp {
+  __device__ __forceinline__ static float of(float a, float b) { return fmaxf(a, b); }
+};
 // The larger of two; NaN where either is (v_max_f32 drops a NaN).
 struct MaxNanOp {
   __device__ __forceinline__ static float of(float a, float b) { return a > b || a != a ? a : b; }

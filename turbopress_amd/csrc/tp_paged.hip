@@ -24,6 +24,7 @@
 #include "tp_ops_common.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace tp {
 
@@ -36,11 +37,18 @@ typedef bf16_t bf16x8 __attribute__((ext_vector_type(8)));
 // Where a running maximum starts: finite, so that a score of -infinity has
 // probability e^-inf = 0 and not NaN, also where every score is -infinity.
 constexpr float kLeastScore = -3.0e38f;
-constexpr int kUnit = 128;   // tokens of a unit
-constexpr int kTile = 32;    // tokens of a wave's step
-constexpr int kWaves = kUnit / kTile;
-constexpr int kAhead = 4;      // states in flight per wave where states are joined
+constexpr int kTile = 32;      // tokens of a wave's step
 constexpr int kHeadTile = 16;  // query heads of a workgroup: columns of a matrix instruction
+
+// Waves of a workgroup; a unit is a step of each.  One workgroup per CU: 64 KB of
+// loads in flight keep it busy (4 waves of 64 columns have half, 8 the same).
+// More only add starts and joins: 64 x 8192 tokens, 8 heads of 128, 4 waves, 1 / 2
+// / 3 workgroups per CU 354 / 392 / 362 us, 1 x 131072 104 / 117 / 117; 8 waves
+// 357 and 107, and 12.3 us for 1 x 577 against 9.7 (fewer, longer units).
+template <int DP>
+__host__ __device__ constexpr int paged_waves() {
+  return DP <= 64 ? 8 : 4;
+}
 
 struct PagedArgs {
   const void *q, *k, *v;
@@ -54,14 +62,14 @@ struct PagedArgs {
   float scale;  // of the scores, in base 2
 };
 
-// What masked tokens' and columns' loads read.
-__device__ const uint4 kZeros[4] = {};
+// The row that masked tokens' loads read, and masked columns'.
+__device__ const uint4 kZeros[32] = {};
 
 // A 16-byte load from global memory (said so: of a pointer chosen from two, the
 // compiler would make a flat load, whose wait covers LDS too).
 template <typename V>
 __device__ __forceinline__ V load16(const void* p) {
-  return *(const __attribute__((address_space(1))) V*)p;
+  return __builtin_nontemporal_load((const __attribute__((address_space(1))) V*)p);
 }
 
 template <typename T>
@@ -87,24 +95,24 @@ __host__ __device__ constexpr int state_floats() {
   return kHeadTile * (DP + 2);
 }
 
-// Row offsets (elements) of a token in the caches; negative: masked.
+// Addresses of a token's rows in the caches; kZeros: masked.
 struct TokenRows {
-  int64_t k, v;
+  uint64_t k, v;
 };
 
-// Tokens of sequence b that attention reads: [first, len), first unit's base.
+// Tokens of a sequence that attention reads: [first, len); its first unit's base.
 struct Span {
   int first, len, base, units;
 };
 
-__device__ __forceinline__ Span span_of(const PagedArgs& a, int b) {
+template <int UNIT>
+__device__ __forceinline__ Span span_of(const PagedArgs& a, int length) {
   Span s;
-  const int64_t cap = a.table_width * a.page_size;
-  s.len = (int)min((int64_t)max(a.lengths[b], 0), cap);
+  s.len = (int)min((int64_t)max(length, 0), a.table_width * a.page_size);
   s.first = a.window > 0 && s.len > a.window ? (int)(s.len - a.window) : 0;
   s.base = s.first & ~(kTile - 1);
   // (an empty sequence is one unit too: its zeros have to be written)
-  s.units = max(1, (s.len - s.base + kUnit - 1) / kUnit);
+  s.units = max(1, (s.len - s.base + UNIT - 1) / UNIT);
   return s;
 }
 
@@ -118,31 +126,38 @@ __device__ __forceinline__ int64_t wave_scan(int64_t v, int lane) {
   return v;
 }
 
+__device__ __forceinline__ int opaque(int v) {
+  __asm__ volatile("" : "+v"(v));
+  return v;
+}
+
 // A value that all lanes share, where the compiler cannot see that they do.
 __device__ __forceinline__ int64_t uniform(int64_t v) {
   const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)v), hi = __builtin_amdgcn_readfirstlane((uint32_t)(v >> 32));
   return (int64_t)((uint64_t)hi << 32 | lo);
 }
 
-// The waves' states joined: f(head, column, 4 outputs, maximum, sum) for each
+// The first `states` waves' states joined: f(head, column, 4 outputs, maximum, sum) for each
 // head and 4 columns.  Wave w's outputs are floats [head][DP] at lds + w * pitch,
 // its maxima and sums ml[0][w] and ml[1][w].
-template <int DP, typename F>
-__device__ __forceinline__ void join_waves(int tid, int heads, const float (&ml)[2][kWaves][kHeadTile], const char* lds,
-                                           int pitch, F f) {
-  for (int i = tid; i < heads * (DP / 4); i += 64 * kWaves) {
+template <int DP, int W, typename F>
+__device__ __forceinline__ void join_waves(int tid, int heads, int states, const float (&ml)[2][W][kHeadTile],
+                                           const char* lds, int pitch, F f) {
+  for (int i = tid; i < heads * (DP / 4); i += 64 * W) {
     const int h = i / (DP / 4), c = 4 * (i - h * (DP / 4));
-    float top = ml[0][0][h];
+    float top = kLeastScore;
 #pragma unroll
-    for (int w = 1; w < kWaves; ++w) top = MaxNanOp::of(top, ml[0][w][h]);
+    for (int w = 0; w < W; ++w)
+      if (w < states) top = MaxOp::of(top, ml[0][w][h]);
     float sum = 0.0f;
     f32x4 y{0, 0, 0, 0};
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
-      const float e = __builtin_amdgcn_exp2f(ml[0][w][h] - top);
-      sum += e * ml[1][w][h];
-      y += e * *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(lds + w * pitch) + h * DP + c);
-    }
+    for (int w = 0; w < W; ++w)
+      if (w < states) {
+        const float e = __builtin_amdgcn_exp2f(ml[0][w][h] - top);
+        sum += e * ml[1][w][h];
+        y += e * *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(lds + w * pitch) + h * DP + c);
+      }
     f(h, c, y, top, sum);
   }
 }
@@ -170,43 +185,45 @@ __device__ __forceinline__ f32x2 get_device(const float* p) {
 }
 
 template <typename T, int DP, bool EXACT>
-__global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) paged_attention_kernel(const PagedArgs a) {
+__global__ void __launch_bounds__(64 * paged_waves<DP>(), 1) paged_attention_kernel(const PagedArgs a) {
+  constexpr int W = paged_waves<DP>(), UNIT = W * kTile;
   typedef typename Mma<T>::v8 v8;
   constexpr int KS = DP / 32;        // k steps of S^T
   constexpr int DT = DP / 16;        // row tiles of O^T
   constexpr int C = DP / 8;          // 16-byte chunks of a row
   constexpr int VL = C / 2;          // V loads per lane and tile
   constexpr int kRow = 2 * DP + 32;  // LDS bytes of a V row: 16 rows' 32-byte pieces fall on distinct banks
-  __shared__ __attribute__((aligned(16))) char v_lds[kWaves][kTile * kRow];
-  __shared__ TokenRows rows[kWaves][2][kTile];
-  __shared__ float ml[2][kWaves][kHeadTile];
+  __shared__ __attribute__((aligned(16))) char v_lds[W][kTile * kRow];
+  __shared__ TokenRows rows[W][2][kTile];
+  __shared__ float ml[2][W][kHeadTile];
   __shared__ uint32_t ticket;
   static_assert(kTile * kRow >= kHeadTile * DP * 4, "a wave's outputs fit its piece of LDS");
 
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int lr = lane & 15, lg = lane >> 4;
+  const int lane0 = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int per_seq = a.hkv * a.head_tiles;  // (cache head, head tile) pairs of a sequence
 
-  // all units, and this workgroup's run of them
-  int64_t all = 0;
-  for (int b0 = 0; b0 < a.batch; b0 += 64) {
-    const int64_t u = b0 + lane < a.batch ? (int64_t)span_of(a, b0 + lane).units : 0;
-    all += __shfl(wave_scan(u, lane), 63);
-  }
-  all = uniform(all);
+  // All units, and this workgroup's run of them.
+  const int units0 = span_of<UNIT>(a, lane0 < a.batch ? a.lengths[lane0] : 0).units;
+  auto units_of = [&](int b0) __attribute__((always_inline)) {
+    const int x = b0 + lane0;
+    const int u = b0 == 0 ? units0 : span_of<UNIT>(a, x < a.batch ? a.lengths[x] : 0).units;
+    return x < a.batch ? (int64_t)u * per_seq : (int64_t)0;
+  };
+  const int64_t upto0 = wave_scan(units_of(0), lane0);  // inclusive, of the first 64 sequences
+  int64_t total = __shfl(upto0, 63);
+  for (int b0 = 64; b0 < a.batch; b0 += 64) total += __shfl(wave_scan(units_of(b0), lane0), 63);
+  total = uniform(total);
   // (no more workgroups than units: every run holds one at least)
-  const int64_t total = all * per_seq, wgs = min((int64_t)gridDim.x, total);
+  const int64_t wgs = min((int64_t)gridDim.x, total);
   if (blockIdx.x >= wgs) return;
   int64_t at = blockIdx.x * total / wgs;
   const int64_t start = at, end = (blockIdx.x + 1) * total / wgs;
-
   // the sequence of its first unit
   int b = 0;
   int64_t seq0 = 0;  // units before sequence b
   for (int b0 = 0; b0 < a.batch; b0 += 64) {
-    const int64_t u = b0 + lane < a.batch ? (int64_t)span_of(a, b0 + lane).units * per_seq : 0;
-    const int64_t upto = wave_scan(u, lane) + seq0;
-    const uint64_t above = __ballot(b0 + lane < a.batch && upto > at);
+    const int64_t u = units_of(b0), upto = b0 == 0 ? upto0 : wave_scan(u, lane0) + seq0;
+    const uint64_t above = __ballot(b0 + lane0 < a.batch && upto > at);
     if (above) {
       const int l = __builtin_ctzll(above);
       b = b0 + l;
@@ -217,10 +234,13 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) paged_attention_kernel
   }
   b = __builtin_amdgcn_readfirstlane(b);
   seq0 = uniform(seq0);
+  Span sp = span_of<UNIT>(a, a.lengths[b]);
 
   while (at < end) {
     // a segment: units [j0, j1) of one (sequence, cache head, head tile)
-    const Span sp = span_of(a, b);
+    // (opaque per segment: addresses made from it are not kept across segments,
+    // nor those of the join across the tiles)
+    const int lane = opaque(lane0), lr = lane & 15, lg = lane >> 4;
     const int64_t off = at - seq0;
     const int pair = (int)(off / sp.units);
     const int j0 = (int)(off - (int64_t)pair * sp.units);
@@ -242,8 +262,8 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) paged_attention_kernel
       q[s] = load16<v8>(in ? p : zeros);
     }
 
-    const int tiles = (j1 - j0) * kWaves;
-    const int token0 = sp.base + j0 * kUnit;
+    const int tiles = (j1 - j0) * W;
+    const int token0 = sp.base + j0 * UNIT;
     auto page_of = [&](int i) __attribute__((always_inline)) {  // of lane's token of tile i; -1: masked
       const int t = token0 + i * kTile + (lane & 31);
       int page = -1;
@@ -253,29 +273,28 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) paged_attention_kernel
     auto put_rows = [&](int i, int page) __attribute__((always_inline)) {
       const int t = token0 + i * kTile + (lane & 31);
       const uint32_t slot = (uint32_t)t % (uint32_t)a.page_size;
-      TokenRows r{-1, -1};
-      if (page >= 0 && page < a.n_pages) r = TokenRows{page * a.kc_page + slot * a.kc_slot, page * a.vc_page + slot * a.vc_slot};
-      if (lane < kTile) rows[wave][(i / kWaves) & 1][lane] = r;
+      TokenRows r{(uint64_t)zeros, (uint64_t)zeros};
+      if (page >= 0 && page < a.n_pages)
+        r = TokenRows{(uint64_t)(kbase + page * a.kc_page + slot * a.kc_slot), (uint64_t)(vbase + page * a.vc_page + slot * a.vc_slot)};
+      if (lane < kTile) rows[wave][(i / W) & 1][lane] = r;
     };
     v8 k[2][KS], v[VL];
     auto load_k = [&](int i) __attribute__((always_inline)) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const int64_t r = rows[wave][(i / kWaves) & 1][16 * h + lr].k;
+        const T* r = reinterpret_cast<const T*>(rows[wave][(i / W) & 1][16 * h + lr].k) + 8 * lg;
 #pragma unroll
-        for (int s = 0; s < KS; ++s) {
-          const bool in = r >= 0 && (EXACT || 32 * s + 8 * lg < a.d);
-          k[h][s] = load16<v8>(in ? kbase + r + 32 * s + 8 * lg : zeros);
-        }
+        for (int s = 0; s < KS; ++s) k[h][s] = load16<v8>(EXACT || 32 * s + 8 * lg < a.d ? r + 32 * s : zeros);
       }
     };
+    // chunk c of a lane: 16-byte piece v_piece(c) of token v_token(c)
+    auto v_token = [&](int c) __attribute__((always_inline)) { return 64 % C == 0 ? lane / C + c * (64 / C) : (lane + 64 * c) / C; };
+    auto v_piece = [&](int c) __attribute__((always_inline)) { return 64 % C == 0 ? lane % C : (lane + 64 * c) % C; };
     auto load_v = [&](int i) __attribute__((always_inline)) {
 #pragma unroll
       for (int c = 0; c < VL; ++c) {
-        const int id = lane + 64 * c, t = id / C, ch = id - t * C;
-        const int64_t r = rows[wave][(i / kWaves) & 1][t].v;
-        const bool in = r >= 0 && (EXACT || 8 * ch < a.d);
-        v[c] = load16<v8>(in ? vbase + r + 8 * ch : zeros);
+        const T* r = reinterpret_cast<const T*>(rows[wave][(i / W) & 1][v_token(c)].v) + 8 * v_piece(c);
+        v[c] = load16<v8>(EXACT || 8 * v_piece(c) < a.d ? r : zeros);
       }
     };
 
@@ -287,18 +306,18 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) paged_attention_kernel
     put_rows(wave, page_of(wave));
     wave_lds_fence();
     // (in the loop's order, next pages, keys, values: its waits count loads)
-    int page = page_of(wave + kWaves);
+    int page = page_of(wave + W);
     __builtin_amdgcn_sched_barrier(0);
     load_k(wave);
     __builtin_amdgcn_sched_barrier(0);
     load_v(wave);
     __builtin_amdgcn_sched_barrier(0);
-    for (int i = wave; i < tiles; i += kWaves) {
+    for (int i = wave; i < tiles; i += W) {
       // rows of the next tile, pages of the one after
-      const uint64_t masked = __ballot(rows[wave][(i / kWaves) & 1][lane & 31].k < 0);
-      put_rows(i + kWaves, page);
+      const uint64_t masked = __ballot(rows[wave][(i / W) & 1][lane & 31].k == (uint64_t)zeros);
+      put_rows(i + W, page);
       wave_lds_fence();
-      page = page_of(i + 2 * kWaves);
+      page = page_of(i + 2 * W);
 
       f32x4 s[2];
 #pragma unroll
@@ -307,19 +326,26 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) paged_attention_kernel
 #pragma unroll
         for (int c = 0; c < KS; ++c) s[h] = Mma<T>::mul(k[h][c], q[c], s[h]);
       }
-      load_k(i + kWaves);
+      // (sched_barrier: moved up, the loads would take registers of their own)
+      __builtin_amdgcn_sched_barrier(0);
+      load_k(i + W);
 
       // lane: head lr, tokens 16 h + 4 lg + e
-      float top = m;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) s[h] *= a.scale;
+      if (masked) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (masked >> (16 * h + 4 * lg + e) & 1) s[h][e] = -INFINITY;
+      }
+      float top = m;  // (a NaN is not its maximum, but makes its exponential, so the sums, NaN)
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          s[h][e] *= a.scale;
-          if (masked && (masked >> (16 * h + 4 * lg + e) & 1)) s[h][e] = -INFINITY;
-          top = MaxNanOp::of(top, s[h][e]);
-        }
-      top = combine32<MaxNanOp>(combine16<MaxNanOp>(top));
+        for (int e = 0; e < 4; ++e) top = fmaxf(top, s[h][e]);
+      top = combine32<MaxOp>(combine16<MaxOp>(top));
       const float keep = __builtin_amdgcn_exp2f(m - top);
       m = top;
       l *= keep;
@@ -337,11 +363,12 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) paged_attention_kernel
 
 #pragma unroll
       for (int c = 0; c < VL; ++c) {
-        const int id = lane + 64 * c, t = id / C, ch = id - t * C;
-        *reinterpret_cast<v8*>(v_lds[wave] + t * kRow + 16 * ch) = v[c];
+        *reinterpret_cast<v8*>(v_lds[wave] + v_token(c) * kRow + 16 * v_piece(c)) = v[c];
       }
       wave_lds_fence();
-      load_v(i + kWaves);
+      __builtin_amdgcn_sched_barrier(0);
+      load_v(i + W);
+      __builtin_amdgcn_sched_barrier(0);
       // V^T: a lane takes column 16 t + lr of tokens 16 h + 4 lg .. + 3
 #pragma unroll
       for (int t = 0; t < DT; ++t) {
@@ -354,11 +381,13 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) paged_attention_kernel
         typedef int16_t i16x8 __attribute__((ext_vector_type(8)));
         const i16x8 both = __builtin_shufflevector(part[0], part[1], 0, 1, 2, 3, 4, 5, 6, 7);
         o[t] = Mma<T>::mul(__builtin_bit_cast(v8, both), p, o[t]);
+        if (t % 4 == 3) __builtin_amdgcn_sched_barrier(0);  // (eight reads at a time: registers)
       }
       wave_lds_fence();
     }
 
     // the waves' states, through LDS
+    const int tid = opaque((int)threadIdx.x);
     l = combine32<AddOp>(combine16<AddOp>(l));
     float* ow = reinterpret_cast<float*>(v_lds[wave]);
 #pragma unroll
@@ -367,7 +396,7 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) paged_attention_kernel
     __syncthreads();
     T* out = static_cast<T*>(a.out) + ((int64_t)b * a.hq + head0) * a.d;
     if (j0 == 0 && j1 == sp.units) {
-      join_waves<DP>(tid, heads, ml, v_lds[0], kTile * kRow, [&](int h, int c, f32x4 y, float, float sum) {
+      join_waves<DP, W>(tid, heads, W, ml, v_lds[0], kTile * kRow, [&](int h, int c, f32x4 y, float, float sum) {
         store_out(out, a.d, h, c, y, sum);
       });
     } else {
@@ -380,7 +409,7 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) paged_attention_kernel
       // whole L2 (64 sequences x 8192 tokens of one cache head: 186 us with a
       // fence per workgroup).
       float* part = a.parts + ((int64_t)blockIdx.x * 2 + (at != start)) * state_floats<DP>();
-      join_waves<DP>(tid, heads, ml, v_lds[0], kTile * kRow, [&](int h, int c, f32x4 y, float top, float sum) {
+      join_waves<DP, W>(tid, heads, W, ml, v_lds[0], kTile * kRow, [&](int h, int c, f32x4 y, float top, float sum) {
         put_device(part + 2 * kHeadTile + h * DP + c, y[0], y[1]);
         put_device(part + 2 * kHeadTile + h * DP + c + 2, y[2], y[3]);
         if (c == 0) put_device(part + 2 * h, top, sum);
@@ -398,36 +427,45 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) paged_attention_kernel
         const int later = g0 * total / wgs < u0;  // g0's state is its second
         const float* parts = a.parts + (g0 * 2 + later) * state_floats<DP>();
         const int64_t next = (2 - later) * state_floats<DP>();  // g0 + 1's, from g0's
-        // a wave takes every fourth state, kAhead of them at a time
-        for (int i = lane; i < heads * (DP / 4); i += 64) {
-          const int h = i / (DP / 4), c = 4 * (i - h * (DP / 4));
-          float top = kLeastScore, sum = 0.0f;
-          f32x4 y{0, 0, 0, 0};
-          for (int g = wave; g < n; g += kWaves * kAhead) {
-            f32x2 pm[kAhead], po[kAhead][2];
+        // 64 pieces (a head, 4 columns) of the states are a wave's, or, of few
+        // pieces, every PG-th of their states; its loads are in flight together
+        const int pieces = heads * (DP / 4), groups = (pieces + 63) / 64, pg = max(1, W / groups);
+        auto gather = [&](auto ahead) __attribute__((always_inline)) {
+          constexpr int A = decltype(ahead)::value;
+          for (int x = wave; x < groups * pg; x += W) {
+            const int part = x / groups, i = (x - part * groups) * 64 + lane;
+            if (i >= pieces) continue;
+            const int h = i / (DP / 4), c = 4 * (i - h * (DP / 4));
+            float top = kLeastScore, sum = 0.0f;
+            f32x4 y{0, 0, 0, 0};
+            for (int g = part; g < n; g += pg * A) {
+              f32x2 pm[A], po[A][2];
 #pragma unroll
-            for (int x = 0; x < kAhead; ++x) {
-              const int gx = min(g + x * kWaves, n - 1);
-              const float* p = parts + (gx == 0 ? 0 : next + (int64_t)(gx - 1) * 2 * state_floats<DP>());
-              pm[x] = get_device(p + 2 * h);
-              po[x][0] = get_device(p + 2 * kHeadTile + h * DP + c);
-              po[x][1] = get_device(p + 2 * kHeadTile + h * DP + c + 2);
-            }
-#pragma unroll
-            for (int x = 0; x < kAhead; ++x)
-              if (g + x * kWaves < n) {
-                const float m2 = MaxNanOp::of(top, pm[x][0]);
-                const float f = __builtin_amdgcn_exp2f(top - m2), fx = __builtin_amdgcn_exp2f(pm[x][0] - m2);
-                sum = sum * f + pm[x][1] * fx;
-                y = y * f + f32x4{po[x][0][0], po[x][0][1], po[x][1][0], po[x][1][1]} * fx;
-                top = m2;
+              for (int z = 0; z < A; ++z) {
+                const int gz = min(g + z * pg, n - 1);
+                const float* p = parts + (gz == 0 ? 0 : next + (int64_t)(gz - 1) * 2 * state_floats<DP>());
+                pm[z] = get_device(p + 2 * h);
+                po[z][0] = get_device(p + 2 * kHeadTile + h * DP + c);
+                po[z][1] = get_device(p + 2 * kHeadTile + h * DP + c + 2);
               }
+#pragma unroll
+              for (int z = 0; z < A; ++z)
+                if (g + z * pg < n) {
+                  const float m2 = MaxOp::of(top, pm[z][0]);
+                  const float f = __builtin_amdgcn_exp2f(top - m2), fz = __builtin_amdgcn_exp2f(pm[z][0] - m2);
+                  sum = sum * f + pm[z][1] * fz;
+                  y = y * f + f32x4{po[z][0][0], po[z][0][1], po[z][1][0], po[z][1][1]} * fz;
+                  top = m2;
+                }
+            }
+            *reinterpret_cast<f32x4*>(reinterpret_cast<float*>(v_lds[part]) + h * DP + c) = y;
+            if (c == 0) ml[0][part][h] = top, ml[1][part][h] = sum;
           }
-          *reinterpret_cast<f32x4*>(ow + h * DP + c) = y;
-          if (c == 0) ml[0][wave][h] = top, ml[1][wave][h] = sum;
-        }
+        };
+        if (n <= 4 * pg) gather(std::integral_constant<int, 4>{});
+        else gather(std::integral_constant<int, 16>{});
         __syncthreads();
-        join_waves<DP>(tid, heads, ml, v_lds[0], kTile * kRow, [&](int h, int c, f32x4 y, float, float sum) {
+        join_waves<DP, W>(tid, heads, pg, ml, v_lds[0], kTile * kRow, [&](int h, int c, f32x4 y, float, float sum) {
           store_out(out, a.d, h, c, y, sum);
         });
       }
@@ -436,7 +474,7 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) paged_attention_kernel
     at += j1 - j0;
     if (at - seq0 == (int64_t)sp.units * per_seq) {
       seq0 = at;
-      ++b;
+      if (++b < a.batch) sp = span_of<UNIT>(a, a.lengths[b]);
     }
   }
 }
@@ -444,18 +482,15 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) paged_attention_kernel
 // Columns that the kernel's instance for d holds.
 inline int padded_d(int64_t d) { return d <= 64 ? 64 : d <= 96 ? 96 : d <= 128 ? 128 : d <= 192 ? 192 : 256; }
 
-// Workgroups of a launch: what the GPU holds at once.
-inline int64_t paged_workgroups(int dp) { return (int64_t)device_cu_count() * (dp <= 128 ? 2 : 1); }
-
 bool paged_sizes_ok(int64_t batch, int64_t hq, int64_t hkv, int64_t d) {
   return batch >= 0 && batch <= (1 << 20) && hq >= 1 && hkv >= 1 && hq <= 65536 && hq % hkv == 0 && d >= 8 && d <= 256 && d % 8 == 0;
 }
 
 template <typename T, int DP>
 void launch_paged(const PagedArgs& a, hipStream_t s) {
-  const dim3 grid((uint32_t)paged_workgroups(DP));
-  if (a.d == DP) hipLaunchKernelGGL((paged_attention_kernel<T, DP, true>), grid, dim3(256), 0, s, a);
-  else hipLaunchKernelGGL((paged_attention_kernel<T, DP, false>), grid, dim3(256), 0, s, a);
+  const dim3 grid((uint32_t)device_cu_count());
+  if (a.d == DP) hipLaunchKernelGGL((paged_attention_kernel<T, DP, true>), grid, dim3(64 * paged_waves<DP>()), 0, s, a);
+  else hipLaunchKernelGGL((paged_attention_kernel<T, DP, false>), grid, dim3(64 * paged_waves<DP>()), 0, s, a);
 }
 
 template <typename T>
@@ -477,7 +512,7 @@ using namespace tp;
 extern "C" int64_t tp_paged_attention_workspace_bytes(int64_t batch, int64_t hq, int64_t hkv, int64_t d) {
   if (!paged_sizes_ok(batch, hq, hkv, d)) return -1;
   const int dp = padded_d(d);
-  return paged_workgroups(dp) * 2 * kHeadTile * (dp + 2) * (int64_t)sizeof(float);
+  return (int64_t)device_cu_count() * 2 * kHeadTile * (dp + 2) * (int64_t)sizeof(float);
 }
 
 extern "C" int64_t tp_paged_attention_counter_bytes(int64_t batch, int64_t hq, int64_t hkv, int64_t d) {
