@@ -11,7 +11,7 @@ import torch
 from torch import Tensor
 
 from turbopress_amd import _lib
-from turbopress_amd import hip_kernel as hk
+from turbopress_amd.hip_kernel import raw_stream as _raw_stream
 from turbopress_amd.norm import DTYPE_CODES, FP8_BLOCK
 
 __all__ = ["fp8_linear", "quantize_fp8_weight"]
@@ -53,17 +53,55 @@ def fp8_linear(a: Tensor, a_scales: Tensor, w: Tensor, w_scales: Tensor, bias: T
     scales fp32 [..., ceil(k / 128)], w float8_e4m3fn [n, k] with scales fp32
     [ceil(n / 128), ceil(k / 128)], bias of out_dtype.  fp32 sums in a fixed
     order, rounded once to out_dtype (fp16, bf16 or fp32): [..., n]."""
+    code, index, shape = DTYPE_CODES.get(out_dtype), a.get_device(), a.shape
+    n, k = w.shape if w.dim() == 2 else (0, 0)
+    kb = -(-k // FP8_BLOCK)
+    if code is None or index < 0 or a.dtype is not F8 or w.dtype is not F8 or k < 1 or not shape or shape[-1] != k \
+            or a_scales.dtype is not torch.float32 or a_scales.shape != (*shape[:-1], kb) \
+            or w_scales.dtype is not torch.float32 or w_scales.shape != (-(-n // FP8_BLOCK), kb) \
+            or a_scales.get_device() != index or w.get_device() != index or w_scales.get_device() != index \
+            or (bias is not None and (bias.dtype is not out_dtype or bias.shape != (n,) or bias.get_device() != index)):
+        _refuse(a, a_scales, w, w_scales, bias, out_dtype)
+    flat = a if len(shape) == 2 else a.reshape(-1, k)
+    lda, step = flat.stride()
+    if step != 1 or lda < k:
+        flat = flat.contiguous()
+        lda = k
+    ldw, step = w.stride()
+    if step != 1 or ldw < k:
+        w = w.contiguous()
+        ldw = k
+    m = flat.shape[0]
+    y = a.new_empty((*shape[:-1], n), dtype=out_dtype)
+    lib = _lib.lib()
+    ap, wp = flat.data_ptr(), w.data_ptr()
+    need = lib.tp_fp8_workspace_bytes(m, n, k, ap, lda, wp, ldw)
+    ws = a.new_empty(need, dtype=torch.uint8) if need > 0 else None
+    if not a_scales.is_contiguous():
+        a_scales = a_scales.contiguous()
+    if not w_scales.is_contiguous():
+        w_scales = w_scales.contiguous()
+    if bias is not None and not bias.is_contiguous():
+        bias = bias.contiguous()
+    st = lib.tp_fp8_linear(code, m, n, k, ap, lda, a_scales.data_ptr(), wp, ldw, w_scales.data_ptr(),
+                           0 if bias is None else bias.data_ptr(), y.data_ptr(), n,
+                           0 if ws is None else ws.data_ptr(), need, _raw_stream(index))
+    if st:
+        _lib.check(st, "fp8_linear")
+    return y
+
+
+def _refuse(a, a_scales, w, w_scales, bias, out_dtype) -> None:
+    """Raise for arguments that fp8_linear does not take."""
     if not a.is_cuda:
         raise RuntimeError("a must be a CUDA (ROCm) tensor; turbopress_amd has no CPU path")
-    code = DTYPE_CODES.get(out_dtype)
-    if code is None:
+    if out_dtype not in DTYPE_CODES:
         raise ValueError(f"out_dtype must be fp16, bf16 or fp32, got {out_dtype}")
     if a.dtype != F8 or w.dtype != F8 or w.dim() != 2 or a.dim() < 1 or a.shape[-1] != w.shape[1] or w.shape[1] < 1:
         raise ValueError(f"expected float8_e4m3fn a [..., k] and w [n, k], got {a.dtype} {list(a.shape)} "
                          f"and {w.dtype} {list(w.shape)}")
     n, k = w.shape
-    kb = -(-k // FP8_BLOCK)
-    dev = a.device
+    kb, dev = -(-k // FP8_BLOCK), a.device
     if a_scales.dtype != torch.float32 or a_scales.shape != (*a.shape[:-1], kb) or a_scales.device != dev:
         raise ValueError(f"a_scales must be fp32 {[*a.shape[:-1], kb]} on {dev}, "
                          f"got {a_scales.dtype} {list(a_scales.shape)} on {a_scales.device}")
@@ -71,21 +109,4 @@ def fp8_linear(a: Tensor, a_scales: Tensor, w: Tensor, w_scales: Tensor, bias: T
             or w.device != dev:
         raise ValueError(f"w_scales must be fp32 {[-(-n // FP8_BLOCK), kb]} beside w on {dev}, "
                          f"got {w_scales.dtype} {list(w_scales.shape)} on {w_scales.device}")
-    if bias is not None and (bias.dtype != out_dtype or bias.shape != (n,) or bias.device != dev):
-        raise ValueError(f"bias must be {out_dtype} [{n}] on {dev}, got {bias.dtype} {list(bias.shape)}")
-    flat = a if a.dim() == 2 else a.reshape(-1, k)
-    if flat.stride(1) != 1 or flat.stride(0) < k:
-        flat = flat.contiguous()
-    if w.stride(1) != 1 or w.stride(0) < k:
-        w = w.contiguous()
-    m = flat.shape[0]
-    y = torch.empty(*a.shape[:-1], n, dtype=out_dtype, device=dev)
-    lib = _lib.lib()
-    need = lib.tp_fp8_workspace_bytes(m, n, k, flat.data_ptr(), flat.stride(0), w.data_ptr(), w.stride(0))
-    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need > 0 else None
-    st = lib.tp_fp8_linear(code, m, n, k, flat.data_ptr(), flat.stride(0), a_scales.contiguous().data_ptr(),
-                           w.data_ptr(), w.stride(0), w_scales.contiguous().data_ptr(),
-                           0 if bias is None else bias.contiguous().data_ptr(), y.data_ptr(), n,
-                           0 if ws is None else ws.data_ptr(), need, hk.current_stream_ptr(dev))
-    _lib.check(st, "fp8_linear")
-    return y
+    raise ValueError(f"bias must be {out_dtype} [{n}] on {dev}, got {bias.dtype} {list(bias.shape)} on {bias.device}")

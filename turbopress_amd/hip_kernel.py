@@ -32,11 +32,14 @@ def _has_hip() -> bool:
 HAS_HIP: bool = _has_hip()
 
 
+# The raw handle of a device index's current stream.  (torch.cuda.current_stream
+# builds a Stream object: 2.1 us of every call against 0.1.)
+raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
 def current_stream_ptr(device: torch.device | None = None) -> int:
-    # (the raw handle: torch.cuda.current_stream builds a Stream object, 2.1 us
-    # of every call against 0.1)
     index = None if device is None else device.index
-    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if index is None else index)
+    return raw_stream(torch.cuda.current_device() if index is None else index)
 
 
 def _require_cuda(t: Tensor, name: str) -> None:
@@ -213,7 +216,7 @@ def shared_workspace(device, nbytes: int) -> Tensor:
     least `nbytes` long (allocated or grown on first need)."""
     dev = torch.device(device)
     index = dev.index if dev.index is not None else torch.cuda.current_device()
-    stream = torch._C._cuda_getCurrentRawStream(index)
+    stream = raw_stream(index)
     key = (index, stream)
     ws = _WORKSPACES.get(key)
     if ws is not None and ws.numel() >= nbytes:

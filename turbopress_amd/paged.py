@@ -15,6 +15,7 @@ lengths from one store.  Inference only: no gradient flows through.
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 
 import torch
@@ -22,6 +23,7 @@ from torch import Tensor
 
 from turbopress_amd import _lib
 from turbopress_amd import hip_kernel as hk
+from turbopress_amd.hip_kernel import raw_stream as _raw_stream
 from turbopress_amd.norm import DTYPE_CODES
 
 __all__ = ["rotary_frequencies", "rotary_table", "rotary", "rotary_append", "paged_attention"]
@@ -97,90 +99,81 @@ def _strides(t: Tensor):
     return got
 
 
-def _heads(t: Tensor, name: str, like: Tensor | None = None) -> Tensor:
-    """t [tokens, heads, d] with contiguous columns, checked against `like`."""
-    if not t.is_cuda:
-        raise RuntimeError(f"{name} must be a CUDA (ROCm) tensor; turbopress_amd has no CPU path")
-    if t.dim() != 3:
-        raise ValueError(f"{name} must be [tokens, heads, head_dim], got {list(t.shape)}")
-    if like is not None and (t.dtype != like.dtype or t.device != like.device or t.shape[0] != like.shape[0]
-                             or t.shape[2] != like.shape[2]):
-        raise ValueError(f"{name} must be {like.dtype} [{like.shape[0]}, heads, {like.shape[2]}] on {like.device}, "
-                         f"got {t.dtype} {list(t.shape)} on {t.device}")
+def _expect(ok: bool, name: str, t, what: str) -> None:
+    if not ok:
+        got = "None" if t is None else f"{t.dtype} {list(t.shape)} on {t.device}"
+        raise ValueError(f"{name} must be {what}, got {got}")
+
+
+def _refuse(q, k, v, table, positions, k_cache, v_cache, block_table, sequences, lengths=None) -> None:
+    """Raise for the first argument that is not as the entry points take it."""
+    if not q.is_cuda:
+        raise RuntimeError("q must be a CUDA (ROCm) tensor; turbopress_amd has no CPU path")
+    _expect(q.dim() == 3, "q", q, "[tokens, heads, head_dim]")
+    dt, dev, (tokens, heads, d) = q.dtype, q.device, q.shape
+    _expect(dt in DTYPE_CODES and (lengths is None or dt != torch.float32), "q", q,
+            "fp16 or bf16" if lengths is not None else "fp16, bf16 or fp32")
+    for name, t in (("k", k), ("v", v)):
+        if t is not None:
+            _expect(t.dtype == dt and t.device == dev and t.dim() == 3 and t.shape[0] == tokens and t.shape[2] == d and
+                    (k is None or t.shape == k.shape), name, t, f"{dt} [{tokens}, kv heads, {d}] on {dev}, k like v")
+    if lengths is None:
+        _expect(table.dtype == torch.float32 and table.device == dev and table.dim() == 2 and table.is_contiguous(), "table",
+                table, f"contiguous fp32 [positions, rotary_dim] on {dev}")
+        rd = table.shape[1]
+        if d % 2 or rd < 2 or rd % 2 or rd > d:
+            raise ValueError(f"head_dim {d} and rotary_dim {rd} must be even, with 2 <= rotary_dim <= head_dim")
+        _expect(positions.dtype == torch.int64 and positions.device == dev and positions.shape == (tokens,), "positions",
+                positions, f"int64 [{tokens}] on {dev}")
+    for name, c in (("k_cache", k_cache), ("v_cache", v_cache)):
+        if c is not None:
+            _expect(c.dtype == dt and c.device == dev and c.dim() == 4 and c.stride(3) == 1 and c.shape[3] == d and
+                    c.shape == k_cache.shape and (k is None or c.shape[2] == k.shape[1]), name, c,
+                    f"{dt} [pages, page_size, kv heads, {d}] on {dev} with contiguous columns, both caches alike")
+    if block_table is not None:
+        _expect(block_table.dtype == torch.int32 and block_table.device == dev and block_table.dim() == 2 and
+                block_table.is_contiguous(), "block_table", block_table, f"contiguous int32 [sequences, width] on {dev}")
+        if sequences is not None:
+            _expect(sequences.dtype == torch.int32 and sequences.device == dev and sequences.shape == (tokens,), "sequences",
+                    sequences, f"int32 [{tokens}] on {dev}")
+        elif block_table.shape[0] < tokens or (lengths is not None and block_table.shape[0] != tokens):
+            raise ValueError(f"block_table has {block_table.shape[0]} rows for {tokens} tokens of as many sequences")
+    if lengths is not None:
+        _expect(lengths.dtype == torch.int32 and lengths.device == dev and lengths.shape == (tokens,), "lengths", lengths,
+                f"int32 [{tokens}] on {dev}")
+        if d % 8 or not 8 <= d <= 256 or heads < 1 or k_cache.shape[2] < 1 or heads % k_cache.shape[2]:
+            raise ValueError(f"head_dim {d} must be a multiple of 8 up to 256 and {heads} query heads a multiple of "
+                             f"the caches' {k_cache.shape[2]}")
+    raise ValueError("arguments do not belong together")
+
+
+def _columns(t: Tensor) -> Tensor:
     return t if t.stride(2) == 1 else t.contiguous()
 
 
-def _check_cache(k_cache: Tensor, v_cache: Tensor, block_table: Tensor, like: Tensor) -> None:
-    for name, c in (("k_cache", k_cache), ("v_cache", v_cache)):
-        if c.dim() != 4 or c.dtype != like.dtype or c.device != like.device or c.stride(3) != 1 \
-                or c.shape[3] != like.shape[2]:
-            raise ValueError(f"{name} must be {like.dtype} [pages, page_size, kv heads, {like.shape[2]}] on "
-                             f"{like.device} with contiguous columns, got {c.dtype} {list(c.shape)} on {c.device}")
-    if k_cache.shape != v_cache.shape:
-        raise ValueError(f"k_cache and v_cache differ in shape: {list(k_cache.shape)} and {list(v_cache.shape)}")
-    if block_table.dim() != 2 or block_table.dtype != torch.int32 or block_table.device != like.device \
-            or not block_table.is_contiguous():
-        raise ValueError(f"block_table must be contiguous int32 [sequences, width] on {like.device}, "
-                         f"got {block_table.dtype} {list(block_table.shape)} on {block_table.device}")
+def _turn(q: Tensor, k: Tensor | None, table: Tensor, positions: Tensor) -> tuple:
+    """(type code, device index, tokens, heads, d, rotary_dim) of arguments that
+    rotary positions take.  (Small calls are bound by the host: the checks
+    compare as little as they can; the words are found where one fails.)"""
+    code, index = DTYPE_CODES.get(q.dtype), q.get_device()
+    if q.dim() == 3 and table.dim() == 2:
+        tokens, hq, d = q.shape
+        rd = table.shape[1]
+        if code is not None and index >= 0 and table.dtype is torch.float32 and table.get_device() == index \
+                and table.is_contiguous() and 2 <= rd <= d and not (d | rd) & 1 and positions.dtype is torch.int64 \
+                and positions.get_device() == index and positions.shape == (tokens,) and (
+                    k is None or (k.dtype is q.dtype and k.get_device() == index and k.dim() == 3 and k.shape[0] == tokens
+                                  and k.shape[2] == d)):
+            return code, index, tokens, hq, d, rd
+    _refuse(q, k, None, table, positions, None, None, None, None)
 
 
-def _rotary(q, k, v, table, positions, k_cache, v_cache, block_table, sequences, interleaved, what):
-    q = _heads(q, "q")
-    code = DTYPE_CODES.get(q.dtype)
-    if code is None:
-        raise ValueError(f"q must be fp16, bf16 or fp32, got {q.dtype}")
-    tokens, hq, d = q.shape
-    dev = q.device
-    if table.dtype != torch.float32 or table.dim() != 2 or table.device != dev or not table.is_contiguous():
-        raise ValueError(f"table must be contiguous fp32 [positions, rotary_dim] on {dev}, "
-                         f"got {table.dtype} {list(table.shape)} on {table.device}")
-    rd = table.shape[1]
-    if d % 2 or rd < 2 or rd % 2 or rd > d:
-        raise ValueError(f"head_dim {d} and rotary_dim {rd} must be even, with 2 <= rotary_dim <= head_dim")
-    if positions.shape != (tokens,) or positions.dtype != torch.int64 or positions.device != dev:
-        raise ValueError(f"positions must be int64 [{tokens}] on {dev}, "
-                         f"got {positions.dtype} {list(positions.shape)} on {positions.device}")
-    positions = positions.contiguous()
-    hk_ = 0
-    k_out = None
-    kp = ks0 = ks1 = vp = vs0 = vs1 = kc = vc = 0
-    kcp = vcp = btp = sp = n_pages = width = n_seq = 0
-    page_size = 1
-    if k is not None:
-        k = _heads(k, "k", q)
-        hk_ = k.shape[1]
-        kp, (ks0, ks1, _) = k.data_ptr(), k.stride()
-    if k_cache is not None:
-        v = _heads(v, "v", k)
-        if v.shape != k.shape:
-            raise ValueError(f"k and v differ in shape: {list(k.shape)} and {list(v.shape)}")
-        _check_cache(k_cache, v_cache, block_table, q)
-        if k_cache.shape[2] != hk_:
-            raise ValueError(f"the caches hold {k_cache.shape[2]} heads, k has {hk_}")
-        if sequences is not None:
-            if sequences.shape != (tokens,) or sequences.dtype != torch.int32 or sequences.device != dev:
-                raise ValueError(f"sequences must be int32 [{tokens}] on {dev}, "
-                                 f"got {sequences.dtype} {list(sequences.shape)} on {sequences.device}")
-            sequences = sequences.contiguous()
-            sp = sequences.data_ptr()
-        elif tokens > block_table.shape[0]:
-            raise ValueError(f"{tokens} tokens without sequences need as many rows of block_table, "
-                             f"got {block_table.shape[0]}")
-        vp, (vs0, vs1, _) = v.data_ptr(), v.stride()
-        kcp, vcp, btp = k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr()
-        kc, vc = _strides(k_cache), _strides(v_cache)
-        n_pages, page_size = k_cache.shape[0], k_cache.shape[1]
-        n_seq, width = block_table.shape
-    elif k is not None:
-        k_out = torch.empty(tokens, hk_, d, dtype=q.dtype, device=dev)
-    q_out = torch.empty(tokens, hq, d, dtype=q.dtype, device=dev)
-    st = _lib.lib().tp_rotary(
-        code, tokens, hq, hk_, d, rd, int(interleaved), q.data_ptr(), q.stride(0), q.stride(1), kp, ks0, ks1,
-        table.data_ptr(), table.shape[0], positions.data_ptr(), q_out.data_ptr(),
-        0 if k_out is None else k_out.data_ptr(), vp, vs0, vs1, kcp, kc or None, vcp, vc or None, n_pages, page_size, btp,
-        width, n_seq, sp, hk.current_stream_ptr(dev))
-    _lib.check(st, what)
-    return q_out, k_out
+def _cached(k_cache: Tensor, v_cache: Tensor, block_table: Tensor, q: Tensor, index: int, d: int) -> bool:
+    shape = k_cache.shape
+    return (k_cache.dtype is q.dtype and v_cache.dtype is q.dtype and len(shape) == 4 and shape[3] == d
+            and v_cache.shape == shape and k_cache.stride(3) == 1 and v_cache.stride(3) == 1
+            and k_cache.get_device() == index and v_cache.get_device() == index and block_table.dtype is torch.int32
+            and block_table.get_device() == index and block_table.dim() == 2 and block_table.is_contiguous())
 
 
 def rotary(q: Tensor, k: Tensor | None, table: Tensor, positions: Tensor, interleaved: bool = False) -> tuple:
@@ -192,7 +185,25 @@ def rotary(q: Tensor, k: Tensor | None, table: Tensor, positions: Tensor, interl
     [tokens].  Pairs are columns (i, i + rotary_dim / 2), or (2 i, 2 i + 1) where
     interleaved.  A negative position is padding and gives zeros; one past the
     table gives NaN."""
-    return _rotary(q, k, None, table, positions, None, None, None, None, interleaved, "rotary")
+    code, index, tokens, hq, d, rd = _turn(q, k, table, positions)
+    q = _columns(q)
+    q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    heads, kp, k_token, k_head, k_out = 0, 0, 0, 0, None
+    if k is not None:
+        k = _columns(k)
+        heads, kp = k.shape[1], k.data_ptr()
+        k_token, k_head, _ = k.stride()
+        k_out = torch.empty_like(k, memory_format=torch.contiguous_format)
+    if not positions.is_contiguous():
+        positions = positions.contiguous()
+    q_token, q_head, _ = q.stride()
+    st = _lib.lib().tp_rotary(code, tokens, hq, heads, d, rd, interleaved, q.data_ptr(), q_token, q_head, kp, k_token, k_head,
+                              table.data_ptr(), table.shape[0], positions.data_ptr(), q_out.data_ptr(),
+                              0 if k_out is None else k_out.data_ptr(), 0, 0, 0, 0, None, 0, None, 0, 1, 0, 0, 0, 0,
+                              _raw_stream(index))
+    if st:
+        _lib.check(st, "rotary")
+    return q_out, k_out
 
 
 def rotary_append(q: Tensor, k: Tensor, v: Tensor, table: Tensor, positions: Tensor, k_cache: Tensor, v_cache: Tensor,
@@ -206,7 +217,62 @@ def rotary_append(q: Tensor, k: Tensor, v: Tensor, table: Tensor, positions: Ten
     sequence that does not exist write nothing."""
     if k is None or v is None or k_cache is None or v_cache is None or block_table is None:
         raise ValueError("rotary_append needs k, v, k_cache, v_cache and block_table")
-    return _rotary(q, k, v, table, positions, k_cache, v_cache, block_table, sequences, interleaved, "rotary_append")[0]
+    code, index, tokens, hq, d, rd = _turn(q, k, table, positions)
+    if v.dtype is not q.dtype or v.get_device() != index or v.shape != k.shape \
+            or not _cached(k_cache, v_cache, block_table, q, index, d) or k_cache.shape[2] != k.shape[1] \
+            or (sequences is None and tokens > block_table.shape[0]) or (sequences is not None and (
+                sequences.dtype is not torch.int32 or sequences.shape != (tokens,) or sequences.get_device() != index)):
+        _refuse(q, k, v, table, positions, k_cache, v_cache, block_table, sequences)
+    q, k, v = _columns(q), _columns(k), _columns(v)
+    q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    if not positions.is_contiguous():
+        positions = positions.contiguous()
+    if sequences is not None and not sequences.is_contiguous():
+        sequences = sequences.contiguous()
+    pages, page_size, heads, _ = k_cache.shape
+    rows, width = block_table.shape
+    q_token, q_head, _ = q.stride()
+    k_token, k_head, _ = k.stride()
+    v_token, v_head, _ = v.stride()
+    st = _lib.lib().tp_rotary(code, tokens, hq, heads, d, rd, interleaved, q.data_ptr(), q_token, q_head, k.data_ptr(),
+                              k_token, k_head, table.data_ptr(), table.shape[0], positions.data_ptr(), q_out.data_ptr(), 0,
+                              v.data_ptr(), v_token, v_head, k_cache.data_ptr(), _strides(k_cache), v_cache.data_ptr(),
+                              _strides(v_cache), pages, page_size, block_table.data_ptr(), width, rows,
+                              0 if sequences is None else sequences.data_ptr(), _raw_stream(index))
+    if st:
+        _lib.check(st, "rotary_append")
+    return q_out
+
+
+# Workspaces of paged_attention by (device index, stream): a buffer whose first
+# bytes are the counters, zero between calls, and how many those are.  Calls in
+# stream order share one; a graph's capture makes its own (the buffers below are
+# a running program's, the graph's have to last as long as it does).
+_WORKSPACES: dict = {}
+_COUNTERS = 1 << 16  # bytes of counters at least
+
+
+@functools.lru_cache(maxsize=1024)
+def _needs(index: int, batch: int, hq: int, hkv: int, d: int) -> tuple:
+    """(workspace bytes, counter bytes) of a call on a device."""
+    lib = _lib.lib()
+    return (lib.tp_paged_attention_workspace_bytes(batch, hq, hkv, d), lib.tp_paged_attention_counter_bytes(batch, hq, hkv, d))
+
+
+def _workspace(index: int, stream: int, need: int, count: int) -> tuple:
+    """(workspace pointer, counters pointer, buffers to hold until the launch)."""
+    if torch.cuda.is_current_stream_capturing():
+        dev = torch.device("cuda", index)
+        ws = torch.empty(need, dtype=torch.uint8, device=dev)
+        counters = hk.shared_workspace(dev, count)  # zero between launches, as the split-K sums' counters
+        return ws.data_ptr(), counters.data_ptr(), (ws, counters)
+    got = _WORKSPACES.get((index, stream))
+    if got is None or got[1] < count or got[0].numel() - got[1] < need:
+        counts = max(_COUNTERS, -(-count // 256) * 256, 0 if got is None else got[1])
+        size = max(need, 0 if got is None else got[0].numel() - got[1])
+        got = _WORKSPACES[(index, stream)] = (torch.zeros(counts + size, dtype=torch.uint8, device=torch.device("cuda", index)), counts)
+    p = got[0].data_ptr()
+    return p + got[1], p, got
 
 
 def paged_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, block_table: Tensor, lengths: Tensor,
@@ -221,40 +287,36 @@ def paged_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, block_table: Te
     The new token's own key and value are read from the cache like the others
     (``rotary_append`` first).  Several new tokens of one sequence are several
     rows of q with that sequence's row of block_table and growing lengths."""
-    q = _heads(q, "q")
-    b, hq, d = q.shape
-    dev = q.device
-    if q.dtype not in (torch.float16, torch.bfloat16):
-        raise ValueError(f"q must be fp16 or bf16, got {q.dtype}")
-    _check_cache(k_cache, v_cache, block_table, q)
-    hkv = k_cache.shape[2]
-    if d % 8 or not 8 <= d <= 256 or hq < 1 or hkv < 1 or hq % hkv:
-        raise ValueError(f"head_dim {d} must be a multiple of 8 up to 256 and {hq} query heads a multiple of {hkv}")
-    if block_table.shape[0] != b:
-        raise ValueError(f"block_table has {block_table.shape[0]} rows, expected {b}")
-    if lengths.shape != (b,) or lengths.dtype != torch.int32 or lengths.device != dev:
-        raise ValueError(f"lengths must be int32 [{b}] on {dev}, "
-                         f"got {lengths.dtype} {list(lengths.shape)} on {lengths.device}")
+    index = q.get_device()
+    code = DTYPE_CODES.get(q.dtype, _lib.TP_F32)
     if window < 0:
         raise ValueError(f"window must be 0 (none) or positive, got {window}")
-    if (q.data_ptr() | 2 * q.stride(0) | 2 * q.stride(1)) & 15:
-        q = q.contiguous()
-        if q.data_ptr() & 15:
-            q = q.clone()
-    lengths = lengths.contiguous()
-    out = torch.empty(b, hq, d, dtype=q.dtype, device=dev)
-    lib = _lib.lib()
+    if q.dim() != 3 or index < 0 or code == _lib.TP_F32 or not _cached(k_cache, v_cache, block_table, q, index, q.shape[2]) \
+            or block_table.shape[0] != q.shape[0] or lengths.dtype is not torch.int32 or lengths.shape != q.shape[:1] \
+            or lengths.get_device() != index:
+        _refuse(q, None, None, None, None, k_cache, v_cache, block_table, None, lengths)
+    b, hq, d = q.shape
+    pages, page_size, hkv, _ = k_cache.shape
+    if d % 8 or not 8 <= d <= 256 or hq < 1 or hkv < 1 or hq % hkv:
+        _refuse(q, None, None, None, None, k_cache, v_cache, block_table, None, lengths)
+    q = _columns(q)
+    q_row, q_head, _ = q.stride()
+    qp = q.data_ptr()
+    if (qp | q_row << 1 | q_head << 1) & 15:  # (a row of 16-byte pieces)
+        q = q.clone(memory_format=torch.contiguous_format)
+        q_row, q_head, qp = hq * d, d, q.data_ptr()
+    if not lengths.is_contiguous():
+        lengths = lengths.contiguous()
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
     if b == 0:
         return out
-    need = lib.tp_paged_attention_workspace_bytes(b, hq, hkv, d)
-    ws = torch.empty(need, dtype=torch.uint8, device=dev)
-    count = lib.tp_paged_attention_counter_bytes(b, hq, hkv, d)
-    counters = hk.shared_workspace(dev, count)  # zero between launches, as the split-K sums' counters
-    st = lib.tp_paged_attention(
-        DTYPE_CODES[q.dtype], b, hq, hkv, d, q.data_ptr(), q.stride(0), q.stride(1), k_cache.data_ptr(),
-        _strides(k_cache), v_cache.data_ptr(), _strides(v_cache), k_cache.shape[0], k_cache.shape[1],
-        block_table.data_ptr(), block_table.shape[1], lengths.data_ptr(),
-        1.0 / math.sqrt(d) if scale is None else scale, window, out.data_ptr(),
-        ws.data_ptr(), need, counters.data_ptr(), count, hk.current_stream_ptr(dev))
-    _lib.check(st, "paged_attention")
+    stream = _raw_stream(index)
+    need, count = _needs(index, b, hq, hkv, d)
+    ws, counters, _held = _workspace(index, stream, need, count)
+    st = _lib.lib().tp_paged_attention(
+        code, b, hq, hkv, d, qp, q_row, q_head, k_cache.data_ptr(), _strides(k_cache), v_cache.data_ptr(), _strides(v_cache),
+        pages, page_size, block_table.data_ptr(), block_table.shape[1], lengths.data_ptr(),
+        d ** -0.5 if scale is None else scale, window, out.data_ptr(), ws, need, counters, count, stream)
+    if st:
+        _lib.check(st, "paged_attention")
     return out
