@@ -12,6 +12,7 @@
 #include "tp_ops_common.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace tp {
 
@@ -25,6 +26,7 @@ struct NormArgs {
   void* h;
   int64_t x_outer, x_inner, r_outer, r_inner, ldc, rows;
   int inner, d, nvec, nblocks, waves_per_row;
+  int large;  // the inputs are past the caches' size
   float eps;
 };
 
@@ -34,9 +36,9 @@ constexpr float kE4m3Max = 448.0f;
 constexpr float kLeastScale = 0x1p-126f;
 
 // Elements [8 i, 8 i + 8) of a row of d, zeros past its end.
-template <typename T>
+template <bool ONCE = false, typename T>
 __device__ __forceinline__ Vec<T> load_row8(const T* row, int i, int d) {
-  if (8 * i + 8 <= d) return load8(row + 8 * i);
+  if (8 * i + 8 <= d) return ONCE ? load8_once(row + 8 * i) : load8(row + 8 * i);
   Vec<T> r;
 #pragma unroll
   for (int e = 0; e < 8; ++e) r.v[e] = 8 * i + e < d ? row[8 * i + e] : (T)0.0f;
@@ -46,7 +48,7 @@ __device__ __forceinline__ Vec<T> load_row8(const T* row, int i, int d) {
 template <typename T>
 __device__ __forceinline__ void store_row8(T* row, int i, int d, const Vec<T>& r) {
   if (8 * i + 8 <= d) {
-    store8(row + 8 * i, r);
+    store8_once(row + 8 * i, r);
     return;
   }
 #pragma unroll
@@ -99,8 +101,13 @@ __device__ __forceinline__ float reduce_row(float v, int wpr, float* slots) {
 }
 
 // A row per SUB lanes (SUB < 64) or per waves_per_row waves (SUB = 64), VPT
-// vectors of 8 elements per lane.
-template <typename T, int OUT, int SUB, int VPT>
+// vectors of 8 elements per lane, one row each.  What stays in registers across
+// the reduction is x and the residual as they were loaded; h is formed again
+// behind it.  (8192 x 9728 fp16: with h kept in fp32 and the weight beside it
+// 100 us, and 102 with workgroups that go on to further rows, the next one's
+// loads in flight: either leaves fewer waves to a CU, and the loads of some
+// waves have to run under the reductions and stores of others.)
+template <typename T, int OUT, bool RES, int SUB, int VPT>
 __global__ void __launch_bounds__(512) rms_norm_kernel(const NormArgs a) {
   __shared__ float slots[32];
   const int wpr = SUB < 64 ? 1 : a.waves_per_row;
@@ -110,92 +117,97 @@ __global__ void __launch_bounds__(512) rms_norm_kernel(const NormArgs a) {
   const bool live = row < a.rows;
   const int64_t rrow = live ? row : a.rows - 1;  // (idle lanes follow a row along, for the barriers)
   const T* x = static_cast<const T*>(a.x) + row_offset(rrow, a.inner, a.x_outer, a.x_inner);
+  const T* res = RES ? static_cast<const T*>(a.residual) + row_offset(rrow, a.inner, a.r_outer, a.r_inner) : nullptr;
   const T* weight = static_cast<const T*>(a.weight);
+  const int last = a.nvec - 1;  // (lanes past the row load its last vector, and add nothing)
 
-  float h[VPT][8];
-  Vec<T> xv[VPT], wv[VPT];
+  Vec<T> xv[VPT], rv[RES ? VPT : 1];
+  auto load = [&](auto once) __attribute__((always_inline)) {
 #pragma unroll
-  for (int j = 0; j < VPT; ++j)
-    if (i0 + j * lanes < a.nvec) xv[j] = load_row8(x, i0 + j * lanes, a.d);
-  if (a.residual) {
-    const T* res = static_cast<const T*>(a.residual) + row_offset(rrow, a.inner, a.r_outer, a.r_inner);
-    Vec<T> rv[VPT];
+    for (int j = 0; j < VPT; ++j) xv[j] = load_row8<decltype(once)::value>(x, min(i0 + j * lanes, last), a.d);
+    if constexpr (RES) {
 #pragma unroll
-    for (int j = 0; j < VPT; ++j)
-      if (i0 + j * lanes < a.nvec) rv[j] = load_row8(res, i0 + j * lanes, a.d);
+      for (int j = 0; j < VPT; ++j) rv[j] = load_row8<decltype(once)::value>(res, min(i0 + j * lanes, last), a.d);
+    }
+  };
+  if (a.large) load(std::true_type{});
+  else load(std::false_type{});
+  auto sum8 = [&](int j, float* h) __attribute__((always_inline)) {
 #pragma unroll
-    for (int j = 0; j < VPT; ++j)
-      if (i0 + j * lanes < a.nvec) wv[j] = load_row8(weight, i0 + j * lanes, a.d);
-#pragma unroll
-    for (int j = 0; j < VPT; ++j)
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        h[j][e] = i0 + j * lanes < a.nvec ? (float)xv[j].v[e] + (float)rv[j].v[e] : 0.0f;
-  } else {
-#pragma unroll
-    for (int j = 0; j < VPT; ++j)
-      if (i0 + j * lanes < a.nvec) wv[j] = load_row8(weight, i0 + j * lanes, a.d);
-#pragma unroll
-    for (int j = 0; j < VPT; ++j)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) h[j][e] = i0 + j * lanes < a.nvec ? (float)xv[j].v[e] : 0.0f;
-  }
-
+    for (int e = 0; e < 8; ++e) {
+      h[e] = (float)xv[j].v[e];
+      if constexpr (RES) h[e] += (float)rv[j].v[e];
+    }
+  };
   float sum = 0.0f;
 #pragma unroll
-  for (int j = 0; j < VPT; ++j)
+  for (int j = 0; j < VPT; ++j) {
+    float h[8], part = 0.0f;
+    sum8(j, h);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) sum = fmaf(h[j][e], h[j][e], sum);
+    for (int e = 0; e < 8; ++e) part = fmaf(h[e], h[e], part);
+    sum += i0 + j * lanes <= last ? part : 0.0f;
+    if (RES && a.h && live && i0 + j * lanes <= last) {
+      Vec<T> o;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) o.v[e] = (T)h[e];
+      store_row8(static_cast<T*>(a.h) + (size_t)row * a.d, i0 + j * lanes, a.d, o);
+    }
+  }
+  if (!RES && a.h && live) {  // (without a residual h is x)
+#pragma unroll
+    for (int j = 0; j < VPT; ++j)
+      if (i0 + j * lanes <= last) store_row8(static_cast<T*>(a.h) + (size_t)row * a.d, i0 + j * lanes, a.d, xv[j]);
+  }
+  Vec<T> wv[VPT];
+#pragma unroll
+  for (int j = 0; j < VPT; ++j) wv[j] = load_row8(weight, min(i0 + j * lanes, last), a.d);
   sum = reduce_row<AddOp, SUB>(sum, wpr, slots);
   const float inv = 1.0f / sqrtf(sum / (float)a.d + a.eps);
-
-  if (a.h && live) {
-    T* hr = static_cast<T*>(a.h) + (size_t)row * a.d;
+  auto norm8 = [&](int j, float* y) __attribute__((always_inline)) {
+    sum8(j, y);
 #pragma unroll
-    for (int j = 0; j < VPT; ++j)
-      if (i0 + j * lanes < a.nvec) {
-        Vec<T> o;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) o.v[e] = (T)h[j][e];
-        store_row8(hr, i0 + j * lanes, a.d, o);
-      }
-  }
-#pragma unroll
-  for (int j = 0; j < VPT; ++j)
-#pragma unroll
-    for (int e = 0; e < 8; ++e) h[j][e] = i0 + j * lanes < a.nvec ? h[j][e] * inv * (float)wv[j].v[e] : 0.0f;
+    for (int e = 0; e < 8; ++e) y[e] = y[e] * inv * (float)wv[j].v[e];
+  };
 
   if constexpr (OUT == kSame) {
-    T* y = static_cast<T*>(a.y) + (size_t)row * a.d;
+    T* yr = static_cast<T*>(a.y) + (size_t)row * a.d;
 #pragma unroll
     for (int j = 0; j < VPT; ++j)
-      if (live && i0 + j * lanes < a.nvec) {
+      if (live && i0 + j * lanes <= last) {
+        float y[8];
+        norm8(j, y);
         Vec<T> o;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) o.v[e] = (T)h[j][e];
-        store_row8(y, i0 + j * lanes, a.d, o);
+        for (int e = 0; e < 8; ++e) o.v[e] = (T)y[e];
+        store_row8(yr, i0 + j * lanes, a.d, o);
       }
   } else {
     float s_row = 0.0f;
     if constexpr (OUT == kFp8Row) {
       float m = 0.0f;
 #pragma unroll
-      for (int j = 0; j < VPT; ++j) m = MaxNanOp::of(m, max_abs8(h[j]));
+      for (int j = 0; j < VPT; ++j) {  // (the last vector again, in lanes past it, changes no maximum)
+        float y[8];
+        norm8(j, y);
+        m = MaxNanOp::of(m, max_abs8(y));
+      }
       s_row = scale_of(reduce_row<MaxNanOp, SUB>(m, wpr, slots + 16));
       if (live && i0 == 0) a.scales[row] = s_row;
     }
 #pragma unroll
     for (int j = 0; j < VPT; ++j) {
       const int i = i0 + j * lanes;
-      float s = s_row;
-      if constexpr (OUT == kFp8Block) {  // 16 lanes hold a block of 128
-        s = scale_of(reduce16<MaxNanOp>(max_abs8(h[j])));
-        if (live && i < a.nvec && (i & 15) == 0) a.scales[(size_t)row * a.nblocks + (i >> 4)] = s;
+      float y[8], s = s_row;
+      norm8(j, y);
+      if constexpr (OUT == kFp8Block) {  // 16 lanes hold a block of 128 (of its vectors, lanes past the row the last)
+        s = scale_of(reduce16<MaxNanOp>(max_abs8(y)));
+        if (live && i <= last && (i & 15) == 0) a.scales[(size_t)row * a.nblocks + (i >> 4)] = s;
       }
       const float is = 1.0f / s;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) h[j][e] *= is;
-      if (live && i < a.nvec) *reinterpret_cast<u32x2*>(a.codes + (size_t)row * a.ldc + 8 * i) = to_e4m3(h[j]);
+      for (int e = 0; e < 8; ++e) y[e] *= is;
+      if (live && i <= last) __builtin_nontemporal_store(to_e4m3(y), reinterpret_cast<u32x2*>(a.codes + (size_t)row * a.ldc + 8 * i));
     }
   }
 }
@@ -307,6 +319,11 @@ inline NormPlan norm_plan(int64_t rows, int nvec, int cus) {
 template <typename T, int OUT>
 int launch_norm(const NormArgs& a0, hipStream_t s) {
   NormArgs a = a0;
+  // Loads past the caches from 128 MB of inputs, half of what the memory side
+  // caches: 8191 x 9727 fp16 76 us against 82, 8192 x 9728 64 against 77; what
+  // the step before has just written is better read from there: 16384 x 1024
+  // with a residual 25.9 against 21.4, 2048 x 2560 12.7 against 9.4.
+  a.large = a.rows * a.d * (int64_t)sizeof(T) * (a.residual ? 2 : 1) >= (128 << 20);
   const NormPlan p = norm_plan(a.rows, a.nvec, device_cu_count());
   if (p.vpt == 0) {
     hipLaunchKernelGGL((rms_norm_long_kernel<T, OUT>), dim3((uint32_t)a.rows), dim3(1024), 0, s, a);
@@ -317,7 +334,11 @@ int launch_norm(const NormArgs& a0, hipStream_t s) {
   const int lanes = p.sub < 64 ? p.sub : 64 * p.waves;
   const int per = threads / lanes;
   const dim3 grid((uint32_t)((a.rows + per - 1) / per)), block(threads);
-#define TP_NORM(SUB, V) hipLaunchKernelGGL((rms_norm_kernel<T, OUT, SUB, V>), grid, block, 0, s, a)
+#define TP_NORM(SUB, V)                                                                              \
+  do {                                                                                               \
+    if (a.residual) hipLaunchKernelGGL((rms_norm_kernel<T, OUT, true, SUB, V>), grid, block, 0, s, a); \
+    else hipLaunchKernelGGL((rms_norm_kernel<T, OUT, false, SUB, V>), grid, block, 0, s, a);           \
+  } while (0)
   if (p.sub == 16) TP_NORM(16, 1);
   else if (p.sub == 32) TP_NORM(32, 1);
   else if (p.vpt == 1) TP_NORM(64, 1);

@@ -31,6 +31,26 @@ __device__ __forceinline__ void store8(T* p, const Vec<T>& r) {
   __builtin_memcpy(p, &r, sizeof(r));
 }
 
+// The same past the caches: of what is read once and is too large to be in them,
+// and of what is written once.
+typedef u32x4 u32x4_any __attribute__((aligned(1)));
+template <typename T>
+__device__ __forceinline__ Vec<T> load8_once(const T* p) {
+  u32x4 w[sizeof(T) / 2];
+#pragma unroll
+  for (int i = 0; i < (int)sizeof(T) / 2; ++i) w[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4_any*>(p) + i);
+  Vec<T> r;
+  __builtin_memcpy(&r, w, sizeof(r));
+  return r;
+}
+template <typename T>
+__device__ __forceinline__ void store8_once(T* p, const Vec<T>& r) {
+  u32x4 w[sizeof(T) / 2];
+  __builtin_memcpy(w, &r, sizeof(r));
+#pragma unroll
+  for (int i = 0; i < (int)sizeof(T) / 2; ++i) __builtin_nontemporal_store(w[i], reinterpret_cast<u32x4_any*>(p) + i);
+}
+
 template <int CTRL>
 __device__ __forceinline__ float dpp(float v) {
   return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), CTRL, 0xF, 0xF, false));
