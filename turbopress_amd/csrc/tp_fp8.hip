@@ -10,12 +10,11 @@
 // over blocks are in a fixed order.
 //
 // Few rows (fp8_takes_rows): every weight is read once, straight into operand
-// registers (bound by HBM: 151936 x 2560, 1 row, 66.8 us = 5.8 TB/s).  More:
-// tiles of both operands are staged in LDS by loads that bypass the registers
-// (bound by the matrix cores and LDS: 4096 x 8192 x 8192 257 us = 2.1 PFLOP/s,
-// where the instructions alone, without staging, sums and LDS reads, ran at
-// 3.6; or by the chain of a tile's blocks, 0.5 us each: 199 x 4096 x 2560
-// 11.6 us).
+// registers (bound by HBM: 151936 x 2560, 1 row, 66 us = 5.9 TB/s).  More: tiles
+// of both operands are staged in LDS by loads that bypass the registers, bound
+// by the matrix cores, LDS and the sums' FMAs together (4096 x 8192 x 8192 256 us
+// = 2.15 PFLOP/s; the instructions alone, no staging, sums or LDS reads, ran at
+// 3.6) or, of few tiles, by the chain of a tile's blocks (0.3 us each).
 #include "tp_ops_common.h"
 
 #include <algorithm>
@@ -216,21 +215,24 @@ __global__ void __launch_bounds__(NC == 1 ? 1024 : 512) fp8_rows_kernel(const Fp
 // ---------------------------------------------------------------------------
 // more rows
 // ---------------------------------------------------------------------------
-// A workgroup of WN x WM waves, a wave TN x TM blocks of 16 weight rows x 16
-// activation rows.  LDS holds kBufs stages of 128 columns; a row's eight 16-byte
+// A workgroup of WK teams of WN x WM waves, a wave TN x TM blocks of 16 weight
+// rows x 16 activation rows; the teams share the columns' blocks, each in LDS of
+// its own, and their sums are joined at the end.  A team's LDS holds kBufs stages of 128 columns; a row's eight 16-byte
 // chunks are stored in the order c ^ (row & 7), so that the rows that a lane
 // group reads at one chunk fall on distinct banks (a load to LDS writes lane
 // after lane, so the lanes' global addresses are permuted).
-template <int WN, int WM, int TN, int TM>
+template <int WN, int WM, int TN, int TM, int WK>
 struct TileShape {
-  static constexpr int kWaves = WN * WM;
+  static constexpr int kWaves = WN * WM;  // of a team
   static constexpr int kBN = 16 * WN * TN, kBM = 16 * WM * TM;
   static constexpr int kStage = (kBN + kBM) * 128;
-  static constexpr int kBufs = 4 * kStage <= 64 * 1024 ? 4 : 3 * kStage <= 72 * 1024 ? 3 : 2;
-  // scales of 8 stages, [row][8] activations' and [8][8] weights': of those in
-  // use, those arriving, and those that stages ahead of the block call for
-  static constexpr int kScales = kBufs * kStage, kScaleBuf = (kBM + 8) * 8 * 4;
-  static constexpr int kLds = kScales + 3 * kScaleBuf;
+  static constexpr int kBufs = WK <= 2 && 4 * kStage <= 64 * 1024 ? 4 : WK == 1 && 3 * kStage <= 72 * 1024 ? 3 : 2;
+  // scales of kSB stages, [row][kSB] activations' and [64 / kSB][kSB] weights': of
+  // those in use, those arriving, and those that stages ahead of the block call for
+  static constexpr int kScales = kBufs * kStage;
+  static constexpr int kSB = WK * (kScales + 3 * (kBM * 32 + 256)) <= 160 * 1024 ? 8 : 4;
+  static constexpr int kScaleBuf = kBM * 4 * kSB + 256;
+  static constexpr int kTeam = kScales + 3 * kScaleBuf, kLds = WK * kTeam;  // bytes of a team, of the workgroup
   static constexpr int kWLoads = kBN / 8 / kWaves, kALoads = kBM / 8 / kWaves;  // 1 KB pieces (8 rows) of a wave
   static constexpr int kLoads = kWLoads + kALoads + 2;
   static_assert(kBN % (8 * kWaves) == 0 && kBM % (8 * kWaves) == 0 && kBM % 64 == 0 && 64 * kWaves >= kBM && kLds <= 160 * 1024, "");
@@ -245,14 +247,21 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_rsrc(const void* p, int64
   return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, (uint32_t)std::min<int64_t>(bytes, 0xfffffff0), 0x00020000);
 }
 
-template <typename T, int WN, int WM, int TN, int TM>
-__global__ void __launch_bounds__(64 * WN * WM, 2) fp8_tile_kernel(const Fp8Args g) {
-  using S = TileShape<WN, WM, TN, TM>;
+constexpr int kLate = 3;  // products between one and its sums
+
+template <typename T, int WN, int WM, int TN, int TM, int WK>
+__global__ void __launch_bounds__(64 * WN * WM * WK, WK > 2 ? 1 : 2) fp8_tile_kernel(const Fp8Args g) {
+  using S = TileShape<WN, WM, TN, TM, WK>;
   using Op = Operand<sizeof(T) == 4>;
   constexpr int BN = S::kBN, BM = S::kBM, NBUF = S::kBufs;
   extern __shared__ __attribute__((aligned(16))) char fp8_lds[];
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int lane = threadIdx.x & 63, wave0 = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int team = WK == 1 ? 0 : wave0 / S::kWaves, wave = WK == 1 ? wave0 : wave0 % S::kWaves;
   const int wn = wave % WN, wm = wave / WN;
+  char* const lds = fp8_lds + team * S::kTeam;
+  // the team's blocks: b0 .. b0 + blocks - 1, the last team's up to the last one
+  // (blocks below 0, of the first teams, are zeros)
+  const int blocks = (g.kb + WK - 1) / WK, b0 = g.kb - (WK - team) * blocks;
 
   // each XCD (blockIdx % 8) takes a contiguous run of tiles, activation tiles
   // fastest: they share a weight tile in its L2
@@ -275,31 +284,33 @@ __global__ void __launch_bounds__(64 * WN * WM, 2) fp8_tile_kernel(const Fp8Args
   const uint32_t wv = (uint32_t)(8 * wave * S::kWLoads + lrow) * (uint32_t)g.ldw + chunk;
   const uint32_t av = (uint32_t)(8 * wave * S::kALoads + lrow) * (uint32_t)g.lda + chunk;
   // Scales go to LDS too (a scalar load would make every LDS wait a full one),
-  // those of 8 blocks together: a load takes 8 rows x 8 blocks, 32 bytes of a
-  // row (64 rows x 1 block at a time, 64 pieces of memory in one load, took as
-  // long as all operands).  With stage 8 q + j goes the j-th eighth of the
-  // scales of blocks 8 q + 8 .. + 15.
-  const uint32_t srow = 8 * (wave % (BM / 64)) + (lane >> 3);  // in an eighth
-  const uint32_t sav = srow * (uint32_t)g.kb * 4u + (lane & 7) * 4u, swv = (lane >> 3) * (uint32_t)g.kb * 4u + (lane & 7) * 4u;
-  auto stage_scales = [&](int j, int b, int ring) __attribute__((always_inline)) {  // blocks b .. b + 7
-    char* p = fp8_lds + S::kScales + ring * S::kScaleBuf;
-    // (blocks past the last: not loaded, nor used)
-    const uint32_t past = b + (int)(lane & 7) >= g.kb ? 0x80000000u : 0u;
-    const uint32_t soff = 4u * min(b, g.kb - 1);
+  // those of SB = 8 (4) blocks together: a load takes 8 rows x 8 blocks, 32 bytes
+  // of a row (64 rows x 1 block at a time, 64 pieces of memory in one load, took
+  // as long as all operands).  With stage SB q + j goes the j-th SB-th part of
+  // the scales of blocks SB (q + 1) .. SB (q + 1) + SB - 1.
+  constexpr int SB = S::kSB, kRows = 64 / SB;  // rows of a load
+  const uint32_t srow = kRows * (wave % (BM / 64)) + lane / SB;
+  const uint32_t sav = srow * (uint32_t)g.kb * 4u, swv = (lane / SB) * (uint32_t)g.kb * 4u;
+  // (j and i count the team's blocks)
+  auto stage_scales = [&](int j, int i, int ring) __attribute__((always_inline)) {  // its blocks i .. i + SB - 1
+    char* p = lds + S::kScales + ring * S::kScaleBuf;
+    const int b = b0 + i + (int)(lane % SB);
+    // (blocks before the first and past the last: zeros)
+    const uint32_t at = (uint32_t)b >= (uint32_t)g.kb ? 0x80000000u : 4u * b;
     __builtin_amdgcn_raw_ptr_buffer_load_lds(
-        sars, (__attribute__((address_space(3))) void*)(p + (j * (BM / 8) + 8 * (wave % (BM / 64))) * 32), 4,
-        (sav | past) + (uint32_t)(j * (BM / 8)) * (uint32_t)g.kb * 4u, soff, 0, 0);
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(swrs, (__attribute__((address_space(3))) void*)(p + BM * 32), 4, swv | past, soff,
-                                             0, 0);
+        sars, (__attribute__((address_space(3))) void*)(p + (j * (BM / SB) + kRows * (wave % (BM / 64))) * 4 * SB), 4,
+        at + sav + (uint32_t)(j * (BM / SB)) * (uint32_t)g.kb * 4u, 0, 0, 0);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(swrs, (__attribute__((address_space(3))) void*)(p + BM * 4 * SB), 4, at + swv, 0, 0,
+                                             0);
   };
   int ring = 1;  // where the next scales go
-  auto stage = [&](int b, int buf) __attribute__((always_inline)) {
-    char* p = fp8_lds + buf * S::kStage;
-    const int bc = min(b, g.kb - 1);
-    // chunks past the columns, and stages past the last, load nothing: zeros
-    const uint32_t past = 128 * b + (int)chunk >= kr ? 0x80000000u : 0u;
-    stage_scales(b & 7, (b & ~7) + 8, ring);
-    ring = (b & 7) == 7 ? (ring == 2 ? 0 : ring + 1) : ring;
+  auto stage = [&](int i, int buf) __attribute__((always_inline)) {
+    char* p = lds + buf * S::kStage;
+    const int b = b0 + i, bc = min(max(b, 0), g.kb - 1);
+    // chunks past the columns, and stages that are not, load nothing: zeros
+    const uint32_t past = b < 0 || 128 * b + (int)chunk >= kr ? 0x80000000u : 0u;
+    stage_scales(i & (SB - 1), (i & -SB) + SB, ring);
+    ring = (i & (SB - 1)) == SB - 1 ? (ring == 2 ? 0 : ring + 1) : ring;
 #pragma unroll
     for (int x = 0; x < S::kWLoads; ++x)
       __builtin_amdgcn_raw_ptr_buffer_load_lds(
@@ -315,8 +326,8 @@ __global__ void __launch_bounds__(64 * WN * WM, 2) fp8_tile_kernel(const Fp8Args
   // anything, are zeroed (by the wave that loaded them).
   auto zero_rest = [&](int buf) __attribute__((always_inline)) {
     const int in = g.k - (128 * (g.kb - 1) + (int)chunk);  // columns of this lane's chunk
-    if (in > 0 && in < 16) {
-      char* p = fp8_lds + buf * S::kStage + lane * 16;
+    if (team == WK - 1 && in > 0 && in < 16) {
+      char* p = lds + buf * S::kStage + lane * 16;
 #pragma nounroll
       for (int x = 0; x < S::kWLoads + S::kALoads; ++x) {
         char* at = p + (x < S::kWLoads ? (wave * S::kWLoads + x) * 1024
@@ -336,55 +347,69 @@ __global__ void __launch_bounds__(64 * WN * WM, 2) fp8_tile_kernel(const Fp8Args
     op.set(i32x8{(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], (int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]});
     return op;
   };
-  f32x4 acc[TN][TM], d[2][TM];
-  float f[TM], fa[TM], fw;  // scales of the products in d; of the current block, apart
+  f32x4 acc[TN][TM], d[kLate + 1];
+  // Scales: of the products in d; of the current block, apart.  A wave's weight
+  // rows lie in one block of 128 where 16 TN divides 128, else in up to 3, whose
+  // first ends at the wave's row `edge`.
+  constexpr bool kOneBlock = 128 % (16 * TN) == 0;
+  constexpr int kWS = kOneBlock ? 1 : 3;
+  const int wrow = (int)(n0 & 127) + wn * 16 * TN, wblk = kOneBlock ? (wn * 16 * TN) >> 7 : wrow >> 7;
+  const int edge = 128 - (wrow & 127);
+  float f[TM], fa[TM], fw[kWS];
 #pragma unroll
   for (int t = 0; t < TN; ++t)
 #pragma unroll
     for (int c = 0; c < TM; ++c) acc[t][c] = f32x4{0, 0, 0, 0};
 #pragma unroll
-  for (int c = 0; c < TM; ++c) d[1][c] = f32x4{0, 0, 0, 0}, f[c] = 0.0f;
-  constexpr int kAhead = TN < 4 ? TN : 4;  // weight operands in registers: read three groups ahead
+  for (int x = 0; x <= kLate; ++x) d[x] = f32x4{0, 0, 0, 0};
+#pragma unroll
+  for (int c = 0; c < TM; ++c) f[c] = 0.0f;
+  constexpr int kAhead = TN * TM >= 40 ? 2 : TN < 4 ? TN : 4;  // weight operands in registers, read kAhead - 1 groups ahead
   Op a[TM], w[kAhead];
   // what a block's first products need
-  auto first = [&](int b, int buf, int ring) __attribute__((always_inline)) {
-    const char* p = fp8_lds + buf * S::kStage;
-    const float* sl = reinterpret_cast<const float*>(fp8_lds + S::kScales + ring * S::kScaleBuf) + (b & 7);
+  auto first = [&](int i, int buf, int ring) __attribute__((always_inline)) {
+    const char* p = lds + buf * S::kStage;
+    const float* sl = reinterpret_cast<const float*>(lds + S::kScales + ring * S::kScaleBuf) + (i & (SB - 1));
     // (the order of their use; the scales' product is formed where it is used)
     w[0] = operand(p + wn * 16 * TN * 128);
 #pragma unroll
     for (int c = 0; c < TM; ++c) a[c] = operand(p + BN * 128 + (wm * TM + c) * 16 * 128);
 #pragma unroll
     for (int t = 1; t < kAhead - 1; ++t) w[t] = operand(p + (wn * TN + t) * 16 * 128);
-    fw = sl[(BM + (wn * 16 * TN) / 128) * 8];
 #pragma unroll
-    for (int c = 0; c < TM; ++c) fa[c] = sl[(wm * 16 * TM + 16 * c + lr) * 8];
-  };
-  auto sums = [&](int t, int c) __attribute__((always_inline)) {
+    for (int x = 0; x < kWS; ++x) fw[x] = sl[(BM + wblk + x) * SB];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) acc[t][c][e] = fmaf(d[t & 1][c][e], f[c], acc[t][c][e]);
+    for (int c = 0; c < TM; ++c) fa[c] = sl[(wm * 16 * TM + 16 * c + lr) * SB];
   };
-  static_assert(TN % 2 == 0, "a block's last products are in d[1], its first weights in w[0]");
+  // Product n of a block is block (n / TM, n % TM); its sums follow kLate products
+  // later, the last ones' in the next block.
+  auto sums = [&](int n) __attribute__((always_inline)) {
+    const int t = n / TM, c = n % TM;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[t][c][e] = fmaf(d[n % (kLate + 1)][e], f[c], acc[t][c][e]);
+  };
+  static_assert(TN * TM % (kLate + 1) == 0 && (kOneBlock || TM == kLate + 1), "products keep their place in d, scales of a group are formed in its block");
 
-  // A block of 128 columns: TN groups of TM products, and under each product
-  // the sums of the group before it (of the last block's last group under the
-  // first).  sched_barrier keeps that order: left alone the scheduler gathers
-  // the reads, and waits for each group's products.
+  // A block of 128 columns.  sched_barrier keeps the order of products, sums and
+  // reads: left alone the scheduler gathers the reads, and waits for each
+  // group's products.
   auto block = [&](int buf) __attribute__((always_inline)) {
-    const char* wl = fp8_lds + buf * S::kStage + wn * 16 * TN * 128;
+    const char* wl = lds + buf * S::kStage + wn * 16 * TN * 128;
 #pragma unroll
-    for (int t = 0; t < TN; ++t) {
-      if (t + kAhead - 1 < TN) w[(t + kAhead - 1) % kAhead] = operand(wl + (t + kAhead - 1) * 16 * 128);
+    for (int n = 0; n < TN * TM; ++n) {
+      const int t = n / TM, c = n % TM;
+      if (c == 0 && t + kAhead - 1 < TN) w[(t + kAhead - 1) % kAhead] = operand(wl + (t + kAhead - 1) * 16 * 128);
+      d[n % (kLate + 1)] = Op::mul(w[t % kAhead], a[c]);
+      // the scales of product n - kLate: its row of blocks' first one is next
+      const int m = (n + TN * TM - kLate) % (TN * TM);
+      if (m % TM == 0 && (m == 0 || !kOneBlock)) {
+        const int r = 16 * (m / TM);
+        const float ws = kOneBlock ? fw[0] : r < edge ? fw[0] : r < edge + 128 ? fw[kWS / 2] : fw[kWS - 1];
 #pragma unroll
-      for (int c = 0; c < TM; ++c) {
-        d[t & 1][c] = Op::mul(w[t % kAhead], a[c]);
-        sums((t + TN - 1) % TN, c);
-        __builtin_amdgcn_sched_barrier(0);
+        for (int x = 0; x < TM; ++x) f[x] = fa[x] * ws;
       }
-      if (t == 0) {
-#pragma unroll
-        for (int c = 0; c < TM; ++c) f[c] = fa[c] * fw;
-      }
+      sums(m);
+      __builtin_amdgcn_sched_barrier(0);
     }
   };
   auto meet = [&]() __attribute__((always_inline)) {
@@ -393,35 +418,35 @@ __global__ void __launch_bounds__(64 * WN * WM, 2) fp8_tile_kernel(const Fp8Args
   };
 
 #pragma unroll
-  for (int j = 0; j < 8; ++j) stage_scales(j, 0, 0);
+  for (int j = 0; j < SB; ++j) stage_scales(j, 0, 0);
 #pragma unroll
   for (int s = 0; s < NBUF; ++s) stage(s, s);
   wait_vm<(NBUF - 1) * S::kLoads>();
   meet();
   first(0, 0, 0);
   int buf = 0, used = 0;  // used: where the block's scales are
-  for (int b = 0; b + 1 < g.kb; ++b) {
+  for (int i = 0; i + 1 < blocks; ++i) {
     block(buf);
     // With the last products under way the next stage is complete (its loads
     // were issued a block ago) and every wave has read this one: its buffer
     // takes the next loads, and the next block's first operands are read.
     wait_vm<(NBUF - 2) * S::kLoads>();
     meet();
-    stage(b + NBUF, buf);
+    stage(i + NBUF, buf);
     buf = buf + 1 == NBUF ? 0 : buf + 1;
-    used = (b & 7) == 7 ? (used == 2 ? 0 : used + 1) : used;
-    first(b + 1, buf, used);
+    used = (i & (SB - 1)) == SB - 1 ? (used == 2 ? 0 : used + 1) : used;
+    first(i + 1, buf, used);
   }
   if (g.k & 15) {
     zero_rest(buf);
     __asm__ volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     meet();
-    first(g.kb - 1, buf, used);
+    first(blocks - 1, buf, used);
   }
   block(buf);
   wait_vm<0>();  // (no load to LDS may be in flight when the workgroup ends)
 #pragma unroll
-  for (int c = 0; c < TM; ++c) sums(TN - 1, c);
+  for (int n = TN * TM - kLate; n < TN * TM; ++n) sums(n);
   // (the sums end here: sunk into the stores' branches they spill)
 #pragma unroll
   for (int t = 0; t < TN; ++t)
@@ -433,14 +458,35 @@ __global__ void __launch_bounds__(64 * WN * WM, 2) fp8_tile_kernel(const Fp8Args
   // columns in 16-byte stores.  Stored as they lie, 8 bytes a lane over 16 rows,
   // a tile of 256 x 256 took about 15 us more.
   meet();
+  if constexpr (WK > 1) {
+    // the teams' sums, in their order
+    f32x4* const sums_lds = reinterpret_cast<f32x4*>(fp8_lds) + lane;
+    static_assert((WK - 1) * S::kWaves * TN * TM * 1024 <= S::kLds, "");
+    if (team > 0)
+#pragma unroll
+      for (int t = 0; t < TN; ++t)
+#pragma unroll
+        for (int c = 0; c < TM; ++c) sums_lds[((((team - 1) * S::kWaves + wave) * TN + t) * TM + c) * 64] = acc[t][c];
+    __asm__ volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    meet();
+    if (team > 0) return;
+#pragma unroll
+    for (int t = 0; t < TN; ++t)
+#pragma unroll
+      for (int c = 0; c < TM; ++c) {
+#pragma unroll
+        for (int x = 0; x < WK - 1; ++x) acc[t][c] += sums_lds[(((x * S::kWaves + wave) * TN + t) * TM + c) * 64];
+      }
+  }
   constexpr int kPer = 16 / sizeof(T);                   // elements of a store
   constexpr int kPitch = 16 * TN * (int)sizeof(T) + 16;  // of a row in LDS
   constexpr int kChunks = 16 * TN / kPer;                // stores of a row
-  static_assert(S::kWaves * 16 * kPitch <= S::kLds, "");
   struct Out {
     T v[kPer];
   };
-  char* const ol = fp8_lds + wave * 16 * kPitch;
+  constexpr int kOut = WK == 1 ? 0 : (WK - 1) * S::kWaves * TN * TM * 1024;  // (behind the sums: other waves still read them)
+  char* const ol = fp8_lds + kOut + wave * 16 * kPitch;
+  static_assert(kOut + S::kWaves * 16 * kPitch <= S::kLds, "");
   const int64_t j0 = n0 + wn * 16 * TN;
   const T* bias = static_cast<const T*>(g.bias);
 #pragma unroll
@@ -463,12 +509,12 @@ __global__ void __launch_bounds__(64 * WN * WM, 2) fp8_tile_kernel(const Fp8Args
 #pragma unroll
     for (int x = 0; x < 16 * kChunks / 64; ++x) {
       const int id = 64 * x + lane, row = id / kChunks, j = (id - row * kChunks) * kPer;
-      Out o;
-      __builtin_memcpy(&o, __builtin_assume_aligned(ol + row * kPitch + j * (int)sizeof(T), 16), 16);
+      const u32x4 w = *reinterpret_cast<const u32x4*>(ol + row * kPitch + j * (int)sizeof(T));
       if (i0 + row < g.m) {
         if (j0 + j + kPer <= g.n) {
-          __builtin_memcpy(y + (int64_t)row * g.ldy + j, &o, 16);
+          __builtin_nontemporal_store(w, reinterpret_cast<u32x4_any*>(y + (int64_t)row * g.ldy + j));
         } else {
+          const Out o = __builtin_bit_cast(Out, w);
 #pragma unroll
           for (int e = 0; e < kPer; ++e)
             if (j0 + j + e < g.n) y[(int64_t)row * g.ldy + j + e] = o.v[e];
@@ -539,49 +585,53 @@ int launch_rows_for(const Fp8Args& g, hipStream_t s) {
   return launch_status();
 }
 
-template <typename T, int WN, int WM, int TN, int TM>
+template <typename T, int WN, int WM, int TN, int TM, int WK = 1>
 int launch_tiles(Fp8Args g, hipStream_t s) {
-  using S = TileShape<WN, WM, TN, TM>;
+  using S = TileShape<WN, WM, TN, TM, WK>;
   g.tiles_m = (int)((g.m + S::kBM - 1) / S::kBM), g.tiles_n = (int)((g.n + S::kBN - 1) / S::kBN);
   const int64_t total = (int64_t)g.tiles_m * g.tiles_n;
   if (total > 0x7fffffff) return TP_ERR_BAD_DIMS;
-  if (S::kLds > 64 * 1024) allow_dynamic_lds(reinterpret_cast<const void*>(&fp8_tile_kernel<T, WN, WM, TN, TM>), 0);
-  hipLaunchKernelGGL((fp8_tile_kernel<T, WN, WM, TN, TM>), dim3((uint32_t)total), dim3(64 * S::kWaves), S::kLds, s, g);
+  if (S::kLds > 64 * 1024) allow_dynamic_lds(reinterpret_cast<const void*>(&fp8_tile_kernel<T, WN, WM, TN, TM, WK>), 0);
+  hipLaunchKernelGGL((fp8_tile_kernel<T, WN, WM, TN, TM, WK>), dim3((uint32_t)total), dim3(64 * S::kWaves * WK), S::kLds, s, g);
   return launch_status();
 }
 
 // Rounds of workgroups over the GPU times what a round takes, us: per block of
 // 128 columns, with one workgroup on a CU and with as many as it holds, and 4 to
-// begin and end.  Times of these picks, and of the other shapes in this order:
-//   2048 x 9728 x 2560 (rows, weight rows, columns)  81 (256 x 192)  88, -, 83, 95, 140
-//   4096 x 8192 x 8192  257 (256 x 256)  -, 300, 330, 410, 652
-//   512 x 4096 x 2560   15.7 (128 x 64)  40, 33, 21, -, 15.5
-//   199 x 4096 x 2560   11.6 (64 x 64)  40, 33, 20, 15, -
+// begin and end.  Times of the shapes in their order (picks in brackets):
+//   2048 x 9728 x 2560 (rows, weight rows, columns)  [62.1] 84 79 77 105 128 -
+//   4096 x 8192 x 8192  287 [256] 300 333 427 647 -
+//   1024 x 2560 x 9728  - - - 68 [62.7] 71 79
+//   512 x 4096 x 2560   50 39 33 21 16 [14.7] 19
+//   256 x 2560 x 9728   - - - 61 41 30 [25.4]
+//   199 x 4096 x 2560   50 39 33 20 15 11.0 [10.6]
 template <typename T>
 int launch_tiles_for(const Fp8Args& g, hipStream_t s) {
   struct Shape {
     int n, m, per_cu;
     double one, full;
   };
-  static const Shape shapes[] = {
-      {256, 256, 1, 1.9, 1.9}, {256, 192, 1, 1.5, 1.5}, {128, 128, 2, 1.0, 1.3}, {128, 64, 2, 0.7, 1.0}, {64, 64, 2, 0.5, 0.75}};
+  static const Shape shapes[] = {{320, 256, 1, 2.4, 2.4}, {256, 256, 1, 1.9, 1.9}, {256, 192, 1, 1.6, 1.6}, {128, 128, 2, 0.78, 1.15},
+                                 {128, 64, 2, 0.5, 0.77}, {64, 64, 2, 0.35, 0.5},  {64, 64, 1, 0.28, 0.28}};
   const int64_t cus = device_cu_count();
   // (fp32 outputs: the operands of the largest, converted, do not fit the registers)
-  int best = sizeof(T) == 4 ? 2 : 0;
+  int best = sizeof(T) == 4 ? 3 : 0;
   double least = 0;
-  for (int x = best, first = best; x < 5; ++x) {
+  for (int x = best, first = best; x < 7; ++x) {
     const Shape& p = shapes[x];
     const int64_t t = ((g.m + p.m - 1) / p.m) * ((g.n + p.n - 1) / p.n);
     const double c = t <= cus ? g.kb * p.one + 4 : (double)((t + cus * p.per_cu - 1) / (cus * p.per_cu)) * (g.kb * p.full + 4);
     if (x == first || c < least) best = x, least = c;
   }
   if constexpr (sizeof(T) != 4) {
-    if (best == 0) return launch_tiles<T, 2, 4, 8, 4>(g, s);
-    if (best == 1) return launch_tiles<T, 2, 4, 8, 3>(g, s);
+    if (best == 0) return launch_tiles<T, 2, 4, 10, 4>(g, s);
+    if (best == 1) return launch_tiles<T, 2, 4, 8, 4>(g, s);
+    if (best == 2) return launch_tiles<T, 2, 4, 8, 3>(g, s);
   }
-  if (best == 2) return launch_tiles<T, 2, 2, 4, 4>(g, s);
-  if (best == 3) return launch_tiles<T, 2, 2, 4, 2>(g, s);
-  return launch_tiles<T, 2, 2, 2, 2>(g, s);
+  if (best == 3) return launch_tiles<T, 2, 2, 4, 4>(g, s);
+  if (best == 4) return launch_tiles<T, 2, 2, 4, 2>(g, s);
+  if (best == 5) return launch_tiles<T, 2, 2, 2, 2>(g, s);
+  return launch_tiles<T, 2, 2, 2, 2, 2>(g, s);
 }
 
 template <typename T>
