@@ -175,7 +175,8 @@ def _fp8_tol(want, size, k, dtype):
 # inside a tile)
 FP8 = [(1, 1, 1), (1, 16, 128), (2, 40, 129), (3, 17, 300), (16, 100, 256), (17, 300, 300), (32, 128, 1000), (1, 20000, 300),
        (33, 65, 127), (64, 64, 128), (65, 130, 384), (200, 257, 777), (130, 1000, 3001), (300, 400, 2576), (33, 20000, 256),
-       (512, 4096, 256), (2048, 4096, 256), (2048, 9728, 384), (4000, 8100, 272)]
+       (512, 4096, 256), (2048, 4096, 256), (2048, 9728, 384), (4000, 8100, 272),
+       (2000, 5000, 300), (20000, 64, 300)]
 
 
 @pytest.mark.gpu

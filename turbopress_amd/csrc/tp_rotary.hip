@@ -25,6 +25,19 @@ struct RotaryArgs {
   int units, rot_units;  // of 2 V elements per head; the first rot_units turn
 };
 
+// Stored past the caches where that is whole 16-byte pieces.
+template <typename P, typename T>
+__device__ __forceinline__ void store_once(T* p, const P& v) {
+  if constexpr (sizeof(P) % 16 == 0) {
+    u32x4 w[sizeof(P) / 16];
+    __builtin_memcpy(w, &v, sizeof(v));
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(P) / 16; ++i) __builtin_nontemporal_store(w[i], reinterpret_cast<u32x4_any*>(p) + i);
+  } else {
+    __builtin_memcpy(p, &v, sizeof(v));
+  }
+}
+
 // A thread per (token, head, unit of 2 V elements): V pairs, or 2 V elements
 // that are copied.  Units of the half layout take V elements of either half.
 template <typename T, int V>
@@ -100,8 +113,8 @@ __global__ void __launch_bounds__(256) rotary_kernel(const RotaryArgs a) {
 #pragma unroll
     for (int e = 0; e < V; ++e) x.v[e] = (T)f[e], y.v[e] = (T)f[V + e];
   }
-  __builtin_memcpy(dst + first, &x, sizeof(x));
-  __builtin_memcpy(dst + second, &y, sizeof(y));
+  store_once(dst + first, x);
+  store_once(dst + second, y);
 }
 
 template <typename T>
