@@ -216,13 +216,13 @@ def shared_workspace(device, nbytes: int) -> Tensor:
     least `nbytes` long (allocated or grown on first need)."""
     dev = torch.device(device)
     index = dev.index if dev.index is not None else torch.cuda.current_device()
-    stream = raw_stream(index)
+    stream = torch.cuda.current_stream(index).cuda_stream
     key = (index, stream)
     ws = _WORKSPACES.get(key)
     if ws is not None and ws.numel() >= nbytes:
         return ws
     new = max(_aligned(nbytes), _WS_ALIGN)
-    if torch.cuda.is_current_stream_capturing():
+    if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
         capture = _lib.lib().tp_stream_capture_id(stream)
         held = _CAPTURED_WORKSPACES.get(key)
         if held is None or held[0] != capture:
