@@ -108,7 +108,8 @@ struct Span {
 template <int UNIT>
 __device__ __forceinline__ Span span_of(const PagedArgs& a, int length) {
   Span s;
-  s.len = (int)min((int64_t)max(length, 0), a.table_width * a.page_size);
+  // (room for the last unit's tokens below 2^31)
+  s.len = (int)min(min((int64_t)max(length, 0), a.table_width * a.page_size), (int64_t)0x7ffff000);
   s.first = a.window > 0 && s.len > a.window ? (int)(s.len - a.window) : 0;
   s.base = s.first & ~(kTile - 1);
   // (an empty sequence is one unit too: its zeros have to be written)
