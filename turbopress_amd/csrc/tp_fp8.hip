@@ -561,8 +561,8 @@ void launch_rows(const Fp8Args& g, int waves, hipStream_t s) {
 
 // Whether a call takes the rows kernel.  us at (n, k), rows kernel against the
 // fastest tiles:
-//   32 rows  4096, 2560: 7.0 / 10.7   2560, 9728: 17.8 / 30.5   9728, 2560: 13.7 / 11.0   16384, 1000: 9.4 / 8.3
-//   64 rows  4096, 2560: 10.3 / 11.1  2560, 9728: 28.8 / 30.7   9728, 2560: 20.2 / 11.5   1024, 1024: 6.0 / 6.4
+//   32 rows  1024, 1024: 4.5 / 6.0   4096, 2560: 7.2 / 9.5   2560, 9728: 17.9 / 23.3   9728, 2560: 15.2 / 10.0
+//   64 rows  4096, 2560: 10.3 / 10.1  2560, 9728: 28.8 / 24.0   9728, 2560: 20.2 / 10.0
 // so 17..32 rows take it for up to 6144 weight rows (the tiles' time is their
 // chain of blocks until their count fills the GPU), more rows never.
 bool fp8_takes_rows(int64_t m, int64_t n) { return m <= 16 || (m <= 32 && n <= 6144); }
@@ -599,12 +599,12 @@ int launch_tiles(Fp8Args g, hipStream_t s) {
 // Rounds of workgroups over the GPU times what a round takes, us: per block of
 // 128 columns, with one workgroup on a CU and with as many as it holds, and 4 to
 // begin and end.  Times of the shapes in their order (picks in brackets):
-//   2048 x 9728 x 2560 (rows, weight rows, columns)  [62.1] 84 79 77 105 128 -
-//   4096 x 8192 x 8192  287 [256] 300 333 427 647 -
-//   1024 x 2560 x 9728  - - - 68 [62.7] 71 79
-//   512 x 4096 x 2560   50 39 33 21 16 [14.7] 19
-//   256 x 2560 x 9728   - - - 61 41 30 [25.4]
-//   199 x 4096 x 2560   50 39 33 20 15 11.0 [10.6]
+//   2048 x 9728 x 2560 (rows, weight rows, columns)  [63] 82 74 78 98 128 171
+//   4096 x 8192 x 8192  289 [262] 298 335 427 648 723
+//   1024 x 2560 x 9728  150 126 106 69 [59] 70 78
+//   512 x 4096 x 2560   50 39 33 21 14.8 [14.3] 18.5
+//   256 x 2560 x 9728   146 122 100 61 40 29 [24.0]
+//   199 x 4096 x 2560   49 39 33 20 14.3 10.8 [10.3]
 template <typename T>
 int launch_tiles_for(const Fp8Args& g, hipStream_t s) {
   struct Shape {

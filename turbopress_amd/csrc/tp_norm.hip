@@ -8,7 +8,9 @@
 // its output, so x and the residual are read once and h, y (or codes) written
 // once; the weight comes from L2.  Nothing is computed to speak of (4 flops per
 // element): many rows are bound by HBM, a few by the latency of load, reduction
-// and store.
+// and store.  8192 x 9728 fp16 60 us = 5.3 TB/s (a copy reaches 5.2); 8191 x 9727
+// 80, for no row but every eighth begins on 16 bytes; 2048 x 2560 with a residual
+// and e4m3 output 10.5; 1 x 2560 3.
 #include "tp_ops_common.h"
 
 #include <algorithm>
@@ -297,6 +299,11 @@ constexpr int kNormMaxVpt = 6;
 // Lanes and vectors per lane of a row.  Few rows: as many lanes as the row
 // feeds (a chain of latencies).  Many: the split with the fewest idle slots,
 // and among those the fewest waves, for a row inside one wave needs no LDS.
+// fp16 with a residual, us, the split of many rows / of few:
+//   d       1 row      512 rows   1024       2048
+//   1024    3.6 / 3.0  4.0 / 3.6  4.3 / 3.9  5.4 / 5.1
+//   2560    5.3 / 3.4  6.5 / 4.6  8.2 / 6.3  9.0 / 9.7
+//   4096    4.8 / 3.5  7.1 / 5.1  7.8 / 7.5  11.7 / 12.6
 struct NormPlan {
   int sub, waves, vpt;  // vpt 0: the long kernel
 };
@@ -304,7 +311,7 @@ struct NormPlan {
 inline NormPlan norm_plan(int64_t rows, int nvec, int cus) {
   if (nvec <= 16) return {16, 1, 1};
   if (nvec <= 32) return {32, 1, 1};
-  const bool few = rows < 4 * (int64_t)cus;
+  const bool few = rows <= 4 * (int64_t)cus;
   NormPlan best{64, 8, 0};
   int64_t best_cost = -1;
   for (int w = 1; w <= 8; w *= 2) {
@@ -320,9 +327,10 @@ template <typename T, int OUT>
 int launch_norm(const NormArgs& a0, hipStream_t s) {
   NormArgs a = a0;
   // Loads past the caches from 128 MB of inputs, half of what the memory side
-  // caches: 8191 x 9727 fp16 76 us against 82, 8192 x 9728 64 against 77; what
-  // the step before has just written is better read from there: 16384 x 1024
-  // with a residual 25.9 against 21.4, 2048 x 2560 12.7 against 9.4.
+  // caches: 8191 x 9727 fp16 80 us against 83, 8192 x 9728 60 against 67, 16384 x
+  // 2560 with a residual 65 against 66; what the step before has just written is
+  // better read from there: 16384 x 1024 with a residual 25.8 against 21.1, 2048 x
+  // 2560 13.5 against 9.0, 4096 x 9728 without 33 against 31.
   a.large = a.rows * a.d * (int64_t)sizeof(T) * (a.residual ? 2 : 1) >= (128 << 20);
   const NormPlan p = norm_plan(a.rows, a.nvec, device_cu_count());
   if (p.vpt == 0) {

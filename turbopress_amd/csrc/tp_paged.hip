@@ -6,7 +6,9 @@
 //
 // and two states join in the same way, so a sequence may be cut anywhere.
 // Keys and values are read once, 4 * (query heads per cache head) flops for
-// each of their elements: bound by HBM.
+// each of their elements: bound by HBM (8 heads of 128: 64 sequences x 8192
+// tokens 351 us = 6.1 TB/s, 1 x 131072 102 us = 5.2 with its start and join; 1 x
+// 577 9 us, the chain of lengths, pages, keys and join).
 //
 // Work: 128 tokens of one (sequence, cache head) are a unit.  A grid of as many
 // workgroups as the GPU holds takes equal runs of the list of all units, so

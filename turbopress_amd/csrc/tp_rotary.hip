@@ -7,6 +7,8 @@
 // once: an angle position * frequency formed in fp32 is off by up to 2^-24 of
 // the position, 0.008 at position 131072).  Each element is read and written
 // once; 3 flops per element: bound by HBM, or by latency for a few tokens.
+// 2047 tokens of 32 + 8 + 8 heads of 128 into the cache 7.8 us (34 MB, part of
+// them out of the memory-side cache), one token of 4 sequences 2.7.
 #include "tp_ops_common.h"
 
 #include <algorithm>
