@@ -84,3 +84,34 @@ def test_pages_are_handed_out_and_taken_back(cuda):
     c.release(0)
     c.reserve(2, 12)
     assert c.block_table[0].max() == -1 and sorted(c.block_table[2, :3].tolist()) == sorted(held[0, :3].tolist())
+
+
+def test_sliding_window_layers_match_the_hf_decoder(cuda, tmp_path):
+    from turbopress_amd.artifact import load_packed_model
+    from turbopress_amd.paged_decode import PagedDecoder
+    from turbopress_amd.synthetic import tiny_qwen3_config, write_synthetic_artifact
+    cfg = tiny_qwen3_config()
+    cfg.use_sliding_window, cfg.sliding_window = True, 6
+    cfg.layer_types = ["sliding_attention", "full_attention"] * (cfg.num_hidden_layers // 2)
+    write_synthetic_artifact(tmp_path, cfg, bits=3, seed=3)
+    windowed = load_packed_model(tmp_path, device="cuda", mode="hip")[0]
+    assert windowed.model.layers[0].self_attn.sliding_window == 6
+    dec = PagedDecoder(windowed, 2, 64, page_size=16, fp8_head=False)
+    for s, p in enumerate(_prompts([21, 4])):
+        _near(dec.prefill(s, p)[0], _hf_logits(windowed, p), TOL)
+        dec.cache.reserve(s, len(p) + 1)
+        tokens = torch.cat((p, dec.tokens[s:s + 1]))
+        logits = dec.step(graph=False)
+        _near(logits[s], _hf_logits(windowed, tokens), TOL)
+        dec.stop(s)
+
+
+def test_what_the_decoder_does_not_run_is_refused(model):
+    from turbopress_amd.paged_decode import PagedDecoder
+    act = model.config.hidden_act
+    model.config.hidden_act = "gelu"
+    try:
+        with pytest.raises(ValueError, match="hidden_act"):
+            PagedDecoder(model, 1, 64)
+    finally:
+        model.config.hidden_act = act

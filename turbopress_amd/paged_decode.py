@@ -96,6 +96,8 @@ class PagedDecoder:
     def __init__(self, model, sequences: int, max_len: int, page_size: int = 64, n_pages: int | None = None,
                  fp8_head: bool = True) -> None:
         cfg = model.config
+        if cfg.hidden_act != "silu":
+            raise ValueError(f"hidden_act {cfg.hidden_act!r}: PagedDecoder runs the gated MLP with silu")
         self.model, self.sequences = model, sequences
         body = model.model
         self.embed, self.layers, self.norm = body.embed_tokens, body.layers, body.norm
@@ -135,7 +137,8 @@ class PagedDecoder:
                 q, k = self._norm(q, at.q_norm), self._norm(k, at.k_norm)
             kc, vc = self.cache.k[i], self.cache.v[i]
             q = rotary_append(q, k, v, self.table, positions, kc, vc, self.cache.block_table, sequences=sequences)
-            o = paged_attention(q, kc, vc, block_table, lengths, scale=self.scale)
+            window = getattr(at, "sliding_window", None) or 0
+            o = paged_attention(q, kc, vc, block_table, lengths, scale=self.scale, window=window)
             x, h = self._norm(at.o_proj(o.view(rows, -1)), layer.post_attention_layernorm, h)
             gate, up = layer.mlp.gate_proj(x), layer.mlp.up_proj(x)
             x = layer.mlp.down_proj(F.silu(gate) * up)
@@ -160,7 +163,7 @@ class PagedDecoder:
         n = int(prompt.shape[0])
         if n < 1:
             raise ValueError("a prompt needs a token")
-        self.cache.release(sequence)
+        self.stop(sequence)
         self.cache.reserve(sequence, n)
         dev = self.tokens.device
         pos = torch.arange(n, device=dev)
