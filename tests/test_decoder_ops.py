@@ -211,6 +211,28 @@ def test_fp8_linear_rows_apart(cuda, m, k, pads):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("offset", [1, 2, 3, 4, 8])
+@pytest.mark.parametrize("m,n,k", [(1, 70, 33), (5, 6200, 257), (20, 6200, 130), (24, 33600, 1001), (40, 70, 1027)])
+def test_fp8_linear_rows_off_their_words(cuda, m, n, k, offset):
+    """Operands that begin anywhere in a word of memory, and rows that begin
+    elsewhere in theirs; the bytes around them are NaN."""
+    from turbopress_amd import fp8_linear
+    g = _gen(m + k + offset)
+    a, sa, w, sw = _fp8_case(g, m, n, k)
+
+    def moved(t, off):
+        ld = t.shape[1] + 3
+        raw = torch.full((off + t.shape[0] * ld + 8,), 0x7f, dtype=torch.uint8, device="cuda")
+        rows = raw[off:off + t.shape[0] * ld].view(-1, ld)[:, :t.shape[1]]
+        rows.copy_(t.view(torch.uint8))
+        return rows.view(torch.float8_e4m3fn)
+
+    want, size = O.fp8_linear(a, sa, w, sw)
+    got = fp8_linear(moved(a, offset), sa, moved(w, 5 * offset), sw, out_dtype=F32)
+    _within(got, want, _fp8_tol(want, size, k, F32))
+
+
+@pytest.mark.gpu
 def test_fp8_linear_rows_do_not_mix(cuda):
     from turbopress_amd import fp8_linear
     g = _gen(9)

@@ -103,28 +103,50 @@ struct Operand<true> {
 // ---------------------------------------------------------------------------
 // few rows
 // ---------------------------------------------------------------------------
-// The first `left` of 32 bytes at any alignment, then zeros.
-__device__ __forceinline__ i32x8 load_rest(const uint8_t* p, int left) {
-  i32x8 r = {0, 0, 0, 0, 0, 0, 0, 0};
-  if (left >= 32) {
-    __builtin_memcpy(&r, p, 32);
-  } else {
+// 4 N bytes at any alignment: the words that hold them, loaded as they lie (a
+// word that holds a byte of a row is memory), and moved over by the address's
+// last bits.  Loads at odd addresses take up to five times as long (16 rows of
+// 2560 x 9727 40 us with them).
+template <int N>
+struct Unaligned {
+  static_assert(N % 4 == 0, "");
+  u32x4 at[N / 4];
+  uint32_t next;
+
+  __device__ __forceinline__ void load(const uint8_t* p) {
+    const uint32_t s = (uint32_t)(uintptr_t)p & 3;
+    const uint32_t* q = reinterpret_cast<const uint32_t*>(p - s);
 #pragma unroll
-    for (int x = 0; x < 8; ++x) {
-      uint32_t v = 0;
+    for (int x = 0; x < N / 4; ++x) __builtin_memcpy(&at[x], __builtin_assume_aligned(q + 4 * x, 4), 16);
+    next = q[s ? N : N - 1];  // (at s = 0 not used)
+  }
+  // The first `left` bytes, then zeros.
+  __device__ __forceinline__ void load(const uint8_t* p, int left) {
+    const uint32_t s = (uint32_t)(uintptr_t)p & 3;
+    const uint32_t* q = reinterpret_cast<const uint32_t*>(p - s);
+    const int n = left > 0 ? left + (int)s : 0;
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (4 * x + e < left) v |= (uint32_t)p[4 * x + e] << (8 * e);
-      r[x] = (int)v;
+    for (int x = 0; x < N; ++x) at[x / 4][x % 4] = 4 * x < n ? q[x] : 0;
+    next = 4 * N < n ? q[N] : 0;
+#pragma unroll
+    for (int x = 0; x <= N; ++x) {
+      const int in = n - 4 * x;  // bytes of the row in this word
+      const uint32_t keep = in >= 4 ? ~0u : in <= 0 ? 0u : (1u << (8 * in)) - 1;
+      if (x < N) at[x / 4][x % 4] &= keep;
+      else next &= keep;
     }
   }
-  return r;
-}
+  // Bytes of the address that it was loaded from.
+  __device__ __forceinline__ uint32_t word(int x, uint32_t s) const {
+    return __builtin_amdgcn_alignbyte(x + 1 < N ? at[(x + 1) / 4][(x + 1) % 4] : next, at[x / 4][x % 4], s);
+  }
+};
 
 // A workgroup takes RT tiles of 16 weight rows and all (up to 16 NC)
 // activation rows; its waves take every waves-th block of columns, the loads
 // of the next one in flight, and their sums are joined through LDS.
-template <typename T, int NC, int RT>
+// ODD: rows of either operand do not begin on words.
+template <typename T, int NC, int RT, bool ODD>
 __global__ void __launch_bounds__(NC == 1 ? 1024 : 512) fp8_rows_kernel(const Fp8Args g) {
   using Op = Operand<sizeof(T) == 4>;
   extern __shared__ __attribute__((aligned(16))) char fp8_lds[];
@@ -153,26 +175,42 @@ __global__ void __launch_bounds__(NC == 1 ? 1024 : 512) fp8_rows_kernel(const Fp
 #pragma unroll
     for (int c = 0; c < NC; ++c) acc[t][c] = f32x4{0, 0, 0, 0};
 
+  using Codes = std::conditional_t<ODD, Unaligned<8>, i32x8>;
   struct Block {
-    i32x8 w[RT], a[NC];
+    Codes w[RT], a[NC];
     float fa[NC], fw[RT];
+  };
+  auto codes = [&](Codes& x, const uint8_t* p) __attribute__((always_inline)) {
+    if constexpr (ODD) x.load(p);
+    else __builtin_memcpy(&x, p, 32);
+  };
+  auto words = [&](const Unaligned<8>& x, const uint8_t* p) __attribute__((always_inline)) {
+    const uint32_t s = (uint32_t)(uintptr_t)p & 3;
+    i32x8 r;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) r[e] = (int)x.word(e, s);
+    return r;
+  };
+  auto aligned = [&](const Codes& x, const uint8_t* p) __attribute__((always_inline)) {
+    if constexpr (ODD) return words(x, p);
+    else return x;
   };
   auto load = [&](Block& x, int b) __attribute__((always_inline)) {
 #pragma unroll
-    for (int t = 0; t < RT; ++t) __builtin_memcpy(&x.w[t], wp[t] + 128 * b, 32);
+    for (int t = 0; t < RT; ++t) codes(x.w[t], wp[t] + 128 * b);
 #pragma unroll
-    for (int c = 0; c < NC; ++c) __builtin_memcpy(&x.a[c], ap[c] + 128 * b, 32), x.fa[c] = sap[c][b];
+    for (int c = 0; c < NC; ++c) codes(x.a[c], ap[c] + 128 * b), x.fa[c] = sap[c][b];
 #pragma unroll
     for (int t = 0; t < RT; ++t) x.fw[t] = swp[t][b];
   };
   auto add = [&](const Block& x) __attribute__((always_inline)) {
     Op a[NC];
 #pragma unroll
-    for (int c = 0; c < NC; ++c) a[c].set(x.a[c]);
+    for (int c = 0; c < NC; ++c) a[c].set(aligned(x.a[c], ap[c]));
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
       Op w;
-      w.set(x.w[t]);
+      w.set(aligned(x.w[t], wp[t]));
 #pragma unroll
       for (int c = 0; c < NC; ++c) acc[t][c] += Op::mul(w, a[c]) * (x.fa[c] * x.fw[t]);
     }
@@ -191,10 +229,16 @@ __global__ void __launch_bounds__(NC == 1 ? 1024 : 512) fp8_rows_kernel(const Fp
   if (whole < g.kb && wave == whole % waves) {
     const int left = g.k - 128 * whole - 32 * lg;  // columns of this lane's 32
     Block x;
+    auto rest = [&](Codes& x, const uint8_t* p) __attribute__((always_inline)) {
+      Unaligned<8> u;
+      u.load(p, min(left, 32));
+      if constexpr (ODD) x = u;
+      else x = words(u, p);
+    };
 #pragma unroll
-    for (int t = 0; t < RT; ++t) x.w[t] = load_rest(wp[t] + 128 * whole, left), x.fw[t] = swp[t][whole];
+    for (int t = 0; t < RT; ++t) rest(x.w[t], wp[t] + 128 * whole), x.fw[t] = swp[t][whole];
 #pragma unroll
-    for (int c = 0; c < NC; ++c) x.a[c] = load_rest(ap[c] + 128 * whole, left), x.fa[c] = sap[c][whole];
+    for (int c = 0; c < NC; ++c) rest(x.a[c], ap[c] + 128 * whole), x.fa[c] = sap[c][whole];
     add(x);
   }
 
@@ -327,14 +371,13 @@ __global__ void __launch_bounds__(64 * WN * WM * WK, WK > 2 ? 1 : 2) fp8_tile_ke
   auto zero_rest = [&](int buf) __attribute__((always_inline)) {
     const int in = g.k - (128 * (g.kb - 1) + (int)chunk);  // columns of this lane's chunk
     if (team == WK - 1 && in > 0 && in < 16) {
-      char* p = lds + buf * S::kStage + lane * 16;
+      u32x4 keep;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) keep[e] = in >= 4 * e + 4 ? ~0u : in <= 4 * e ? 0u : (1u << (8 * (in - 4 * e))) - 1;
+      u32x4* p = reinterpret_cast<u32x4*>(lds + buf * S::kStage) + lane;
 #pragma nounroll
-      for (int x = 0; x < S::kWLoads + S::kALoads; ++x) {
-        char* at = p + (x < S::kWLoads ? (wave * S::kWLoads + x) * 1024
-                                       : BN * 128 + (wave * S::kALoads + x - S::kWLoads) * 1024);
-#pragma nounroll
-        for (int e = in; e < 16; ++e) at[e] = 0;
-      }
+      for (int x = 0; x < S::kWLoads + S::kALoads; ++x)
+        p[64 * (x < S::kWLoads ? wave * S::kWLoads + x : BN / 8 + wave * S::kALoads + x - S::kWLoads)] &= keep;
     }
   };
 
@@ -525,24 +568,36 @@ __global__ void __launch_bounds__(64 * WN * WM * WK, WK > 2 ? 1 : 2) fp8_tile_ke
   }
 }
 
-// Rows of any alignment copied to rows of `ld` bytes (a multiple of 16).
-__global__ void __launch_bounds__(256) fp8_align_kernel(const uint8_t* __restrict__ src, int64_t lds, uint8_t* __restrict__ dst,
-                                                        int64_t ldd, int64_t rows, int k) {
-  const int64_t chunks = ldd / 16, all = rows * chunks;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (int64_t)gridDim.x * 256) {
-    const int64_t r = i / chunks;
-    const int c = (int)(i - r * chunks) * 16;
-    const uint8_t* p = src + r * lds + c;
-    u32x4 v = {0, 0, 0, 0};
-    if (c + 16 <= k) {
-      __builtin_memcpy(&v, p, 16);
-    } else {
+// Rows of any alignment, of one operand or of both, copied to rows of `ld` bytes
+// (a multiple of 16): 16 lanes copy 1 KB of a row, 4 chunks each.
+struct Fp8Copies {
+  const uint8_t* src[2];
+  uint8_t* dst[2];
+  int64_t from[2], rows[2];  // row strides of the sources, rows (none: aligned)
+  int64_t ld;
+  int k;
+};
+
+__global__ void __launch_bounds__(256) fp8_align_kernel(Fp8Copies g) {
+  int64_t r = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
+  const bool second = r >= g.rows[0];
+  if (second) r -= g.rows[0];
+  if (second && r >= g.rows[1]) return;
+  const uint8_t* const src = g.src[second] + r * g.from[second];
+  uint8_t* const dst = g.dst[second] + r * g.ld;
+  const int first = (int)blockIdx.y * 1024 + (int)(threadIdx.x & 15) * 16;
+  Unaligned<4> v[4];
 #pragma unroll
-      for (int x = 0; x < 16; ++x)
-        if (c + x < k) v[x >> 2] |= (uint32_t)p[x] << (8 * (x & 3));
-    }
-    *reinterpret_cast<u32x4*>(dst + r * ldd + c) = v;
+  for (int x = 0; x < 4; ++x) {
+    const int c = first + 256 * x;
+    if (c + 16 <= g.k) v[x].load(src + c);
+    else v[x].load(src + c, g.k - c);
   }
+  const uint32_t s = (uint32_t)(uintptr_t)src & 3;
+#pragma unroll
+  for (int x = 0; x < 4; ++x)
+    if (first + 256 * x < g.k)
+      *reinterpret_cast<u32x4*>(dst + first + 256 * x) = u32x4{v[x].word(0, s), v[x].word(1, s), v[x].word(2, s), v[x].word(3, s)};
 }
 
 bool fp8_sizes_ok(int64_t m, int64_t n, int64_t k) {
@@ -551,12 +606,12 @@ bool fp8_sizes_ok(int64_t m, int64_t n, int64_t k) {
 
 bool fp8_rows_aligned(const void* p, int64_t ld) { return ((ld | (int64_t)(uintptr_t)p) & 15) == 0; }
 
-template <typename T, int NC, int RT>
+template <typename T, int NC, int RT, bool ODD>
 void launch_rows(const Fp8Args& g, int waves, hipStream_t s) {
   const int64_t groups = (g.n + 16 * RT - 1) / (16 * RT);
   const int lds = waves * RT * NC * 64 * 16;
-  if (lds > 64 * 1024) allow_dynamic_lds(reinterpret_cast<const void*>(&fp8_rows_kernel<T, NC, RT>), 0);
-  hipLaunchKernelGGL((fp8_rows_kernel<T, NC, RT>), dim3((uint32_t)groups), dim3(64 * waves), lds, s, g);
+  if (lds > 64 * 1024) allow_dynamic_lds(reinterpret_cast<const void*>(&fp8_rows_kernel<T, NC, RT, ODD>), 0);
+  hipLaunchKernelGGL((fp8_rows_kernel<T, NC, RT, ODD>), dim3((uint32_t)groups), dim3(64 * waves), lds, s, g);
 }
 
 // Whether a call takes the rows kernel.  us at (n, k), rows kernel against the
@@ -564,8 +619,13 @@ void launch_rows(const Fp8Args& g, int waves, hipStream_t s) {
 //   32 rows  1024, 1024: 4.5 / 6.0   4096, 2560: 7.2 / 9.5   2560, 9728: 17.9 / 23.3   9728, 2560: 15.2 / 10.0
 //   64 rows  4096, 2560: 10.3 / 10.1  2560, 9728: 28.8 / 24.0   9728, 2560: 20.2 / 10.0
 // so 17..32 rows take it for up to 6144 weight rows (the tiles' time is their
-// chain of blocks until their count fills the GPU), more rows never.
-bool fp8_takes_rows(int64_t m, int64_t n) { return m <= 16 || (m <= 32 && n <= 6144); }
+// chain of blocks until their count fills the GPU), more rows never.  Operands
+// that do not begin on 16 bytes are copied for the tiles: 32 rows, 7000, 100: 3.8
+// / 9.4  16384, 1000: 11.4 / 19.2  16000, 5003: 57.6 / 51.4, so they take it up to
+// 32 MB of weights, halfway.
+bool fp8_takes_rows(int64_t m, int64_t n, int64_t k, bool aligned) {
+  return m <= 16 || (m <= 32 && (n <= 6144 || (!aligned && n * k <= (32 << 20))));
+}
 
 template <typename T>
 int launch_rows_for(const Fp8Args& g, hipStream_t s) {
@@ -576,11 +636,16 @@ int launch_rows_for(const Fp8Args& g, hipStream_t s) {
   int waves = 8;
   while (waves > 1 && waves > g.kb) waves /= 2;
   const bool two = (g.n + 15) / 16 >= 4 * (int64_t)device_cu_count();
+  const bool odd = (((uintptr_t)g.a | (uintptr_t)g.w | g.lda | g.ldw) & 3) != 0;
   if (g.m <= 16) {
-    if (two) launch_rows<T, 1, 2>(g, waves, s);
-    else launch_rows<T, 1, 1>(g, waves, s);
+    if (two && odd) launch_rows<T, 1, 2, true>(g, waves, s);
+    else if (two) launch_rows<T, 1, 2, false>(g, waves, s);
+    else if (odd) launch_rows<T, 1, 1, true>(g, waves, s);
+    else launch_rows<T, 1, 1, false>(g, waves, s);
+  } else if (odd) {
+    launch_rows<T, 2, 1, true>(g, waves, s);
   } else {
-    launch_rows<T, 2, 1>(g, waves, s);
+    launch_rows<T, 2, 1, false>(g, waves, s);
   }
   return launch_status();
 }
@@ -635,8 +700,8 @@ int launch_tiles_for(const Fp8Args& g, hipStream_t s) {
 }
 
 template <typename T>
-int launch_fp8(const Fp8Args& g, hipStream_t s) {
-  return fp8_takes_rows(g.m, g.n) ? launch_rows_for<T>(g, s) : launch_tiles_for<T>(g, s);
+int launch_fp8(const Fp8Args& g, bool rows, hipStream_t s) {
+  return rows ? launch_rows_for<T>(g, s) : launch_tiles_for<T>(g, s);
 }
 
 int64_t align_bytes(int64_t rows, int64_t k) { return rows * ((k + 15) & ~(int64_t)15); }
@@ -648,7 +713,8 @@ using namespace tp;
 extern "C" int64_t tp_fp8_workspace_bytes(int64_t m, int64_t n, int64_t k, const uint8_t* a, int64_t lda,
                                           const uint8_t* w, int64_t ldw) {
   if (!fp8_sizes_ok(m, n, k)) return -1;
-  if (m == 0 || n == 0 || fp8_takes_rows(m, n)) return 0;
+  const bool aligned = fp8_rows_aligned(a, lda) && fp8_rows_aligned(w, ldw);
+  if (m == 0 || n == 0 || fp8_takes_rows(m, n, k, aligned)) return 0;
   return (fp8_rows_aligned(a, lda) ? 0 : align_bytes(m, k)) + (fp8_rows_aligned(w, ldw) ? 0 : align_bytes(n, k));
 }
 
@@ -662,25 +728,27 @@ extern "C" int tp_fp8_linear(int dtype, int64_t m, int64_t n, int64_t k, const u
   if (!a || !a_scales || !w || !w_scales || !y) return TP_ERR_NULL_POINTER;
   const uintptr_t mask = dtype_bytes(dtype) - 1;
   if ((((uintptr_t)a_scales | (uintptr_t)w_scales) & 3) || (((uintptr_t)bias | (uintptr_t)y) & mask)) return TP_ERR_MISALIGNED;
+  const bool rows = fp8_takes_rows(m, n, k, fp8_rows_aligned(a, lda) && fp8_rows_aligned(w, ldw));
   const int64_t need = tp_fp8_workspace_bytes(m, n, k, a, lda, w, ldw);
   if (need > 0 && (!workspace || workspace_bytes < need)) return TP_ERR_WORKSPACE;
   if (need > 0 && ((uintptr_t)workspace & 15)) return TP_ERR_MISALIGNED;
   hipStream_t s = (hipStream_t)stream;
   if (need > 0) {
-    const int64_t ld = (k + 15) & ~(int64_t)15;
+    Fp8Copies c{{a, w}, {nullptr, nullptr}, {lda, ldw}, {0, 0}, (k + 15) & ~(int64_t)15, (int)k};
     uint8_t* free = static_cast<uint8_t*>(workspace);
-    auto align = [&](const uint8_t*& p, int64_t& from, int64_t rows) {
+    auto align = [&](int x, const uint8_t*& p, int64_t& from, int64_t rows) {
       if (fp8_rows_aligned(p, from)) return;
-      const int64_t blocks = std::min<int64_t>((rows * (ld / 16) + 255) / 256, 16 * device_cu_count());
-      hipLaunchKernelGGL(fp8_align_kernel, dim3((uint32_t)blocks), dim3(256), 0, s, p, from, free, ld, rows, (int)k);
-      p = free, from = ld;
-      free += rows * ld;
+      c.dst[x] = free, c.rows[x] = rows;
+      p = free, from = c.ld;
+      free += rows * c.ld;
     };
-    align(a, lda, m);
-    align(w, ldw, n);
+    align(0, a, lda, m);
+    align(1, w, ldw, n);
+    const dim3 grid((uint32_t)((c.rows[0] + c.rows[1] + 15) / 16), (uint32_t)((k + 1023) / 1024));
+    hipLaunchKernelGGL(fp8_align_kernel, grid, dim3(256), 0, s, c);
   }
   Fp8Args g{a, w, a_scales, w_scales, bias, y, lda, ldw, ldy, m, n, (int)k, (int)((k + 127) / 128), 0, 0};
-  if (dtype == TP_F16) return launch_fp8<f16_t>(g, s);
-  if (dtype == TP_BF16) return launch_fp8<bf16_t>(g, s);
-  return launch_fp8<float>(g, s);
+  if (dtype == TP_F16) return launch_fp8<f16_t>(g, rows, s);
+  if (dtype == TP_BF16) return launch_fp8<bf16_t>(g, rows, s);
+  return launch_fp8<float>(g, rows, s);
 }
