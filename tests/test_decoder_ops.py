@@ -69,6 +69,29 @@ def test_rms_norm(cuda, rows, d, dtype, residual):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("rows,d,pad", [(5, 128, 1), (70, 100, 3), (9, 7, 0), (3, 256, 1), (33, 200, 5), (4, 2560, 1), (2000, 2560, 3),
+                                        (6, 9727, 0), (3, 9728, 1), (2, 30001, 1)])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_rms_norm_rows_off_their_words(cuda, rows, d, pad, dtype):
+    """Rows of 2-byte elements that begin in the middle of a word, NaN between them."""
+    from turbopress_amd import rms_norm, rms_norm_fp8
+    g = _gen(rows + d + pad)
+
+    def moved(t, off):
+        raw = torch.full((off + rows * (d + pad) + 1,), float("nan"), dtype=dtype, device="cuda")
+        out = raw[off:off + rows * (d + pad)].view(rows, d + pad)[:, :d]
+        return out.copy_(t)
+
+    x, r, w = _randn(g, rows, d, dtype=dtype), _randn(g, rows, d, dtype=dtype), _randn(g, d, dtype=dtype)
+    for off in (0, 1):
+        assert torch.equal(rms_norm(moved(x, off), w), rms_norm(x, w))
+        for got, want in zip(rms_norm(moved(x, off), w, residual=moved(r, 1 - off)), rms_norm(x, w, residual=r)):
+            assert torch.equal(got, want)
+        for got, want in zip(rms_norm_fp8(moved(x, off), w, residual=moved(r, 0)), rms_norm_fp8(x, w, residual=r)):
+            assert torch.equal(got.float(), want.float())
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("rows,d", NORM)
 @pytest.mark.parametrize("dtype,residual", [(F16, True), (BF16, False), (F32, True)])
 @pytest.mark.parametrize("block", [128, None])

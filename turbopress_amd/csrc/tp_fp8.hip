@@ -103,45 +103,6 @@ struct Operand<true> {
 // ---------------------------------------------------------------------------
 // few rows
 // ---------------------------------------------------------------------------
-// 4 N bytes at any alignment: the words that hold them, loaded as they lie (a
-// word that holds a byte of a row is memory), and moved over by the address's
-// last bits.  Loads at odd addresses take up to five times as long (16 rows of
-// 2560 x 9727 40 us with them).
-template <int N>
-struct Unaligned {
-  static_assert(N % 4 == 0, "");
-  u32x4 at[N / 4];
-  uint32_t next;
-
-  __device__ __forceinline__ void load(const uint8_t* p) {
-    const uint32_t s = (uint32_t)(uintptr_t)p & 3;
-    const uint32_t* q = reinterpret_cast<const uint32_t*>(p - s);
-#pragma unroll
-    for (int x = 0; x < N / 4; ++x) __builtin_memcpy(&at[x], __builtin_assume_aligned(q + 4 * x, 4), 16);
-    next = q[s ? N : N - 1];  // (at s = 0 not used)
-  }
-  // The first `left` bytes, then zeros.
-  __device__ __forceinline__ void load(const uint8_t* p, int left) {
-    const uint32_t s = (uint32_t)(uintptr_t)p & 3;
-    const uint32_t* q = reinterpret_cast<const uint32_t*>(p - s);
-    const int n = left > 0 ? left + (int)s : 0;
-#pragma unroll
-    for (int x = 0; x < N; ++x) at[x / 4][x % 4] = 4 * x < n ? q[x] : 0;
-    next = 4 * N < n ? q[N] : 0;
-#pragma unroll
-    for (int x = 0; x <= N; ++x) {
-      const int in = n - 4 * x;  // bytes of the row in this word
-      const uint32_t keep = in >= 4 ? ~0u : in <= 0 ? 0u : (1u << (8 * in)) - 1;
-      if (x < N) at[x / 4][x % 4] &= keep;
-      else next &= keep;
-    }
-  }
-  // Bytes of the address that it was loaded from.
-  __device__ __forceinline__ uint32_t word(int x, uint32_t s) const {
-    return __builtin_amdgcn_alignbyte(x + 1 < N ? at[(x + 1) / 4][(x + 1) % 4] : next, at[x / 4][x % 4], s);
-  }
-};
-
 // A workgroup takes RT tiles of 16 weight rows and all (up to 16 NC)
 // activation rows; its waves take every waves-th block of columns, the loads
 // of the next one in flight, and their sums are joined through LDS.
@@ -231,7 +192,7 @@ __global__ void __launch_bounds__(NC == 1 ? 1024 : 512) fp8_rows_kernel(const Fp
     Block x;
     auto rest = [&](Codes& x, const uint8_t* p) __attribute__((always_inline)) {
       Unaligned<8> u;
-      u.load(p, min(left, 32));
+      u.load_first(p, min(left, 32));
       if constexpr (ODD) x = u;
       else x = words(u, p);
     };
@@ -591,7 +552,7 @@ __global__ void __launch_bounds__(256) fp8_align_kernel(Fp8Copies g) {
   for (int x = 0; x < 4; ++x) {
     const int c = first + 256 * x;
     if (c + 16 <= g.k) v[x].load(src + c);
-    else v[x].load(src + c, g.k - c);
+    else v[x].load_first(src + c, g.k - c);
   }
   const uint32_t s = (uint32_t)(uintptr_t)src & 3;
 #pragma unroll

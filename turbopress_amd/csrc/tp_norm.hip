@@ -4,13 +4,13 @@
 //   h = x + residual,  y = h / sqrt(mean(h^2) + eps) * weight
 //   scale = max(max |y| / 448, 2^-126),  code = e4m3(y / scale)
 //
-// One pass: a row's h stays in registers (fp32) between its sum of squares and
-// its output, so x and the residual are read once and h, y (or codes) written
-// once; the weight comes from L2.  Nothing is computed to speak of (4 flops per
+// One pass: a row's x and residual stay in registers between its sum of squares
+// and its output, so they are read once and h, y (or codes) written once; the
+// weight comes from L2.  Nothing is computed to speak of (4 flops per
 // element): many rows are bound by HBM, a few by the latency of load, reduction
 // and store.  8192 x 9728 fp16 60 us = 5.3 TB/s (a copy reaches 5.2); 8191 x 9727
-// 80, for no row but every eighth begins on 16 bytes; 2048 x 2560 with a residual
-// and e4m3 output 10.5; 1 x 2560 3.
+// 72, half of its rows off their words; 2048 x 2560 with a residual and e4m3
+// output 10; 1 x 2560 3.
 #include "tp_ops_common.h"
 
 #include <algorithm>
@@ -29,6 +29,7 @@ struct NormArgs {
   int64_t x_outer, x_inner, r_outer, r_inner, ldc, rows;
   int inner, d, nvec, nblocks, waves_per_row;
   int large;  // the inputs are past the caches' size
+  int odd;    // rows of 2-byte elements that do not all begin on words
   float eps;
 };
 
@@ -132,8 +133,43 @@ __global__ void __launch_bounds__(512) rms_norm_kernel(const NormArgs a) {
       for (int j = 0; j < VPT; ++j) rv[j] = load_row8<decltype(once)::value>(res, min(i0 + j * lanes, last), a.d);
     }
   };
-  if (a.large) load(std::true_type{});
-  else load(std::false_type{});
+  // The word behind a vector is the next lane's first (loaded by every lane, 8191
+  // x 9727 fp16 took 79 us, no less than unaligned), but for a wave's or a row's
+  // last lane.  All vectors are loaded, then moved.
+  auto load_odd = [&](auto once) __attribute__((always_inline)) {
+    Unaligned<4> xu[VPT], ru[RES ? VPT : 1];
+    auto get = [&](Unaligned<4>& u, const T* r, int i) __attribute__((always_inline)) {
+      if (8 * i + 8 <= a.d) u.load<decltype(once)::value>(r + 8 * i, i == last || (i0 & (SUB - 1)) == SUB - 1);
+      else u.load_first(r + 8 * i, (a.d - 8 * i) * (int)sizeof(T));
+    };
+    auto moved = [&](Vec<T>& v, Unaligned<4>& u, const T* r, int i) __attribute__((always_inline)) {
+      const uint32_t s = (uint32_t)(uintptr_t)r & 3, behind = from_next_lane(u.at[0][0]);
+      if (i != last && (i0 & (SUB - 1)) != SUB - 1) u.next = behind;
+      const u32x4 w = {u.word(0, s), u.word(1, s), u.word(2, s), u.word(3, s)};
+      __builtin_memcpy(&v, &w, 16);
+    };
+#pragma unroll
+    for (int j = 0; j < VPT; ++j) get(xu[j], x, min(i0 + j * lanes, last));
+    if constexpr (RES) {
+#pragma unroll
+      for (int j = 0; j < VPT; ++j) get(ru[j], res, min(i0 + j * lanes, last));
+    }
+#pragma unroll
+    for (int j = 0; j < VPT; ++j) {
+      moved(xv[j], xu[j], x, min(i0 + j * lanes, last));
+      if constexpr (RES) moved(rv[j], ru[j], res, min(i0 + j * lanes, last));
+    }
+  };
+  if (sizeof(T) == 2 && a.odd) {
+    if constexpr (sizeof(T) == 2) {
+      if (a.large) load_odd(std::true_type{});
+      else load_odd(std::false_type{});
+    }
+  } else if (a.large) {
+    load(std::true_type{});
+  } else {
+    load(std::false_type{});
+  }
   auto sum8 = [&](int j, float* h) __attribute__((always_inline)) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
@@ -327,11 +363,14 @@ template <typename T, int OUT>
 int launch_norm(const NormArgs& a0, hipStream_t s) {
   NormArgs a = a0;
   // Loads past the caches from 128 MB of inputs, half of what the memory side
-  // caches: 8191 x 9727 fp16 80 us against 83, 8192 x 9728 60 against 67, 16384 x
+  // caches: 8192 x 9728 fp16 60 us against 67, 16384 x
   // 2560 with a residual 65 against 66; what the step before has just written is
   // better read from there: 16384 x 1024 with a residual 25.8 against 21.1, 2048 x
   // 2560 13.5 against 9.0, 4096 x 9728 without 33 against 31.
   a.large = a.rows * a.d * (int64_t)sizeof(T) * (a.residual ? 2 : 1) >= (128 << 20);
+  const int64_t at = (int64_t)(uintptr_t)a.x | (int64_t)(uintptr_t)a.residual |
+                     ((a.x_outer | a.x_inner | a.r_outer | a.r_inner) * (int64_t)sizeof(T));
+  a.odd = (at & 3) != 0;
   const NormPlan p = norm_plan(a.rows, a.nvec, device_cu_count());
   if (p.vpt == 0) {
     hipLaunchKernelGGL((rms_norm_long_kernel<T, OUT>), dim3((uint32_t)a.rows), dim3(1024), 0, s, a);

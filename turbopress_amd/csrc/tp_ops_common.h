@@ -34,6 +34,7 @@ __device__ __forceinline__ void store8(T* p, const Vec<T>& r) {
 // The same past the caches: of what is read once and is too large to be in them,
 // and of what is written once.
 typedef u32x4 u32x4_any __attribute__((aligned(1)));
+typedef u32x4 u32x4_words __attribute__((aligned(4)));
 template <typename T>
 __device__ __forceinline__ Vec<T> load8_once(const T* p) {
   u32x4 w[sizeof(T) / 2];
@@ -49,6 +50,57 @@ __device__ __forceinline__ void store8_once(T* p, const Vec<T>& r) {
   __builtin_memcpy(w, &r, sizeof(r));
 #pragma unroll
   for (int i = 0; i < (int)sizeof(T) / 2; ++i) __builtin_nontemporal_store(w[i], reinterpret_cast<u32x4_any*>(p) + i);
+}
+
+// 4 N bytes at any alignment: the words that hold them, loaded as they lie (a
+// word that holds a byte of a row is memory), and moved over by the address's
+// last bits.  Loads off their words take several times as long: the product of
+// 16 rows and 2560 x 9727 e4m3 weights 40 us against 15, the norm of 8191 x 9727
+// fp16 79 against 72 (stores off their words cost little).  ONCE: past the caches.
+template <int N>
+struct Unaligned {
+  static_assert(N % 4 == 0, "");
+  u32x4 at[N / 4];
+  uint32_t next;
+
+  // (own: with the word behind; else the caller gets it from who has it)
+  template <bool ONCE = false>
+  __device__ __forceinline__ void load(const void* p, bool own = true) {
+    const uint32_t s = (uint32_t)(uintptr_t)p & 3;
+    const uint32_t* q = reinterpret_cast<const uint32_t*>(static_cast<const char*>(p) - s);
+#pragma unroll
+    for (int x = 0; x < N / 4; ++x) {
+      const u32x4_words* w = reinterpret_cast<const u32x4_words*>(q) + x;
+      at[x] = ONCE ? __builtin_nontemporal_load(w) : *w;
+    }
+    next = 0;
+    if (own) next = q[s ? N : N - 1];  // (at s = 0 not used)
+  }
+  // The first `left` bytes, then zeros.
+  __device__ __forceinline__ void load_first(const void* p, int left) {
+    const uint32_t s = (uint32_t)(uintptr_t)p & 3;
+    const uint32_t* q = reinterpret_cast<const uint32_t*>(static_cast<const char*>(p) - s);
+    const int n = left > 0 ? left + (int)s : 0;
+#pragma unroll
+    for (int x = 0; x < N; ++x) at[x / 4][x % 4] = 4 * x < n ? q[x] : 0;
+    next = 4 * N < n ? q[N] : 0;
+#pragma unroll
+    for (int x = 0; x <= N; ++x) {
+      const int in = n - 4 * x;  // bytes of the row in this word
+      const uint32_t keep = in >= 4 ? ~0u : in <= 0 ? 0u : (1u << (8 * in)) - 1;
+      if (x < N) at[x / 4][x % 4] &= keep;
+      else next &= keep;
+    }
+  }
+  // Word x of what was loaded; s: the address's last two bits.
+  __device__ __forceinline__ uint32_t word(int x, uint32_t s) const {
+    return __builtin_amdgcn_alignbyte(x + 1 < N ? at[(x + 1) / 4][(x + 1) % 4] : next, at[x / 4][x % 4], s);
+  }
+};
+
+// Lane i takes lane i + 1's value (wave_shl:1), lane 63 keeps its own.
+__device__ __forceinline__ uint32_t from_next_lane(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_update_dpp((int)v, (int)v, 0x130, 0xF, 0xF, false);
 }
 
 template <int CTRL>
