@@ -412,7 +412,8 @@ int tp_rms_norm_fp8(int dtype, int64_t rows, int64_t inner, int64_t d, const voi
  * * sum_{c in b} a[i, c] * w[j, c], plus bias[j]: a e4m3 [m, lda], a_scales
  * fp32 [m, ceil(k / 128)], w e4m3 [n, ldw], w_scales fp32 [ceil(n / 128),
  * ceil(k / 128)], bias (may be NULL) and y of `dtype`, y [m, ldy].  lda and
- * ldw are at least k (and at most 2^22); rows of any alignment are taken; with many
+ * ldw are at least k (and at most 2^22), m at most 2^24, n at most 2^26, k at
+ * most 2^20; rows of any alignment are taken; with many
  * activation rows an operand that is not 16-byte aligned (pointer, lda or ldw)
  * is copied into the workspace first.  Columns [k, ld) are not used, whatever
  * they hold.  Sums are fp32, added in a fixed order; y rounds once.

@@ -758,3 +758,19 @@ def test_c_entry_points_refuse_on_the_host(built_lib):
     assert att(q=None) == att(kc=None) == att(strides=None) == L.TP_ERR_NULL_POINTER
     assert att(q=ctypes.c_void_p(264)) == att(strides=(ctypes.c_int64 * 3)(1024, 64, 4)) == L.TP_ERR_MISALIGNED
     assert att(ws=None) == att(size=need - 1) == att(cnt=None) == att(csize=count - 1) == L.TP_ERR_WORKSPACE
+
+
+def test_c_entry_points_refuse_more_threads_than_a_launch_holds(built_lib):
+    import ctypes
+
+    from turbopress_amd import _lib as L
+    lib, p = L.lib(), ctypes.c_void_p(4096)
+
+    def rot(tokens, hq, d):
+        return lib.tp_rotary(0, tokens, hq, 0, d, d, 0, p, d * hq, d, None, 0, 0, p, 16, p, p, None, None, 0, 0, None, None,
+                             None, None, 0, 1, None, 0, 0, None, None)
+
+    assert rot(1 << 40, 65536, 65536) == rot(1 << 33, 1, 2) == rot(1 << 28, 8, 64) == L.TP_ERR_BAD_DIMS
+    for rows, d in ((1 << 28, 128), (1 << 23, 30000)):
+        assert lib.tp_rms_norm(0, rows, 1, d, p, d, 0, None, 0, 0, p, 1e-6, p, None, None) == L.TP_ERR_BAD_DIMS
+    assert lib.tp_fp8_linear(0, 1, 1 << 27, 16, p, 16, p, p, 16, p, None, p, 1 << 27, None, 0, None) == L.TP_ERR_BAD_DIMS

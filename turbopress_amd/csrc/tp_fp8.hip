@@ -562,7 +562,7 @@ __global__ void __launch_bounds__(256) fp8_align_kernel(Fp8Copies g) {
 }
 
 bool fp8_sizes_ok(int64_t m, int64_t n, int64_t k) {
-  return m >= 0 && n >= 0 && k >= 1 && m <= (1 << 24) && n <= (1 << 28) && k <= (1 << 20);
+  return m >= 0 && n >= 0 && k >= 1 && m <= (1 << 24) && n <= (1 << 26) && k <= (1 << 20);
 }
 
 bool fp8_rows_aligned(const void* p, int64_t ld) { return ((ld | (int64_t)(uintptr_t)p) & 15) == 0; }
@@ -616,7 +616,7 @@ int launch_tiles(Fp8Args g, hipStream_t s) {
   using S = TileShape<WN, WM, TN, TM, WK>;
   g.tiles_m = (int)((g.m + S::kBM - 1) / S::kBM), g.tiles_n = (int)((g.n + S::kBN - 1) / S::kBN);
   const int64_t total = (int64_t)g.tiles_m * g.tiles_n;
-  if (total > 0x7fffffff) return TP_ERR_BAD_DIMS;
+  if (!grid_fits(total, 64 * S::kWaves * WK)) return TP_ERR_BAD_DIMS;
   if (S::kLds > 64 * 1024) allow_dynamic_lds(reinterpret_cast<const void*>(&fp8_tile_kernel<T, WN, WM, TN, TM, WK>), 0);
   hipLaunchKernelGGL((fp8_tile_kernel<T, WN, WM, TN, TM, WK>), dim3((uint32_t)total), dim3(64 * S::kWaves * WK), S::kLds, s, g);
   return launch_status();

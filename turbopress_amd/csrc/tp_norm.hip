@@ -373,6 +373,7 @@ int launch_norm(const NormArgs& a0, hipStream_t s) {
   a.odd = (at & 3) != 0;
   const NormPlan p = norm_plan(a.rows, a.nvec, device_cu_count());
   if (p.vpt == 0) {
+    if (!grid_fits(a.rows, 1024)) return TP_ERR_BAD_DIMS;
     hipLaunchKernelGGL((rms_norm_long_kernel<T, OUT>), dim3((uint32_t)a.rows), dim3(1024), 0, s, a);
     return launch_status();
   }
@@ -380,6 +381,7 @@ int launch_norm(const NormArgs& a0, hipStream_t s) {
   const int threads = p.waves > 4 ? 64 * p.waves : 256;
   const int lanes = p.sub < 64 ? p.sub : 64 * p.waves;
   const int per = threads / lanes;
+  if (!grid_fits((a.rows + per - 1) / per, threads)) return TP_ERR_BAD_DIMS;
   const dim3 grid((uint32_t)((a.rows + per - 1) / per)), block(threads);
 #define TP_NORM(SUB, V)                                                                              \
   do {                                                                                               \

@@ -98,6 +98,9 @@ struct Unaligned {
   }
 };
 
+// A launch holds less than 2^32 threads.
+inline bool grid_fits(int64_t blocks, int threads) { return blocks * threads <= 0xffffffffll; }
+
 // Lane i takes lane i + 1's value (wave_shl:1), lane 63 keeps its own.
 __device__ __forceinline__ uint32_t from_next_lane(uint32_t v) {
   return (uint32_t)__builtin_amdgcn_update_dpp((int)v, (int)v, 0x130, 0xF, 0xF, false);

@@ -125,9 +125,9 @@ int launch_rotary(RotaryArgs a, hipStream_t s) {
   int v = 8;
   while (v > 1 && ((a.rd / 2) % v || (a.d - a.rd) % (2 * v))) v /= 2;
   a.units = a.d / (2 * v), a.rot_units = a.rd / (2 * v);
-  const int64_t total = a.tokens * (a.hq + a.hk + a.hv) * a.units;
-  const int64_t blocks = (total + 255) / 256;
-  if (blocks > 0x7fffffff) return TP_ERR_BAD_DIMS;
+  const int64_t each = (int64_t)(a.hq + a.hk + a.hv) * a.units;  // units of a token
+  if (a.tokens > 0xffffff00ll / each) return TP_ERR_BAD_DIMS;    // (a launch holds less than 2^32 threads)
+  const int64_t blocks = (a.tokens * each + 255) / 256;
   const dim3 grid((uint32_t)blocks), block(256);
   if (v == 8) hipLaunchKernelGGL((rotary_kernel<T, 8>), grid, block, 0, s, a);
   else if (v == 4) hipLaunchKernelGGL((rotary_kernel<T, 4>), grid, block, 0, s, a);
