@@ -134,3 +134,44 @@ def test_reciprocal_division_is_exact_below_its_bound():
         xs = np.array([top, top - 1, top - d + 1, (top // d) * d, (top // d) * d - 1], dtype=np.uint64)
         xs = xs[xs * np.uint64(d) < np.uint64(1 << 32)]
         assert np.array_equal(udiv(xs, d), xs // np.uint64(d)), d
+
+
+def test_a_capture_never_shares_the_eager_workspace(monkeypatch):
+    """A stream with an eager workspace that is large enough: each capture on it
+    gets a buffer of its own all the same (two graphs, or a graph beside eager
+    work, may run at once), one for the whole capture; attention's counters too."""
+    from turbopress_amd import paged
+    monkeypatch.setattr(hk, "_WORKSPACES", {})
+    monkeypatch.setattr(hk, "_CAPTURED_WORKSPACES", {})
+    monkeypatch.setattr(hk, "_RETIRED_WORKSPACES", [])
+    capture = 0
+
+    class S:
+        cuda_stream = 1234
+
+    class Lib:
+        @staticmethod
+        def tp_stream_capture_id(stream):
+            assert stream == 1234
+            return capture
+
+    empty = torch.empty
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda index=None: S())
+    monkeypatch.setattr(torch.cuda, "is_available", lambda: True)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: capture > 0)
+    monkeypatch.setattr(hk._lib, "lib", lambda: Lib)
+    monkeypatch.setattr(torch, "zeros", lambda n, dtype, device: empty(n, dtype=dtype))
+    monkeypatch.setattr(torch, "empty", lambda n, dtype, device: empty(n, dtype=dtype))
+    eager = hk.shared_workspace("cuda:0", 5000)
+    held = [eager]
+    for capture in (7, 8):
+        mine = hk.shared_workspace("cuda:0", 1000)
+        assert all(mine is not other for other in held)
+        assert hk.shared_workspace("cuda:0", 500) is mine
+        _, counters, buffers = paged._workspace(0, 1234, 4096, 256)
+        assert counters == mine.data_ptr() and buffers[1] is mine
+        larger = hk.shared_workspace("cuda:0", 3000)
+        assert larger.numel() >= 3000 and larger is not eager and hk.shared_workspace("cuda:0", 3000) is larger
+        held += [mine, larger]
+    capture = 0
+    assert hk.shared_workspace("cuda:0", 5000) is eager

@@ -193,8 +193,8 @@ def workspace_bytes(n: int) -> tuple:
 # launched on that stream.  The kernels leave it zero when they finish, so
 # launches in stream order can share it; launches that overlap on one
 # workspace (two streams would need two) are not allowed, hence one per
-# stream.  A workspace that grows is replaced, and the old one stays alive:
-# a captured graph may still name it.
+# stream (and one per capture, below).  A workspace that grows is replaced, and
+# the old one stays alive: a caller may still hold its address.
 _WORKSPACES: dict = {}
 _RETIRED_WORKSPACES: list = []
 _WS_ALIGN = 256
@@ -204,25 +204,31 @@ def _aligned(nbytes: int) -> int:
     return (nbytes + _WS_ALIGN - 1) // _WS_ALIGN * _WS_ALIGN
 
 
-# Workspaces made while a graph was being captured, by (device, stream): the
-# capture's id and its buffers.  Their zeros are nodes of that graph, so only
+# Workspaces of the capture that a stream is, or was last, part of, by (device,
+# stream): its id and its buffers.  Their zeros are nodes of that graph, so only
 # that capture may share them: another graph replayed before it would find
-# whatever the memory held.
+# whatever the memory held.  A capture takes no eager buffer either: its graph
+# may be replayed on another stream, beside another graph or eager work.
 _CAPTURED_WORKSPACES: dict = {}
 
 
+def _capturing() -> bool:
+    try:
+        return torch.cuda.is_current_stream_capturing()
+    except RuntimeError:  # (no GPU; asking for one first takes 1 us of every call)
+        return False
+
+
 def shared_workspace(device, nbytes: int) -> Tensor:
-    """The zeroed split-K workspace of `device` and its current stream, at
-    least `nbytes` long (allocated or grown on first need)."""
+    """The zeroed split-K workspace of `device` and its current stream, or of
+    the capture that the stream is part of, at least `nbytes` long (allocated or
+    grown on first need)."""
     dev = torch.device(device)
     index = dev.index if dev.index is not None else torch.cuda.current_device()
     stream = torch.cuda.current_stream(index).cuda_stream
     key = (index, stream)
-    ws = _WORKSPACES.get(key)
-    if ws is not None and ws.numel() >= nbytes:
-        return ws
     new = max(_aligned(nbytes), _WS_ALIGN)
-    if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
+    if _capturing():
         capture = _lib.lib().tp_stream_capture_id(stream)
         held = _CAPTURED_WORKSPACES.get(key)
         if held is None or held[0] != capture:
@@ -230,6 +236,9 @@ def shared_workspace(device, nbytes: int) -> Tensor:
         if not held[1] or held[1][-1].numel() < nbytes:
             held[1].append(torch.zeros(new, dtype=torch.uint8, device=torch.device("cuda", index)))
         return held[1][-1]
+    ws = _WORKSPACES.get(key)
+    if ws is not None and ws.numel() >= nbytes:
+        return ws
     if ws is not None:
         _RETIRED_WORKSPACES.append(ws)
     ws = _WORKSPACES[key] = torch.zeros(new, dtype=torch.uint8, device=torch.device("cuda", index))

@@ -246,8 +246,8 @@ def rotary_append(q: Tensor, k: Tensor, v: Tensor, table: Tensor, positions: Ten
 
 # Workspaces of paged_attention by (device index, stream): a buffer whose first
 # bytes are the counters, zero between calls, and how many those are.  Calls in
-# stream order share one; a graph's capture makes its own (the buffers below are
-# a running program's, the graph's have to last as long as it does).
+# stream order share one; a graph's capture makes its own, whatever its stream
+# has here (a graph may be replayed beside eager calls and other graphs).
 _WORKSPACES: dict = {}
 _COUNTERS = 1 << 16  # bytes of counters at least
 
@@ -264,7 +264,7 @@ def _workspace(index: int, stream: int, need: int, count: int) -> tuple:
     if torch.cuda.is_current_stream_capturing():
         dev = torch.device("cuda", index)
         ws = torch.empty(need, dtype=torch.uint8, device=dev)
-        counters = hk.shared_workspace(dev, count)  # zero between launches, as the split-K sums' counters
+        counters = hk.shared_workspace(dev, count)  # the capture's own; zero between launches, as split-K sums leave it
         return ws.data_ptr(), counters.data_ptr(), (ws, counters)
     got = _WORKSPACES.get((index, stream))
     if got is None or got[1] < count or got[0].numel() - got[1] < need:
