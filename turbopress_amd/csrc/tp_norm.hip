@@ -78,6 +78,22 @@ __device__ __forceinline__ float max_abs8(const float* v) {
 
 __device__ __forceinline__ float scale_of(float amax) { return MaxNanOp::of(amax / kE4m3Max, kLeastScale); }
 
+// y / s as a division rounds it (codes at ties depend on its last bit), with one
+// reciprocal for all that share s: the product with 1 / s is off by a unit or so,
+// and its remainder q s - y, exact in an FMA, sets it right (Markstein's
+// method; zeros keep their signs).  A division's own steps, per element, are
+// about ten instructions; these are three.
+struct Divisor {
+  float s, inv;
+  __device__ __forceinline__ explicit Divisor(float scale) : s(scale), inv(1.0f / scale) {
+    if (inv == 0.0f) s = 0.0f;  // (an infinite scale: zeros, as finite / infinite, and NaN of infinite y)
+  }
+  __device__ __forceinline__ float of(float y) const {
+    const float q = y * inv;
+    return fmaf(-fmaf(q, s, -y), inv, q);
+  }
+};
+
 __device__ __forceinline__ size_t row_offset(int64_t row, int inner, int64_t outer_stride, int64_t inner_stride) {
   const int64_t o = row / inner;
   return (size_t)(o * outer_stride + (row - o * inner) * inner_stride);
@@ -242,9 +258,9 @@ __global__ void __launch_bounds__(512) rms_norm_kernel(const NormArgs a) {
         s = scale_of(reduce16<MaxNanOp>(max_abs8(y)));
         if (live && i <= last && (i & 15) == 0) a.scales[(size_t)row * a.nblocks + (i >> 4)] = s;
       }
-      const float is = 1.0f / s;
+      const Divisor by(s);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) y[e] *= is;
+      for (int e = 0; e < 8; ++e) y[e] = by.of(y[e]);
       if (live && i <= last) __builtin_nontemporal_store(to_e4m3(y), reinterpret_cast<u32x2*>(a.codes + (size_t)row * a.ldc + 8 * i));
     }
   }
@@ -322,9 +338,9 @@ __global__ void __launch_bounds__(1024) rms_norm_long_kernel(const NormArgs a) {
         s = scale_of(reduce16<MaxNanOp>(max_abs8(y)));
         if (in && (i & 15) == 0) a.scales[(size_t)row * a.nblocks + (i >> 4)] = s;
       }
-      const float is = 1.0f / s;
+      const Divisor by(s);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) y[e] *= is;
+      for (int e = 0; e < 8; ++e) y[e] = by.of(y[e]);
       if (in) *reinterpret_cast<u32x2*>(a.codes + (size_t)row * a.ldc + 8 * i) = to_e4m3(y);
     }
   }
