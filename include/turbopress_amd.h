@@ -412,10 +412,11 @@ int tp_rms_norm_fp8(int dtype, int64_t rows, int64_t inner, int64_t d, const voi
  * * sum_{c in b} a[i, c] * w[j, c], plus bias[j]: a e4m3 [m, lda], a_scales
  * fp32 [m, ceil(k / 128)], w e4m3 [n, ldw], w_scales fp32 [ceil(n / 128),
  * ceil(k / 128)], bias (may be NULL) and y of `dtype`, y [m, ldy].  lda and
- * ldw are at least k (and at most 2^22), m at most 2^24, n at most 2^26, k at
- * most 2^20; rows of any alignment are taken; with many
- * activation rows an operand that is not 16-byte aligned (pointer, lda or ldw)
- * is copied into the workspace first.  Columns [k, ld) are not used, whatever
+ * ldw are at least k (and at most 2^36), m at most 2^24, n at most 2^26, k at
+ * most 2^20; rows of any alignment and distance are taken; with many
+ * activation rows an operand that is not 16-byte aligned (pointer, lda or ldw),
+ * or whose rows are more than 2^22 apart, is copied into the workspace first.
+ * Columns [k, ld) are not used, whatever
  * they hold.  Sums are fp32, added in a fixed order; y rounds once.
  * The workspace (tp_fp8_workspace_bytes, 16-byte aligned; NULL when that is 0)
  * may hold anything.  m = 0 or n = 0 does nothing. */
@@ -424,7 +425,7 @@ int tp_fp8_linear(int dtype, int64_t m, int64_t n, int64_t k, const uint8_t* a, 
                   void* workspace, int64_t workspace_bytes, void* stream);
 
 /* Bytes of workspace of a tp_fp8_linear call of these operands (0: none, as for
- * few rows and for aligned operands; -1: sizes it does not take).  The
+ * few rows and for operands that need no copy; -1: sizes it does not take).  The
  * pointers are not read. */
 int64_t tp_fp8_workspace_bytes(int64_t m, int64_t n, int64_t k, const uint8_t* a, int64_t lda, const uint8_t* w,
                                int64_t ldw);

@@ -68,3 +68,42 @@ def test_norm_codes_of_zeros_and_infinities(cuda, block):
     assert torch.equal(codes.cpu().float().nan_to_num(7), want.float().nan_to_num(7))
     finite = ~torch.isnan(want.float())
     assert torch.equal(codes.cpu().view(torch.uint8)[finite], want.view(torch.uint8)[finite])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m", [1, 4, 20, 40, 100])
+def test_fp8_linear_rows_far_apart(cuda, m):
+    """The last token of each of m prompts of 2048: rows 5 242 880 codes apart,
+    through operand registers and through tiles, with weights as far apart."""
+    from turbopress_amd import fp8_linear
+    k = 2560
+    a, sa, w, sw = _fp8_case(_gen(m), m, 7000, k)
+    far = torch.full((m, 2048, k), 0x7f, dtype=torch.uint8, device="cuda").view(F8)
+    far[:, -1] = a
+    scales = sa[:, None].expand(m, 3, sa.shape[1])[:, -1]
+    assert far[:, -1].stride(0) == 2048 * k
+    for n in (300, 7000):
+        got = fp8_linear(far[:, -1], scales, w[:n], sw[:-(-n // 128)], out_dtype=F32)
+        if not 16 < m <= 32:  # (of those, wide weights' rows as they lie and copied ones take different paths)
+            assert torch.equal(got, fp8_linear(a, sa, w[:n], sw[:-(-n // 128)], out_dtype=F32))
+        want, size = O.fp8_linear(a, sa, w[:n], sw[:-(-n // 128)])
+        _within(got, want, _fp8_tol(want, size, k, F32))
+    wide = torch.full((70, 2048, k), 0x7f, dtype=torch.uint8, device="cuda").view(F8)
+    wide[:, -1] = w[:70]
+    assert torch.equal(fp8_linear(a, sa, wide[:, -1], sw[:1], out_dtype=F32), fp8_linear(a, sa, w[:70], sw[:1], out_dtype=F32))
+
+
+def test_fp8_entry_points_take_rows_far_apart(built_lib):
+    """A row stride above 2^22 is copied for the tiles and read in place by few
+    rows; only offsets past 64 bits are refused."""
+    from turbopress_amd import _lib as L
+    lib, p, far = built_lib, ctypes.c_void_p(256), 5242880
+    assert lib.tp_fp8_workspace_bytes(1, 300, 2560, p, far, p, 2560) == 0
+    assert lib.tp_fp8_workspace_bytes(100, 300, 2560, p, far, p, 2560) == 100 * 2560
+    assert lib.tp_fp8_workspace_bytes(100, 300, 2560, p, 2560, p, far) == 300 * 2560
+
+    def fp8(lda, ldw, m=100):
+        return lib.tp_fp8_linear(0, m, 300, 2560, p, lda, p, p, ldw, p, None, p, 300, None, 0, None)
+
+    assert fp8(far, 2560) == fp8(2560, far) == L.TP_ERR_WORKSPACE
+    assert fp8(1 << 40, 2560) == fp8(2560, 1 << 40) == fp8(1 << 40, 2560, 1) == L.TP_ERR_BAD_DIMS

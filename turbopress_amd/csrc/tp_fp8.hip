@@ -561,11 +561,16 @@ __global__ void __launch_bounds__(256) fp8_align_kernel(Fp8Copies g) {
       *reinterpret_cast<u32x4*>(dst + first + 256 * x) = u32x4{v[x].word(0, s), v[x].word(1, s), v[x].word(2, s), v[x].word(3, s)};
 }
 
+constexpr int64_t kMaxLd = (int64_t)1 << 36;  // (times 2^26 rows: offsets of 64 bits)
+
 bool fp8_sizes_ok(int64_t m, int64_t n, int64_t k) {
   return m >= 0 && n >= 0 && k >= 1 && m <= (1 << 24) && n <= (1 << 26) && k <= (1 << 20);
 }
 
-bool fp8_rows_aligned(const void* p, int64_t ld) { return ((ld | (int64_t)(uintptr_t)p) & 15) == 0; }
+// Rows that the tiles load as they lie: 16-byte pieces, 32-bit offsets inside a
+// tile (320 rows of up to 2^22 bytes).  Others are copied for them; the rows
+// kernel, whose offsets have 64 bits, takes any.
+bool fp8_rows_tiled(const void* p, int64_t ld) { return ((ld | (int64_t)(uintptr_t)p) & 15) == 0 && ld <= (1 << 22); }
 
 template <typename T, int NC, int RT, bool ODD>
 void launch_rows(const Fp8Args& g, int waves, hipStream_t s) {
@@ -581,11 +586,11 @@ void launch_rows(const Fp8Args& g, int waves, hipStream_t s) {
 //   64 rows  4096, 2560: 10.3 / 10.1  2560, 9728: 28.8 / 24.0   9728, 2560: 20.2 / 10.0
 // so 17..32 rows take it for up to 6144 weight rows (the tiles' time is their
 // chain of blocks until their count fills the GPU), more rows never.  Operands
-// that do not begin on 16 bytes are copied for the tiles: 32 rows, 7000, 100: 3.8
+// that are not fp8_rows_tiled are copied for the tiles: 32 rows, 7000, 100: 3.8
 // / 9.4  16384, 1000: 11.4 / 19.2  16000, 5003: 57.6 / 51.4, so they take it up to
 // 32 MB of weights, halfway.
-bool fp8_takes_rows(int64_t m, int64_t n, int64_t k, bool aligned) {
-  return m <= 16 || (m <= 32 && (n <= 6144 || (!aligned && n * k <= (32 << 20))));
+bool fp8_takes_rows(int64_t m, int64_t n, int64_t k, bool tiled) {
+  return m <= 16 || (m <= 32 && (n <= 6144 || (!tiled && n * k <= (32 << 20))));
 }
 
 template <typename T>
@@ -674,9 +679,9 @@ using namespace tp;
 extern "C" int64_t tp_fp8_workspace_bytes(int64_t m, int64_t n, int64_t k, const uint8_t* a, int64_t lda,
                                           const uint8_t* w, int64_t ldw) {
   if (!fp8_sizes_ok(m, n, k)) return -1;
-  const bool aligned = fp8_rows_aligned(a, lda) && fp8_rows_aligned(w, ldw);
-  if (m == 0 || n == 0 || fp8_takes_rows(m, n, k, aligned)) return 0;
-  return (fp8_rows_aligned(a, lda) ? 0 : align_bytes(m, k)) + (fp8_rows_aligned(w, ldw) ? 0 : align_bytes(n, k));
+  const bool tiled = fp8_rows_tiled(a, lda) && fp8_rows_tiled(w, ldw);
+  if (m == 0 || n == 0 || fp8_takes_rows(m, n, k, tiled)) return 0;
+  return (fp8_rows_tiled(a, lda) ? 0 : align_bytes(m, k)) + (fp8_rows_tiled(w, ldw) ? 0 : align_bytes(n, k));
 }
 
 extern "C" int tp_fp8_linear(int dtype, int64_t m, int64_t n, int64_t k, const uint8_t* a, int64_t lda,
@@ -684,12 +689,12 @@ extern "C" int tp_fp8_linear(int dtype, int64_t m, int64_t n, int64_t k, const u
                              const void* bias, void* y, int64_t ldy, void* workspace, int64_t workspace_bytes,
                              void* stream) {
   if (!dtype_ok(dtype)) return TP_ERR_BAD_TYPE;
-  if (!fp8_sizes_ok(m, n, k) || lda < k || ldw < k || ldy < n || lda > (1 << 22) || ldw > (1 << 22)) return TP_ERR_BAD_DIMS;
+  if (!fp8_sizes_ok(m, n, k) || lda < k || ldw < k || ldy < n || lda > kMaxLd || ldw > kMaxLd) return TP_ERR_BAD_DIMS;
   if (m == 0 || n == 0) return TP_OK;
   if (!a || !a_scales || !w || !w_scales || !y) return TP_ERR_NULL_POINTER;
   const uintptr_t mask = dtype_bytes(dtype) - 1;
   if ((((uintptr_t)a_scales | (uintptr_t)w_scales) & 3) || (((uintptr_t)bias | (uintptr_t)y) & mask)) return TP_ERR_MISALIGNED;
-  const bool rows = fp8_takes_rows(m, n, k, fp8_rows_aligned(a, lda) && fp8_rows_aligned(w, ldw));
+  const bool rows = fp8_takes_rows(m, n, k, fp8_rows_tiled(a, lda) && fp8_rows_tiled(w, ldw));
   const int64_t need = tp_fp8_workspace_bytes(m, n, k, a, lda, w, ldw);
   if (need > 0 && (!workspace || workspace_bytes < need)) return TP_ERR_WORKSPACE;
   if (need > 0 && ((uintptr_t)workspace & 15)) return TP_ERR_MISALIGNED;
@@ -698,7 +703,7 @@ extern "C" int tp_fp8_linear(int dtype, int64_t m, int64_t n, int64_t k, const u
     Fp8Copies c{{a, w}, {nullptr, nullptr}, {lda, ldw}, {0, 0}, (k + 15) & ~(int64_t)15, (int)k};
     uint8_t* free = static_cast<uint8_t*>(workspace);
     auto align = [&](int x, const uint8_t*& p, int64_t& from, int64_t rows) {
-      if (fp8_rows_aligned(p, from)) return;
+      if (fp8_rows_tiled(p, from)) return;
       c.dst[x] = free, c.rows[x] = rows;
       p = free, from = c.ld;
       free += rows * c.ld;
