@@ -107,3 +107,25 @@ def test_fp8_entry_points_take_rows_far_apart(built_lib):
 
     assert fp8(far, 2560) == fp8(2560, far) == L.TP_ERR_WORKSPACE
     assert fp8(1 << 40, 2560) == fp8(2560, 1 << 40) == fp8(1 << 40, 2560, 1) == L.TP_ERR_BAD_DIMS
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("d", [64, 128])
+def test_paged_attention_keeps_small_weights(cuda, d, dtype):
+    """Tokens of value zero whose scores are the largest, then 8000 whose
+    weights are 2^-26 of theirs and which alone make up the output."""
+    from turbopress_amd import paged_attention
+    g = _gen(d)
+    n, first, batch = 8192, 256, 512  # (more heads than workgroups: a wave meets both kinds)
+    k = torch.zeros(n // 64, 64, 1, d, dtype=dtype, device="cuda")
+    v = (3e4 + 1e4 * torch.rand(n // 64, 64, 1, d, generator=g, device="cuda")).to(dtype)
+    k.view(n, d)[:first, 0], v.view(n, d)[:first] = 18, 0
+    bt = torch.arange(n // 64, dtype=torch.int32, device="cuda").expand(batch, -1).contiguous()
+    lengths = torch.full((batch,), n, dtype=torch.int32, device="cuda")
+    q = torch.zeros(batch, 1, d, dtype=dtype, device="cuda")
+    q[:, :, 0] = 1
+    want, size, dots = O.paged_attention(q[:1], k, v, bt[:1], lengths[:1], 1.0)
+    assert 0.005 < want.min() and want.max() < 0.05
+    got = paged_attention(q, k, v, bt, lengths, scale=1.0)
+    _within(got, want.expand(batch, -1, -1), _attention_tol(want, size, dots, d, dtype))

@@ -74,11 +74,16 @@ __device__ __forceinline__ V load16(const void* p) {
   return __builtin_nontemporal_load((const __attribute__((address_space(1))) V*)p);
 }
 
+// kUnit: of the probabilities, the sums and the outputs of a state (a power of
+// two, which the last division takes out).  In fp16 the largest is 2^15, so that
+// those down to 2^-39 of it count (of a largest of 1 those below 2^-25 would be
+// in the sum alone); bf16 has the exponents of fp32.
 template <typename T>
 struct Mma;
 template <>
 struct Mma<f16_t> {
   typedef f16x8 v8;
+  static constexpr float kUnit = 0x1p15f;
   __device__ __forceinline__ static f32x4 mul(v8 a, v8 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
   }
@@ -86,6 +91,7 @@ struct Mma<f16_t> {
 template <>
 struct Mma<bf16_t> {
   typedef bf16x8 v8;
+  static constexpr float kUnit = 1.0f;
   __device__ __forceinline__ static f32x4 mul(v8 a, v8 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
   }
@@ -357,7 +363,7 @@ __global__ void __launch_bounds__(64 * paged_waves<DP>(), 1) paged_attention_ker
       for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float x = __builtin_amdgcn_exp2f(s[h][e] - top);
+          const float x = __builtin_amdgcn_exp2f(s[h][e] - top) * Mma<T>::kUnit;
           l += x;
           p[4 * h + e] = (T)x;
         }
