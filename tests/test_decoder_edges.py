@@ -129,3 +129,64 @@ def test_paged_attention_keeps_small_weights(cuda, d, dtype):
     assert 0.005 < want.min() and want.max() < 0.05
     got = paged_attention(q, k, v, bt, lengths, scale=1.0)
     _within(got, want.expand(batch, -1, -1), _attention_tol(want, size, dots, d, dtype))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("d", [64, 80, 128, 256])
+def test_paged_attention_of_values_that_cancel(cuda, d, dtype):
+    """Values of either sign whose weighted mean nearly vanishes: the error is of
+    the fp32 scores and exponentials and of the output's rounding, not of the
+    probabilities' (held in two pieces of the cache's type, 2^-16 of each at
+    least)."""
+    from turbopress_amd import paged_attention
+    g = _gen(d)
+    lengths = [2, 5, 33, 400, 3000]
+    page, width = 16, -(-3000 // 16)
+    bt = torch.randperm(5 * width, generator=g, device="cuda").view(5, width).int()
+    k = (_randn(g, 5 * width, page, 2, d) * d ** -0.25).to(dtype)
+    v = (1 - 2 * torch.randint(0, 2, (5 * width, page, 2, d), generator=g, device="cuda")).to(dtype)
+    n = torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    q = _randn(g, 5, 6, d, dtype=dtype)
+    want, size, dots = O.paged_attention(q, k, v, bt, n)
+    u, least = (2.0 ** -11, 2.0 ** -24) if dtype == F16 else (2.0 ** -8, 2.0 ** -130)
+    near = 2 * (d + 8) * E * dots[..., None] + 2.0 ** -18 + 2.0 ** -16
+    _within(paged_attention(q, k, v, bt, n), want, u * want.abs() + near * size + least)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_paged_attention_infinite_values(cuda, dtype):
+    """A value that is infinite makes its column so where its token has weight,
+    whatever that weight is; the other columns and sequences are as without it."""
+    from turbopress_amd import paged_attention
+    g = _gen(2)
+    k, v = (_randn(g, 40, 16, 1, 64, dtype=dtype) for _ in "kv")
+    bt = torch.arange(40, dtype=torch.int32, device="cuda").view(2, 20)
+    n = torch.tensor([300, 1], dtype=torch.int32, device="cuda")
+    q = _randn(g, 2, 4, 64, dtype=dtype)
+    clean = paged_attention(q, k, v, bt, n)
+    v[20, 0, 0, 9] = -math.inf  # (the second sequence's only token: its weight is 1)
+    v[3, 5, 0, 7] = math.inf
+    got = paged_attention(q, k, v, bt, n)
+    assert (got[0, :, 7] == math.inf).all() and (got[1, :, 9] == -math.inf).all()
+    got[0, :, 7], got[1, :, 9] = clean[0, :, 7], clean[1, :, 9]
+    assert torch.equal(got, clean)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_paged_attention_keys_without_weight(cuda, dtype):
+    """Tokens whose keys are at -infinity have no weight at all, whatever their values."""
+    from turbopress_amd import paged_attention
+    g = _gen(3)
+    k, v = (_randn(g, 700, 16, 1, 64, dtype=dtype) for _ in "kv")
+    bt = torch.arange(700, dtype=torch.int32, device="cuda").view(2, 350)
+    n = torch.tensor([5600, 4001], dtype=torch.int32, device="cuda")
+    q = _randn(g, 2, 4, 64, dtype=dtype).abs()
+    none = torch.rand(700, 16, generator=g, device="cuda") < 0.9
+    k[none] = -math.inf
+    v[none] = 0
+    want = paged_attention(q, k, v, bt, n)
+    v[none] = 65504
+    assert torch.equal(paged_attention(q, k, v, bt, n), want)
