@@ -450,7 +450,10 @@ int64_t tp_fp8_workspace_bytes(int64_t m, int64_t n, int64_t k, const uint8_t* a
  * A token of a negative position is padding: its outputs are zero and nothing
  * is written into the caches.  A position >= n_positions gives NaN outputs and
  * writes nothing; a sequence outside [0, n_sequences), a position past
- * table_width pages and a page outside [0, n_pages) write nothing. */
+ * table_width pages and a page outside [0, n_pages) write nothing.
+ *
+ * hq, hk and d are at most 65536; a token of 2^31 pairs (of all its heads) or a
+ * call of 2^32 may be refused. */
 int tp_rotary(int dtype, int64_t tokens, int64_t hq, int64_t hk, int64_t d, int64_t rotary_dim, int interleaved,
               const void* q, int64_t q_token, int64_t q_head, const void* k, int64_t k_token, int64_t k_head,
               const float* table, int64_t n_positions, const int64_t* positions, void* q_out, void* k_out,

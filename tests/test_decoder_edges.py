@@ -190,3 +190,12 @@ def test_paged_attention_keys_without_weight(cuda, dtype):
     want = paged_attention(q, k, v, bt, n)
     v[none] = 65504
     assert torch.equal(paged_attention(q, k, v, bt, n), want)
+
+
+def test_rotary_refuses_tokens_of_more_than_31_bits_of_pairs(built_lib):
+    """One token of 65536 + 40 heads of 65536 columns, of which two turn."""
+    from turbopress_amd import _lib as L
+    p, d = ctypes.c_void_p(4096), 65536
+    st = built_lib.tp_rotary(0, 1, 65536, 40, d, 2, 0, p, 65536 * d, d, p, 40 * d, d, p, 8, p, p, p, None, 0, 0, None, None,
+                             None, None, 0, 1, None, 0, 0, None, None)
+    assert st == L.TP_ERR_BAD_DIMS

@@ -126,7 +126,9 @@ int launch_rotary(RotaryArgs a, hipStream_t s) {
   while (v > 1 && ((a.rd / 2) % v || (a.d - a.rd) % (2 * v))) v /= 2;
   a.units = a.d / (2 * v), a.rot_units = a.rd / (2 * v);
   const int64_t each = (int64_t)(a.hq + a.hk + a.hv) * a.units;  // units of a token
-  if (a.tokens > 0xffffff00ll / each) return TP_ERR_BAD_DIMS;    // (a launch holds less than 2^32 threads)
+  // (a launch holds less than 2^32 threads; a token's are counted in 31 bits, for
+  // unsigned division made 32768 tokens of 12 heads of 64 2 % slower)
+  if (each > 0x7fffffff || a.tokens > 0xffffff00ll / each) return TP_ERR_BAD_DIMS;
   const int64_t blocks = (a.tokens * each + 255) / 256;
   const dim3 grid((uint32_t)blocks), block(256);
   if (v == 8) hipLaunchKernelGGL((rotary_kernel<T, 8>), grid, block, 0, s, a);
