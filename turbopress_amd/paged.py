@@ -37,8 +37,9 @@ def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: dict | N
     original / low_freq_factor / factor, below original / high_freq_factor
     kept, between them blended); ``yarn`` (frequencies that turn fewer than
     beta_slow times over the original length / factor, more than beta_fast
-    times kept, a ramp between; cosines and sines times attention_factor or
-    0.1 ln(factor) + 1)."""
+    times kept, a ramp between; cosines and sines times attention_factor or, with
+    t(m) = 0.1 m ln(factor) + 1, t(mscale) / t(mscale_all_dim) where both are
+    given and t(1) where not)."""
     if rotary_dim < 2 or rotary_dim % 2:
         raise ValueError(f"rotary_dim must be even and at least 2, got {rotary_dim}")
     half = rotary_dim // 2
@@ -72,7 +73,11 @@ def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: dict | N
     ramp = ((torch.arange(half, dtype=torch.float64) - lo) / max(hi - lo, 1e-3)).clamp(0, 1)
     attention = scaling.get("attention_factor")
     if attention is None:
-        attention = 0.1 * math.log(factor) + 1.0 if factor > 1 else 1.0
+        def temperature(m):
+            return 0.1 * m * math.log(factor) + 1.0 if factor > 1 else 1.0
+
+        m, m_all = scaling.get("mscale"), scaling.get("mscale_all_dim")
+        attention = temperature(m) / temperature(m_all) if m and m_all else temperature(1.0)
     return freq * (1 - ramp) + freq / factor * ramp, float(attention)
 
 
