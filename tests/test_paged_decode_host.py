@@ -19,3 +19,34 @@ def test_yarn_keys_match_transformers(keys, factor):
     got, got_factor = rotary_frequencies(64, 1e4, scaling)
     assert abs(got_factor - want_factor) < 1e-6
     assert ((got - want.double()).abs() <= 2.0 ** -21 * want.double()).all()
+
+
+TINY = dict(vocab_size=64, hidden_size=64, intermediate_size=128, num_hidden_layers=4, num_attention_heads=4,
+            num_key_value_heads=2, max_position_embeddings=128, pad_token_id=0, bos_token_id=1, eos_token_id=2)
+
+
+def tiny_model(family, **kw):
+    from transformers import AutoConfig, AutoModelForCausalLM
+    return AutoModelForCausalLM.from_config(AutoConfig.for_model(family, **TINY, **kw)).half()
+
+
+@pytest.mark.parametrize("family", ["smollm3", "granite", "ernie4_5", "olmo2", "phi3", "cohere", "seed_oss"])
+def test_families_with_other_layers_are_refused(family):
+    from turbopress_amd.paged_decode import PagedDecoder
+    with pytest.raises(ValueError, match=family):
+        PagedDecoder(tiny_model(family), 1, 64, fp8_head=False)
+
+
+@pytest.mark.parametrize("family,kw,windows", [
+    ("llama", {}, [0] * 4), ("mistral", {"sliding_window": 6}, [6] * 4), ("mistral", {"sliding_window": None}, [0] * 4),
+    ("qwen2", {"use_sliding_window": True, "sliding_window": 6, "max_window_layers": 2}, [0, 0, 6, 6]),
+    ("qwen3", {"use_sliding_window": True, "sliding_window": 6, "max_window_layers": 1, "head_dim": 16}, [0, 6, 6, 6])])
+def test_windows_of_the_layers(family, kw, windows):
+    from turbopress_amd.paged_decode import PagedDecoder
+    assert PagedDecoder(tiny_model(family, **kw), 1, 64, fp8_head=False).windows == windows
+
+
+def test_a_rotary_share_that_the_family_ignores_is_refused():
+    from turbopress_amd.paged_decode import PagedDecoder
+    with pytest.raises(ValueError, match="partial_rotary_factor"):
+        PagedDecoder(tiny_model("llama", partial_rotary_factor=0.5), 1, 64, fp8_head=False)

@@ -3,8 +3,8 @@ operators between the packed projections.
 
 The reference decodes one sequence over transformers' StaticCache and leaves
 everything but the projections to the HF decoder
-(``scripts/graph_decode_bench.py:39-118``).  ``PagedDecoder`` runs a packed
-Llama- or Qwen3-shaped causal LM's layers itself: norm and residual, projections
+(``scripts/graph_decode_bench.py:39-118``).  ``PagedDecoder`` runs the layers of
+a packed Llama, Mistral, Qwen2 or Qwen3 causal LM itself: norm and residual, projections
 (``PackedTCQLinear``), norms of the heads, rotary positions and the cache's
 writes, attention over each sequence's pages, and the dense head in 8 bits.  Its
 decode step takes one token of every sequence, has no host synchronisation and
@@ -84,9 +84,24 @@ def _rope(config) -> tuple:
     return float(base), scaling, float(share)
 
 
+# Families whose layers are what PagedDecoder runs: projections, norms of the
+# heads where there are any, halves of the heads turned, a gated MLP, two norms.
+# Others with the same modules are not (layers without positions, multipliers of
+# embeddings, residuals or logits, pairs in place of halves, norms elsewhere).
+_FAMILIES = ("llama", "mistral", "qwen2", "qwen3")
+
+
+def _windows(config, layers) -> list:
+    """The sliding window of each layer's attention (0: none)."""
+    if config.model_type == "mistral":  # (one for all layers, which do not name it)
+        return [getattr(config, "sliding_window", None) or 0] * len(layers)
+    return [getattr(layer.self_attn, "sliding_window", None) or 0 for layer in layers]
+
+
 class PagedDecoder:
-    """A causal LM (HF Llama or Qwen3 modules, projections packed or dense, fp16
-    or bf16) decoding `sequences` sequences of up to `max_len` tokens at once.
+    """A causal LM (HF Llama, Mistral, Qwen2 or Qwen3 modules, projections packed
+    or dense, fp16 or bf16; others are refused) decoding `sequences` sequences of
+    up to `max_len` tokens at once.
 
     ``fp8_head``: the head's weights in e4m3 with a scale per 128 x 128 block
     (half of the dense head's bytes); False keeps the dense one.  Logits are
@@ -96,18 +111,23 @@ class PagedDecoder:
     def __init__(self, model, sequences: int, max_len: int, page_size: int = 64, n_pages: int | None = None,
                  fp8_head: bool = True) -> None:
         cfg = model.config
+        if cfg.model_type not in _FAMILIES:
+            raise ValueError(f"model_type {cfg.model_type!r}: PagedDecoder runs the layers of {', '.join(_FAMILIES)}")
         if cfg.hidden_act != "silu":
             raise ValueError(f"hidden_act {cfg.hidden_act!r}: PagedDecoder runs the gated MLP with silu")
         self.model, self.sequences = model, sequences
         body = model.model
         self.embed, self.layers, self.norm = body.embed_tokens, body.layers, body.norm
         attn = self.layers[0].self_attn
+        self.windows = _windows(cfg, self.layers)
         self.head_dim = getattr(cfg, "head_dim", None) or cfg.hidden_size // cfg.num_attention_heads
         self.heads, self.kv_heads = cfg.num_attention_heads, cfg.num_key_value_heads
         self.scale = getattr(attn, "scaling", self.head_dim ** -0.5)
         dev, dtype = self.embed.weight.device, self.embed.weight.dtype
         base, scaling, share = _rope(cfg)
-        self.table = rotary_table(max_len, int(self.head_dim * share), base, scaling, device=dev)
+        if share != 1:  # (these families turn whole heads, whatever it says)
+            raise ValueError(f"partial_rotary_factor {share}: the heads of {cfg.model_type} turn as a whole")
+        self.table = rotary_table(max_len, self.head_dim, base, scaling, device=dev)
         self.cache = PagedCache(len(self.layers), sequences, max_len, self.kv_heads, self.head_dim, page_size, n_pages,
                                 dtype, dev)
         self.head = quantize_fp8_weight(model.lm_head.weight) if fp8_head else None
@@ -137,8 +157,7 @@ class PagedDecoder:
                 q, k = self._norm(q, at.q_norm), self._norm(k, at.k_norm)
             kc, vc = self.cache.k[i], self.cache.v[i]
             q = rotary_append(q, k, v, self.table, positions, kc, vc, self.cache.block_table, sequences=sequences)
-            window = getattr(at, "sliding_window", None) or 0
-            o = paged_attention(q, kc, vc, block_table, lengths, scale=self.scale, window=window)
+            o = paged_attention(q, kc, vc, block_table, lengths, scale=self.scale, window=self.windows[i])
             x, h = self._norm(at.o_proj(o.view(rows, -1)), layer.post_attention_layernorm, h)
             gate, up = layer.mlp.gate_proj(x), layer.mlp.up_proj(x)
             x = layer.mlp.down_proj(F.silu(gate) * up)
