@@ -50,3 +50,47 @@ def test_a_rotary_share_that_the_family_ignores_is_refused():
     from turbopress_amd.paged_decode import PagedDecoder
     with pytest.raises(ValueError, match="partial_rotary_factor"):
         PagedDecoder(tiny_model("llama", partial_rotary_factor=0.5), 1, 64, fp8_head=False)
+
+
+@pytest.fixture
+def stubbed(monkeypatch):
+    """A decoder of three sequences whose layers and head are not run."""
+    from turbopress_amd.paged_decode import PagedDecoder
+    dec = PagedDecoder(tiny_model("llama"), 3, 32, page_size=8, fp8_head=False)
+    ran = []
+    monkeypatch.setattr(dec, "_rows", lambda tokens, *a: ran.append(len(tokens)) or (torch.zeros(len(tokens), 64),) * 2)
+    monkeypatch.setattr(dec, "_logits", lambda x, h: torch.zeros(len(x), 64))
+    dec.ran = ran
+    return dec
+
+
+def test_a_step_without_a_page_is_refused(stubbed):
+    """Before anything runs, and without moving the other sequences."""
+    dec = stubbed
+    dec.prefill(0, torch.arange(7))
+    dec.prefill(2, torch.arange(12))
+    dec.step(graph=False)  # tokens 7 and 12: in the prompts' pages
+    for graph in (False, True):
+        with pytest.raises(RuntimeError, match="token 8 of sequence 0"):
+            dec.step(graph=graph)
+    assert dec.ran == [7, 12, 3] and dec.positions.tolist() == [8, -1, 13] and dec.lengths.tolist() == [9, 0, 14]
+    dec.cache.reserve(0, 9)
+    dec.step(graph=False)
+    dec.stop(0)
+    for _ in range(2):
+        dec.step(graph=False)
+    with pytest.raises(RuntimeError, match="token 16 of sequence 2"):
+        dec.step(graph=False)
+    assert dec.positions.tolist() == [-1, -1, 16]
+
+
+def test_a_step_past_the_longest_length_is_refused(stubbed):
+    dec = stubbed
+    dec.prefill(1, torch.arange(31))
+    dec.step(graph=False)
+    with pytest.raises(RuntimeError, match="token 32 of sequence 1"):
+        dec.step(graph=False)
+    with pytest.raises(ValueError):
+        dec.cache.reserve(1, 33)
+    dec.stop(1)
+    dec.step(graph=False)

@@ -64,6 +64,10 @@ class PagedCache:
         held += new
         self.block_table[sequence, at:at + need] = torch.tensor(new, dtype=torch.int32).to(self.block_table.device)
 
+    def room(self, sequence: int) -> int:
+        """Tokens that the sequence's pages hold."""
+        return min(len(self._held[sequence]) * self.page_size, self.max_len)
+
     def release(self, sequence: int) -> None:
         """The sequence's pages are free again."""
         self._free += reversed(self._held[sequence])
@@ -136,6 +140,7 @@ class PagedDecoder:
         self.tokens = torch.zeros(sequences, dtype=torch.int64, device=dev)
         self.positions = torch.full((sequences,), -1, dtype=torch.int64, device=dev)
         self.lengths = torch.zeros(sequences, dtype=torch.int32, device=dev)
+        self._next = [-1] * sequences  # the positions, on the host
         self._graph = None
         self._graph_logits = None
 
@@ -193,11 +198,13 @@ class PagedDecoder:
         self.tokens[sequence] = logits[0].argmax()
         self.positions[sequence] = n
         self.lengths[sequence] = n + 1
+        self._next[sequence] = n
         return logits
 
     def stop(self, sequence: int) -> None:
         """End a sequence: its pages are free, its row of the step idles."""
         self.cache.release(sequence)
+        self._next[sequence] = -1
         self.positions[sequence] = -1
         self.lengths[sequence] = 0
 
@@ -212,12 +219,18 @@ class PagedDecoder:
         live = self.positions >= 0
         self.positions += live
         self.lengths += live.int()
+        self._next = [p + (p >= 0) for p in self._next]
 
     def step(self, graph: bool = True) -> Tensor:
         """One token of every live sequence: the logits [sequences, vocabulary]
         of ``tokens``, which become the greedy next ones.  Pages for the tokens
-        have to be reserved (``cache.reserve``).  graph: the step is captured
-        on first use and replayed (the logits are then a fixed buffer)."""
+        have to be reserved (``cache.reserve``); where one is not, nothing is
+        run and RuntimeError raised.  graph: the step is captured on first use
+        and replayed (the logits are then a fixed buffer)."""
+        for s, p in enumerate(self._next):
+            if p >= self.cache.room(s):  # (its key and value would be dropped, and attention miss them)
+                raise RuntimeError(f"no page for token {p} of sequence {s}: pages hold {self.cache.room(s)} tokens of it "
+                                   f"(cache.reserve), at most {self.cache.max_len}")
         if graph and self._graph is None:
             side = torch.cuda.Stream()
             side.wait_stream(torch.cuda.current_stream())
