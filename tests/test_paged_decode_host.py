@@ -94,3 +94,16 @@ def test_a_step_past_the_longest_length_is_refused(stubbed):
         dec.cache.reserve(1, 33)
     dec.stop(1)
     dec.step(graph=False)
+
+
+@pytest.mark.parametrize("sequence", [-1, 3])
+def test_sequences_that_do_not_exist_are_refused(stubbed, sequence):
+    """-1 too: its rows were the last sequence's on the host and no one's on the device."""
+    dec = stubbed
+    dec.prefill(2, torch.arange(4))
+    before = dec.cache.block_table.clone()
+    for call in (lambda: dec.prefill(sequence, torch.arange(3)), lambda: dec.stop(sequence),
+                 lambda: dec.cache.reserve(sequence, 9), lambda: dec.cache.release(sequence), lambda: dec.cache.room(sequence)):
+        with pytest.raises(IndexError, match="outside"):
+            call()
+    assert dec.ran == [4] and dec.positions.tolist() == [-1, -1, 4] and torch.equal(dec.cache.block_table, before)

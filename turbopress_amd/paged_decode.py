@@ -49,8 +49,13 @@ class PagedCache:
         self._free = list(range(n_pages - 1, -1, -1))
         self._held: list = [[] for _ in range(sequences)]
 
+    def _check(self, sequence: int) -> None:
+        if not 0 <= sequence < len(self._held):
+            raise IndexError(f"sequence {sequence} outside [0, {len(self._held)})")
+
     def reserve(self, sequence: int, length: int) -> None:
         """Pages for `length` tokens of a sequence, beside those it holds."""
+        self._check(sequence)
         if not 0 <= length <= self.max_len:
             raise ValueError(f"length {length} outside [0, {self.max_len}]")
         held = self._held[sequence]
@@ -66,10 +71,12 @@ class PagedCache:
 
     def room(self, sequence: int) -> int:
         """Tokens that the sequence's pages hold."""
+        self._check(sequence)
         return min(len(self._held[sequence]) * self.page_size, self.max_len)
 
     def release(self, sequence: int) -> None:
         """The sequence's pages are free again."""
+        self._check(sequence)
         self._free += reversed(self._held[sequence])
         self._held[sequence] = []
         self.block_table[sequence] = -1
