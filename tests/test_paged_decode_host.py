@@ -107,3 +107,14 @@ def test_sequences_that_do_not_exist_are_refused(stubbed, sequence):
         with pytest.raises(IndexError, match="outside"):
             call()
     assert dec.ran == [4] and dec.positions.tolist() == [-1, -1, 4] and torch.equal(dec.cache.block_table, before)
+
+
+def test_generate_fills_the_longest_length(stubbed, monkeypatch):
+    """A prompt and its new tokens but the last, which nothing reads, take max_len places."""
+    dec = stubbed
+    monkeypatch.setattr(torch.cuda, "synchronize", lambda: None)
+    tokens, _ = dec.generate([torch.arange(20), torch.arange(2)], 13, graph=False)
+    assert len(tokens) == 2 and all(len(t) == 13 for t in tokens)
+    assert dec.positions.tolist() == [32, 14, -1] and dec.cache.room(0) == 32 and dec.cache.room(1) == 16
+    with pytest.raises(ValueError):
+        dec.generate([torch.arange(20)], 14, graph=False)

@@ -265,7 +265,7 @@ class PagedDecoder:
             self.stop(s)
         for s, p in enumerate(prompts):
             self.prefill(s, p)
-            self.cache.reserve(s, int(p.shape[0]) + n_new)
+            self.cache.reserve(s, int(p.shape[0]) + n_new - 1)  # (the last new token is not read back)
         out = [self.tokens.clone()]
         start, timed = None, 0
         for i in range(1, n_new):
