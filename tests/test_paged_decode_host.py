@@ -118,3 +118,11 @@ def test_generate_fills_the_longest_length(stubbed, monkeypatch):
     assert dec.positions.tolist() == [32, 14, -1] and dec.cache.room(0) == 32 and dec.cache.room(1) == 16
     with pytest.raises(ValueError):
         dec.generate([torch.arange(20)], 14, graph=False)
+
+
+def test_the_head_is_the_models_own_unless_asked():
+    from turbopress_amd.paged_decode import PagedDecoder
+    model = tiny_model("llama")
+    assert PagedDecoder(model, 1, 32).head is None
+    codes, scales = PagedDecoder(model, 1, 32, fp8_head=True).head
+    assert codes.shape == (64, 64) and codes.dtype == torch.float8_e4m3fn and scales.shape == (1, 1)

@@ -6,7 +6,8 @@ everything but the projections to the HF decoder
 (``scripts/graph_decode_bench.py:39-118``).  ``PagedDecoder`` runs the layers of
 a packed Llama, Mistral, Qwen2 or Qwen3 causal LM itself: norm and residual, projections
 (``PackedTCQLinear``), norms of the heads, rotary positions and the cache's
-writes, attention over each sequence's pages, and the dense head in 8 bits.  Its
+writes, attention over each sequence's pages, and the head, in 8 bits on
+request.  Its
 decode step takes one token of every sequence, has no host synchronisation and
 is captured in one HIP graph; sequences have lengths of their own and hold
 pages only for what they have.
@@ -114,13 +115,14 @@ class PagedDecoder:
     or dense, fp16 or bf16; others are refused) decoding `sequences` sequences of
     up to `max_len` tokens at once.
 
-    ``fp8_head``: the head's weights in e4m3 with a scale per 128 x 128 block
-    (half of the dense head's bytes); False keeps the dense one.  Logits are
-    fp32 [rows, vocabulary] with it, the model's type without."""
+    ``fp8_head``: the head's weights in e4m3 with a scale per 128 x 128 block,
+    made of the dense ones here (half of their bytes, codes within 2^-4 of each);
+    without, the model's own.  Logits are fp32 [rows, vocabulary] with it, the
+    model's type without."""
 
     @torch.no_grad()
     def __init__(self, model, sequences: int, max_len: int, page_size: int = 64, n_pages: int | None = None,
-                 fp8_head: bool = True) -> None:
+                 fp8_head: bool = False) -> None:
         cfg = model.config
         if cfg.model_type not in _FAMILIES:
             raise ValueError(f"model_type {cfg.model_type!r}: PagedDecoder runs the layers of {', '.join(_FAMILIES)}")
@@ -302,7 +304,9 @@ def main(argv=None) -> int:
     ap.add_argument("--prompt-len", type=int, default=40, help="of the longest; the others are shorter")
     ap.add_argument("--new-tokens", type=int, default=64)
     ap.add_argument("--page-size", type=int, default=64)
-    ap.add_argument("--dense-head", action="store_true", help="keep the head's dense weights")
+    head = ap.add_mutually_exclusive_group()
+    head.add_argument("--fp8-head", action="store_true", help="the head's weights in 8 bits")
+    head.add_argument("--dense-head", action="store_true", help="the head's dense weights (the default)")
     args = ap.parse_args(argv)
 
     def progress(msg: str) -> None:
@@ -320,12 +324,12 @@ def main(argv=None) -> int:
     prompts = [torch.randint(0, model.config.vocab_size, (max(1, args.prompt_len - 7 * s),), generator=gen).cuda()
                for s in range(args.sequences)]
     decoder = PagedDecoder(model, args.sequences, args.prompt_len + args.new_tokens, args.page_size,
-                           fp8_head=not args.dense_head)
+                           fp8_head=args.fp8_head)
     eager, eager_rate = decoder.generate(prompts, args.new_tokens, graph=False)
     graph, graph_rate = decoder.generate(prompts, args.new_tokens, graph=True)
     print(json.dumps({"model": args.synthetic or str(args.artifact), "sequences": args.sequences,
                       "prompt_lens": [int(p.shape[0]) for p in prompts], "new_tokens": args.new_tokens,
-                      "head": "dense" if args.dense_head else "fp8", "eager_tok_s": round(eager_rate, 1),
+                      "head": "fp8" if args.fp8_head else "dense", "eager_tok_s": round(eager_rate, 1),
                       "graph_tok_s": round(graph_rate, 1), "greedy_tokens_match": eager == graph}), flush=True)
     return 0
 
