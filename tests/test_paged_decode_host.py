@@ -126,3 +126,20 @@ def test_the_head_is_the_models_own_unless_asked():
     assert PagedDecoder(model, 1, 32).head is None
     codes, scales = PagedDecoder(model, 1, 32, fp8_head=True).head
     assert codes.shape == (64, 64) and codes.dtype == torch.float8_e4m3fn and scales.shape == (1, 1)
+
+
+def test_runs_from_one_beginning(stubbed, monkeypatch):
+    """Both runs of the command decode from the same prefill: the second one
+    finds the first one's beginning, whatever its prefill would have been."""
+    dec = stubbed
+    monkeypatch.setattr(torch.cuda, "synchronize", lambda: None)
+    tokens = iter(range(1000))
+    monkeypatch.setattr(dec, "_logits", lambda x, h: torch.nn.functional.one_hot(
+        torch.tensor([next(tokens) % 64] * len(x)), 64).float())
+    begin = dec._begin([torch.arange(20), torch.arange(2)], 5)
+    assert dec.ran == [20, 2]
+    first = dec._decode(begin, 5, graph=False)[0]
+    assert dec.positions.tolist() == [24, 6, -1] and dec._next == [24, 6, -1]
+    second = dec._decode(begin, 5, graph=False)[0]
+    assert [t[0] for t in first] == [t[0] for t in second] == [0, 1]
+    assert dec.positions.tolist() == [24, 6, -1] and dec.lengths.tolist() == [25, 7, 0] and dec.ran == [20, 2] + [3] * 8

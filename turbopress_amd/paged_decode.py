@@ -258,9 +258,9 @@ class PagedDecoder:
         return logits
 
     @torch.inference_mode()
-    def generate(self, prompts, n_new: int, graph: bool = True) -> tuple:
-        """Greedy tokens (n_new per prompt) of up to `sequences` prompts, and the
-        decode steps' tokens/s over all of them."""
+    def _begin(self, prompts, n_new: int) -> tuple:
+        """Prefill up to `sequences` prompts, with pages for n_new tokens of each:
+        the state from which their decoding begins."""
         if len(prompts) > self.sequences:
             raise ValueError(f"{len(prompts)} prompts for {self.sequences} sequences")
         for s in range(self.sequences):
@@ -268,6 +268,18 @@ class PagedDecoder:
         for s, p in enumerate(prompts):
             self.prefill(s, p)
             self.cache.reserve(s, int(p.shape[0]) + n_new - 1)  # (the last new token is not read back)
+        return len(prompts), self.tokens.clone(), self.positions.clone(), self.lengths.clone(), list(self._next)
+
+    @torch.inference_mode()
+    def _decode(self, begin: tuple, n_new: int, graph: bool) -> tuple:
+        """Greedy tokens from a state of ``_begin``, as often as wanted (what a
+        run leaves in the cache the next one writes again before it reads it),
+        and tokens/s."""
+        count, tokens, positions, lengths, following = begin
+        self.tokens.copy_(tokens)
+        self.positions.copy_(positions)
+        self.lengths.copy_(lengths)
+        self._next = list(following)
         out = [self.tokens.clone()]
         start, timed = None, 0
         for i in range(1, n_new):
@@ -278,8 +290,13 @@ class PagedDecoder:
             timed += i >= 2
             out.append(self.tokens.clone())
         torch.cuda.synchronize()
-        rate = timed * len(prompts) / (time.perf_counter() - start) if timed else float("inf")
-        return torch.stack(out, 1)[:len(prompts)].tolist(), rate
+        rate = timed * count / (time.perf_counter() - start) if timed else float("inf")
+        return torch.stack(out, 1)[:count].tolist(), rate
+
+    def generate(self, prompts, n_new: int, graph: bool = True) -> tuple:
+        """Greedy tokens (n_new per prompt) of up to `sequences` prompts, and the
+        decode steps' tokens/s over all of them."""
+        return self._decode(self._begin(prompts, n_new), n_new, graph)
 
 
 def main(argv=None) -> int:
@@ -325,8 +342,11 @@ def main(argv=None) -> int:
                for s in range(args.sequences)]
     decoder = PagedDecoder(model, args.sequences, args.prompt_len + args.new_tokens, args.page_size,
                            fp8_head=args.fp8_head)
-    eager, eager_rate = decoder.generate(prompts, args.new_tokens, graph=False)
-    graph, graph_rate = decoder.generate(prompts, args.new_tokens, graph=True)
+    # (one prefill for both: the sums of a prompt of 17..32 tokens are not always
+    # added in one order, and a near tie may fall either way)
+    begin = decoder._begin(prompts, args.new_tokens)
+    eager, eager_rate = decoder._decode(begin, args.new_tokens, graph=False)
+    graph, graph_rate = decoder._decode(begin, args.new_tokens, graph=True)
     print(json.dumps({"model": args.synthetic or str(args.artifact), "sequences": args.sequences,
                       "prompt_lens": [int(p.shape[0]) for p in prompts], "new_tokens": args.new_tokens,
                       "head": "fp8" if args.fp8_head else "dense", "eager_tok_s": round(eager_rate, 1),
