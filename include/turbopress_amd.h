@@ -430,6 +430,13 @@ int tp_fp8_linear(int dtype, int64_t m, int64_t n, int64_t k, const uint8_t* a, 
 int64_t tp_fp8_workspace_bytes(int64_t m, int64_t n, int64_t k, const uint8_t* a, int64_t lda, const uint8_t* w,
                                int64_t ldw);
 
+/* Host only: how tp_fp8_linear cuts a call on a device of `cus` compute units
+ * (tiled: both operands need no copy): out[0] = 1 where every weight is read once
+ * into operand registers, 0 where tiles are staged, out[1] and out[2] = weight
+ * and activation rows of a workgroup's tile, out[3] = waves, or teams of waves,
+ * that share its columns, out[4] = workgroups (tests and tuning). */
+int tp_fp8_plan(int dtype, int64_t m, int64_t n, int64_t k, int tiled, int cus, int64_t* out);
+
 /* Rotary positions: for each token t and head, with c, s the two halves of
  * row positions[t] of `table` (fp32 [n_positions, rotary_dim]: cosines, then
  * sines, of the position's rotary_dim / 2 angles), the pair (a, b) of index i

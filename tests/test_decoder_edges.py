@@ -199,3 +199,83 @@ def test_rotary_refuses_tokens_of_more_than_31_bits_of_pairs(built_lib):
     st = built_lib.tp_rotary(0, 1, 65536, 40, d, 2, 0, p, 65536 * d, d, p, 40 * d, d, p, 8, p, p, p, None, 0, 0, None, None,
                              None, None, 0, 1, None, 0, 0, None, None)
     assert st == L.TP_ERR_BAD_DIMS
+
+
+# (weight rows, activation rows, teams) of a tile -> a call that takes it, of several
+# tiles either way and ragged ends, and a K past three of its groups of staged scales
+# (8 blocks of 128 columns each, 4 of the largest tile's, per team)
+TILES = {(320, 256, 1): (1537, 10000, 1801), (256, 256, 1): (2045, 6000, 3301), (256, 192, 1): (1537, 5000, 3301),
+         (128, 128, 1): (400, 10000, 3301), (128, 64, 1): (200, 4100, 3301), (64, 64, 1): (1277, 1597, 3301),
+         (64, 64, 2): (70, 150, 6401)}
+CODE = {F16: 0, BF16: 1, F32: 2}
+
+
+def _fp8_plan(dtype, m, n, k, cus):
+    from turbopress_amd import _lib
+    out = (ctypes.c_int64 * 5)()
+    _lib.check(_lib.lib().tp_fp8_plan(CODE[dtype], m, n, k, 1, cus, out), "fp8_plan")
+    return tuple(out)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tile", TILES)
+@pytest.mark.parametrize("tail", [True, False])
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+def test_fp8_linear_every_tile(cuda, tile, tail, dtype):
+    """Each tile by the plan's word, at K of no multiple of 16 (NaN behind it) and
+    of 16, over all of its rings of stages and scales; scales differ from block to
+    block by up to 2^12."""
+    from turbopress_amd import fp8_linear
+    m, n, k = TILES[tile]
+    if not tail:
+        k += -k % 16
+    cus = torch.cuda.get_device_properties(0).multi_processor_count
+    plan = _fp8_plan(dtype, m, n, k, cus)
+    if dtype == F32 and tile[0] > 128:
+        assert plan[0] == 0 and plan[1] <= 128
+        pytest.skip("fp32 outputs do not take the largest tiles")
+    assert plan[:4] == (0, *tile)
+    g = _gen(m + n + k)
+    a, sa, w, sw = _fp8_case(g, m, n, k, -k % 16, -k % 16)
+    sa, sw = (s * torch.exp2(torch.randint(-6, 7, s.shape, generator=g, device="cuda").float()) for s in (sa, sw))
+    bias = _randn(g, n, dtype=dtype)
+    if dtype == F16:  # (inside its range)
+        top = O.fp8_linear(a, sa, w, sw)[0].abs().max()
+        sa = sa * torch.exp2(-torch.ceil(torch.log2(top / 30000))).float()
+    want, size = O.fp8_linear(a, sa, w, sw, bias)
+    got = fp8_linear(a, sa, w, sw, bias=bias, out_dtype=dtype)
+    _within(got, want, _fp8_tol(want, size, k, dtype))
+    assert torch.equal(got, fp8_linear(a, sa, w, sw, bias=bias, out_dtype=dtype))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m", [3, 20])
+@pytest.mark.parametrize("n", [150, 17000])
+def test_fp8_linear_few_rows_of_long_columns(cuda, m, n):
+    """The rows kernel past several rounds of its waves over the columns."""
+    from turbopress_amd import fp8_linear
+    k = 8165 if n == 150 else 1701
+    plan = _fp8_plan(F32, m, n, k, torch.cuda.get_device_properties(0).multi_processor_count)
+    g = _gen(m + n)
+    a, sa, w, sw = _fp8_case(g, m, n, k, -k % 16, -k % 16)
+    sa, sw = (s * torch.exp2(torch.randint(-6, 7, s.shape, generator=g, device="cuda").float()) for s in (sa, sw))
+    want, size = O.fp8_linear(a, sa, w, sw)
+    _within(fp8_linear(a, sa, w, sw, out_dtype=F32), want, _fp8_tol(want, size, k, F32))
+    assert plan[0] == (m <= 16 or n <= 6144) and (not plan[0] or plan[3] == 8)
+
+
+def test_fp8_plan(built_lib):
+    """The plan on 256 compute units, and its refusals."""
+    from turbopress_amd import _lib as L
+    assert _fp8_plan(F32, 1, 151936, 2560, 256) == (1, 32, 16, 8, 4748)
+    assert _fp8_plan(F16, 20, 4096, 300, 256) == (1, 16, 32, 2, 256)
+    assert _fp8_plan(F16, 199, 4096, 2560, 256) == (0, 64, 64, 2, 256)
+    assert _fp8_plan(BF16, 2048, 9728, 2560, 256) == (0, 320, 256, 1, 248)
+    assert _fp8_plan(F32, 2048, 9728, 2560, 256)[1] <= 128
+    for tile, (m, n, k) in TILES.items():
+        assert _fp8_plan(BF16, m, n, k, 256)[:4] == _fp8_plan(F16, m, n, k + -k % 16, 256)[:4] == (0, *tile)
+    out = (ctypes.c_int64 * 5)(7, 7, 7, 7, 7)
+    assert built_lib.tp_fp8_plan(3, 1, 1, 1, 1, 256, out) == L.TP_ERR_BAD_TYPE and list(out) == [0] * 5
+    assert built_lib.tp_fp8_plan(0, 0, 1, 1, 1, 256, out) == built_lib.tp_fp8_plan(0, 1, 1, 1, 1, 0, out) == L.TP_ERR_BAD_DIMS
+    assert built_lib.tp_fp8_plan(0, 1, 1, 0, 1, 256, out) == L.TP_ERR_BAD_DIMS
+    assert built_lib.tp_fp8_plan(0, 1, 1, 1, 1, 256, None) == L.TP_ERR_NULL_POINTER

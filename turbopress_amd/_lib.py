@@ -94,6 +94,7 @@ SIGNATURES.update({
                                 _P, _I64, _P, _P, _P]),
     "tp_fp8_linear": (c_int, [c_int, _I64, _I64, _I64, _P, _I64, _P, _P, _I64, _P, _P, _P, _I64, _P, _I64, _P]),
     "tp_fp8_workspace_bytes": (_I64, [_I64, _I64, _I64, _P, _I64, _P, _I64]),
+    "tp_fp8_plan": (c_int, [c_int, _I64, _I64, _I64, c_int, c_int, POINTER(c_int64)]),
     "tp_rotary": (c_int, [c_int, _I64, _I64, _I64, _I64, _I64, c_int, _P, _I64, _I64, _P, _I64, _I64,
                           _P, _I64, _P, _P, _P, _P, _I64, _I64, _P, POINTER(c_int64), _P, POINTER(c_int64),
                           _I64, _I64, _P, _I64, _I64, _P, _P]),

@@ -593,15 +593,26 @@ bool fp8_takes_rows(int64_t m, int64_t n, int64_t k, bool tiled) {
   return m <= 16 || (m <= 32 && (n <= 6144 || (!tiled && n * k <= (32 << 20))));
 }
 
+// How the rows kernel cuts a call.
+struct RowsPlan {
+  int waves, tiles;  // that share a tile's columns; tiles of a workgroup
+};
+
+// 8 waves share a tile's columns (4 / 8 / 16 waves, 1 row: 4096 x 2560 5.5 / 4.6 /
+// 4.9 us, 2560 x 9728 12.6 / 8.4 / 8.3); two tiles per workgroup where that leaves
+// two workgroups per CU (1 / 2 tiles, 1 row: 151936 x 2560 76.9 / 66.8 us, 16384 x
+// 1000 8.5 / 7.4, 9728 x 2560 7.8 / 8.5)
+inline RowsPlan rows_plan(int64_t m, int64_t n, int64_t kb, int64_t cus) {
+  RowsPlan p{8, m <= 16 && (n + 15) / 16 >= 4 * cus ? 2 : 1};
+  while (p.waves > 1 && p.waves > kb) p.waves /= 2;
+  return p;
+}
+
 template <typename T>
 int launch_rows_for(const Fp8Args& g, hipStream_t s) {
-  // 8 waves share a tile's columns (4 / 8 / 16 waves, 1 row: 4096 x 2560 5.5 /
-  // 4.6 / 4.9 us, 2560 x 9728 12.6 / 8.4 / 8.3); two tiles per workgroup where
-  // that leaves two workgroups per CU (1 / 2 tiles, 1 row: 151936 x 2560 76.9 /
-  // 66.8 us, 16384 x 1000 8.5 / 7.4, 9728 x 2560 7.8 / 8.5)
-  int waves = 8;
-  while (waves > 1 && waves > g.kb) waves /= 2;
-  const bool two = (g.n + 15) / 16 >= 4 * (int64_t)device_cu_count();
+  const RowsPlan p = rows_plan(g.m, g.n, g.kb, device_cu_count());
+  const int waves = p.waves;
+  const bool two = p.tiles == 2;
   const bool odd = (((uintptr_t)g.a | (uintptr_t)g.w | g.lda | g.ldw) & 3) != 0;
   if (g.m <= 16) {
     if (two && odd) launch_rows<T, 1, 2, true>(g, waves, s);
@@ -636,24 +647,30 @@ int launch_tiles(Fp8Args g, hipStream_t s) {
 //   512 x 4096 x 2560   50 39 33 21 14.8 [14.3] 18.5
 //   256 x 2560 x 9728   146 122 100 61 40 29 [24.0]
 //   199 x 4096 x 2560   49 39 33 20 14.3 10.8 [10.3]
-template <typename T>
-int launch_tiles_for(const Fp8Args& g, hipStream_t s) {
-  struct Shape {
-    int n, m, per_cu;
-    double one, full;
-  };
-  static const Shape shapes[] = {{320, 256, 1, 2.4, 2.4}, {256, 256, 1, 1.9, 1.9}, {256, 192, 1, 1.6, 1.6}, {128, 128, 2, 0.78, 1.15},
-                                 {128, 64, 2, 0.5, 0.77}, {64, 64, 2, 0.35, 0.5},  {64, 64, 1, 0.28, 0.28}};
-  const int64_t cus = device_cu_count();
+struct Fp8Shape {
+  int n, m, teams, per_cu;
+  double one, full;
+};
+constexpr Fp8Shape kFp8Shapes[] = {{320, 256, 1, 1, 2.4, 2.4}, {256, 256, 1, 1, 1.9, 1.9},   {256, 192, 1, 1, 1.6, 1.6},
+                                   {128, 128, 1, 2, 0.78, 1.15}, {128, 64, 1, 2, 0.5, 0.77}, {64, 64, 1, 2, 0.35, 0.5},
+                                   {64, 64, 2, 1, 0.28, 0.28}};
+
+inline int pick_tiles(bool f32, int64_t m, int64_t n, int64_t kb, int64_t cus) {
   // (fp32 outputs: the operands of the largest, converted, do not fit the registers)
-  int best = sizeof(T) == 4 ? 3 : 0;
+  int best = f32 ? 3 : 0;
   double least = 0;
   for (int x = best, first = best; x < 7; ++x) {
-    const Shape& p = shapes[x];
-    const int64_t t = ((g.m + p.m - 1) / p.m) * ((g.n + p.n - 1) / p.n);
-    const double c = t <= cus ? g.kb * p.one + 4 : (double)((t + cus * p.per_cu - 1) / (cus * p.per_cu)) * (g.kb * p.full + 4);
+    const Fp8Shape& p = kFp8Shapes[x];
+    const int64_t t = ((m + p.m - 1) / p.m) * ((n + p.n - 1) / p.n);
+    const double c = t <= cus ? kb * p.one + 4 : (double)((t + cus * p.per_cu - 1) / (cus * p.per_cu)) * (kb * p.full + 4);
     if (x == first || c < least) best = x, least = c;
   }
+  return best;
+}
+
+template <typename T>
+int launch_tiles_for(const Fp8Args& g, hipStream_t s) {
+  const int best = pick_tiles(sizeof(T) == 4, g.m, g.n, g.kb, device_cu_count());
   if constexpr (sizeof(T) != 4) {
     if (best == 0) return launch_tiles<T, 2, 4, 10, 4>(g, s);
     if (best == 1) return launch_tiles<T, 2, 4, 8, 4>(g, s);
@@ -682,6 +699,23 @@ extern "C" int64_t tp_fp8_workspace_bytes(int64_t m, int64_t n, int64_t k, const
   const bool tiled = fp8_rows_tiled(a, lda) && fp8_rows_tiled(w, ldw);
   if (m == 0 || n == 0 || fp8_takes_rows(m, n, k, tiled)) return 0;
   return (fp8_rows_tiled(a, lda) ? 0 : align_bytes(m, k)) + (fp8_rows_tiled(w, ldw) ? 0 : align_bytes(n, k));
+}
+
+extern "C" int tp_fp8_plan(int dtype, int64_t m, int64_t n, int64_t k, int tiled, int cus, int64_t* out) {
+  if (!out) return TP_ERR_NULL_POINTER;
+  for (int i = 0; i < 5; ++i) out[i] = 0;
+  if (!dtype_ok(dtype)) return TP_ERR_BAD_TYPE;
+  if (!fp8_sizes_ok(m, n, k) || m == 0 || n == 0 || cus < 1) return TP_ERR_BAD_DIMS;
+  const int64_t kb = (k + 127) / 128;
+  if (fp8_takes_rows(m, n, k, tiled != 0)) {
+    const RowsPlan p = rows_plan(m, n, kb, cus);
+    out[0] = 1, out[1] = 16 * p.tiles, out[2] = m <= 16 ? 16 : 32, out[3] = p.waves;
+  } else {
+    const Fp8Shape& p = kFp8Shapes[pick_tiles(dtype == TP_F32, m, n, kb, cus)];
+    out[1] = p.n, out[2] = p.m, out[3] = p.teams;
+  }
+  out[4] = ((n + out[1] - 1) / out[1]) * ((m + out[2] - 1) / out[2]);
+  return TP_OK;
 }
 
 extern "C" int tp_fp8_linear(int dtype, int64_t m, int64_t n, int64_t k, const uint8_t* a, int64_t lda,
