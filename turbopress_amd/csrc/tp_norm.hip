@@ -351,19 +351,28 @@ constexpr int kNormMaxVpt = 6;
 // Lanes and vectors per lane of a row.  Few rows: as many lanes as the row
 // feeds (a chain of latencies).  Many: the split with the fewest idle slots,
 // and among those the fewest waves, for a row inside one wave needs no LDS.
-// fp16 with a residual, us, the split of many rows / of few:
-//   d       1 row      512 rows   1024       2048
-//   1024    3.6 / 3.0  4.0 / 3.6  4.3 / 3.9  5.4 / 5.1
-//   2560    5.3 / 3.4  6.5 / 4.6  8.2 / 6.3  9.0 / 9.7
-//   4096    4.8 / 3.5  7.1 / 5.1  7.8 / 7.5  11.7 / 12.6
+// Few are up to 4 per CU, 2 with a scale per row (whose maximum is a second chain
+// through LDS), 8 of fp32 in and out.  With a residual, us, the split of many rows
+// / of few:
+//           fp16                            bf16 -> e4m3 per 128
+//   d       1 row    512      1024     2048      512      1024     2048
+//   1024    3.1/2.7  3.6/3.2  3.9/3.6  4.5/4.5   4.1/3.5  4.2/3.8  4.9/4.9
+//   2560    4.6/3.0  5.5/4.4  6.2/6.0  8.4/9.3   6.5/4.8  7.2/6.7  9.8/10.8
+//   4096    4.3/3.2  5.3/4.6  7.4/7.2  12/12.2   6.3/5.0  8.7/8.2  13.2/13.5
+//   9728    5.2/4.2  8.5/7.8  14/13.4  27/25.3   9.9/9.4  16/16.3  27.7/27.8
+//           bf16 -> e4m3 per row            fp32
+//   1024    3.4/3.2  4.0/3.7  4.2/4.1  4.9/5.1   3.6/3.4  4.3/4.2  7.6/7.6
+//   2560    5.0/3.8  6.0/5.4  6.8/7.6  9.0/12.1  6.3/5.1  8.6/8.5  19/16.0
+//   4096    4.9/3.8  6.0/5.5  8.2/8.8  13/14.3   7.5/7.3  15/13.2  25.7/25.2
+//   9728    5.8/5.0  9.5/9.3  14.6/16  27/27.2   17/15.6  31/28.9  65/66.7
 struct NormPlan {
   int sub, waves, vpt;  // vpt 0: the long kernel
 };
 
-inline NormPlan norm_plan(int64_t rows, int nvec, int cus) {
+inline NormPlan norm_plan(int64_t rows, int nvec, int64_t few_rows) {
   if (nvec <= 16) return {16, 1, 1};
   if (nvec <= 32) return {32, 1, 1};
-  const bool few = rows <= 4 * (int64_t)cus;
+  const bool few = rows <= few_rows;
   NormPlan best{64, 8, 0};
   int64_t best_cost = -1;
   for (int w = 1; w <= 8; w *= 2) {
@@ -387,7 +396,8 @@ int launch_norm(const NormArgs& a0, hipStream_t s) {
   const int64_t at = (int64_t)(uintptr_t)a.x | (int64_t)(uintptr_t)a.residual |
                      ((a.x_outer | a.x_inner | a.r_outer | a.r_inner) * (int64_t)sizeof(T));
   a.odd = (at & 3) != 0;
-  const NormPlan p = norm_plan(a.rows, a.nvec, device_cu_count());
+  constexpr int64_t kFewPerCu = OUT == kFp8Row ? 2 : OUT == kSame && sizeof(T) == 4 ? 8 : 4;
+  const NormPlan p = norm_plan(a.rows, a.nvec, kFewPerCu * device_cu_count());
   if (p.vpt == 0) {
     if (!grid_fits(a.rows, 1024)) return TP_ERR_BAD_DIMS;
     hipLaunchKernelGGL((rms_norm_long_kernel<T, OUT>), dim3((uint32_t)a.rows), dim3(1024), 0, s, a);
