@@ -417,7 +417,9 @@ int tp_rms_norm_fp8(int dtype, int64_t rows, int64_t inner, int64_t d, const voi
  * activation rows an operand that is not 16-byte aligned (pointer, lda or ldw),
  * or whose rows are more than 2^22 apart, is copied into the workspace first.
  * Columns [k, ld) are not used, whatever
- * they hold.  Sums are fp32, added in a fixed order; y rounds once.
+ * they hold.  Scaled sums of blocks are added in fp32 in a fixed order; y rounds
+ * once.  A block's own sum is in fp32 for TP_F32, for the other types the 8-bit
+ * matrix instructions' (good to about 2^-16 of the result).
  * The workspace (tp_fp8_workspace_bytes, 16-byte aligned; NULL when that is 0)
  * may hold anything.  m = 0 or n = 0 does nothing. */
 int tp_fp8_linear(int dtype, int64_t m, int64_t n, int64_t k, const uint8_t* a, int64_t lda, const float* a_scales,

@@ -6,11 +6,13 @@
 //
 // One pass: a row's x and residual stay in registers between its sum of squares
 // and its output, so they are read once and h, y (or codes) written once; the
-// weight comes from L2.  Nothing is computed to speak of (4 flops per
-// element): many rows are bound by HBM, a few by the latency of load, reduction
+// weight comes from L2.  4 flops per element (a wave's vector instructions for 64
+// of them: 16 of fp16 rows off their words, 29 with a residual and e4m3 output, for
+// conversions, maxima and quotients): many rows are bound by HBM, a few by the latency of load, reduction
 // and store.  8192 x 9728 fp16 60 us = 5.3 TB/s (a copy reaches 5.2); 8191 x 9727
-// 72, half of its rows off their words; 2048 x 2560 with a residual and e4m3
-// output 10; 1 x 2560 3.
+// 70, half of its rows off their words; 2048 x 2560 with a residual and e4m3
+// output 10.2 (scales per row 10.0), of which the instructions' issue alone is 3.9;
+// 1 x 2560 3.0.
 #include "tp_ops_common.h"
 
 #include <algorithm>

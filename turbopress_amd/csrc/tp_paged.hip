@@ -7,10 +7,12 @@
 // and two states join in the same way, so a sequence may be cut anywhere.
 // Keys and values are read once, 4 * (query heads per cache head) flops for
 // each of their elements: bound by HBM (8 heads of 128: 64 sequences x 8192
-// tokens 351 us = 6.1 TB/s, 1 x 131072 102 us = 5.2 with its start and join; 1 x
-// 577 9 us, the chain of lengths, pages, keys and join).
+// tokens 352 us = 6.1 TB/s, 1 x 131072 99 us = 5.4 with its start and join; 1 x
+// 577 9.2 us, the chain of lengths, pages, keys and join).
 //
-// Work: 128 tokens of one (sequence, cache head) are a unit.  A grid of as many
+// Work: 128 tokens (256 of up to 64 columns) of one (sequence, cache head) are a
+// unit, for up to 16 query heads: more of them read keys and values again (16 x
+// 8192 tokens of one cache head of 128: 16 query heads 25 us, 32 32, 48 47).  A grid of as many
 // workgroups as the GPU holds takes equal runs of the list of all units, so
 // uneven sequences, one long one and many short ones all fill it; the lengths
 // are only known on the device, and every workgroup finds its run by a scan of

@@ -51,8 +51,12 @@ def fp8_linear(a: Tensor, a_scales: Tensor, w: Tensor, w_scales: Tensor, bias: T
                out_dtype: torch.dtype = torch.float16) -> Tensor:
     """``(a * a_scales) @ (w * w_scales)^T + bias``: a float8_e4m3fn [..., k] with
     scales fp32 [..., ceil(k / 128)], w float8_e4m3fn [n, k] with scales fp32
-    [ceil(n / 128), ceil(k / 128)], bias of out_dtype.  fp32 sums in a fixed
-    order, rounded once to out_dtype (fp16, bf16 or fp32): [..., n]."""
+    [ceil(n / 128), ceil(k / 128)], bias of out_dtype: [..., n] of out_dtype
+    (fp16, bf16 or fp32).  The scaled sums of blocks of 128 columns are added in
+    fp32 in a fixed order and rounded once.  A block's own sum is in fp32 for fp32
+    outputs; for the others it is the 8-bit matrix instructions', good to about
+    2^-16 of the result (1.3e-5 rms), well below their rounding.  Rows may lie
+    anywhere (any alignment, any distance)."""
     code, index, shape = DTYPE_CODES.get(out_dtype), a.get_device(), a.shape
     n, k = w.shape if w.dim() == 2 else (0, 0)
     kb = -(-k // FP8_BLOCK)
