@@ -218,9 +218,8 @@ def _fp8_plan(dtype, m, n, k, cus):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("tile", TILES)
+@pytest.mark.parametrize("tile,dtype", [(t, dt) for t in TILES for dt in (F16, BF16, F32) if dt != F32 or t[0] <= 128])
 @pytest.mark.parametrize("tail", [True, False])
-@pytest.mark.parametrize("dtype", [F16, BF16, F32])
 def test_fp8_linear_every_tile(cuda, tile, tail, dtype):
     """Each tile by the plan's word, at K of no multiple of 16 (NaN behind it) and
     of 16, over all of its rings of stages and scales; scales differ from block to
@@ -230,11 +229,7 @@ def test_fp8_linear_every_tile(cuda, tile, tail, dtype):
     if not tail:
         k += -k % 16
     cus = torch.cuda.get_device_properties(0).multi_processor_count
-    plan = _fp8_plan(dtype, m, n, k, cus)
-    if dtype == F32 and tile[0] > 128:
-        assert plan[0] == 0 and plan[1] <= 128
-        pytest.skip("fp32 outputs do not take the largest tiles")
-    assert plan[:4] == (0, *tile)
+    assert _fp8_plan(dtype, m, n, k, cus)[:4] == (0, *tile)
     g = _gen(m + n + k)
     a, sa, w, sw = _fp8_case(g, m, n, k, -k % 16, -k % 16)
     sa, sw = (s * torch.exp2(torch.randint(-6, 7, s.shape, generator=g, device="cuda").float()) for s in (sa, sw))
@@ -273,6 +268,7 @@ def test_fp8_plan(built_lib):
     assert _fp8_plan(BF16, 2048, 9728, 2560, 256) == (0, 320, 256, 1, 248)
     assert _fp8_plan(F32, 2048, 9728, 2560, 256)[1] <= 128
     for tile, (m, n, k) in TILES.items():
+        assert _fp8_plan(F32, m, n, k, 256)[1] <= 128  # (fp32 outputs do not take the largest)
         assert _fp8_plan(BF16, m, n, k, 256)[:4] == _fp8_plan(F16, m, n, k + -k % 16, 256)[:4] == (0, *tile)
     out = (ctypes.c_int64 * 5)(7, 7, 7, 7, 7)
     assert built_lib.tp_fp8_plan(3, 1, 1, 1, 1, 256, out) == L.TP_ERR_BAD_TYPE and list(out) == [0] * 5
