@@ -498,6 +498,80 @@ int tp_paged_attention(int dtype, int64_t batch, int64_t hq, int64_t hkv, int64_
 int64_t tp_paged_attention_workspace_bytes(int64_t batch, int64_t hq, int64_t hkv, int64_t d);
 int64_t tp_paged_attention_counter_bytes(int64_t batch, int64_t hq, int64_t hkv, int64_t d);
 
+/* tp_rotary into the paged caches with the place of each token's key and value
+ * apart from its position: they go to token slots[t] of the sequence
+ * (slot slots[t] % page_size of its page slots[t] / page_size), for tokens that
+ * share a position (a tree of drafted ones).  A negative slot writes nothing;
+ * two tokens of one slot of one sequence in a call race. */
+int tp_rotary_slots(int dtype, int64_t tokens, int64_t hq, int64_t hk, int64_t d, int64_t rotary_dim, int interleaved,
+                    const void* q, int64_t q_token, int64_t q_head, const void* k, int64_t k_token, int64_t k_head,
+                    const float* table, int64_t n_positions, const int64_t* positions, void* q_out, const void* v,
+                    int64_t v_token, int64_t v_head, void* k_cache, const int64_t* kc, void* v_cache,
+                    const int64_t* vc, int64_t n_pages, int64_t page_size, const int32_t* block_table,
+                    int64_t table_width, int64_t n_sequences, const int32_t* sequences, const int64_t* slots,
+                    void* stream);
+
+/* tp_paged_attention over the last `window` tokens and the first `sinks`: t in
+ * [max(0, lengths[b] - window), lengths[b]) or [0, min(sinks, lengths[b])).
+ * Without a window sinks have no effect. */
+int tp_paged_attention_sinks(int dtype, int64_t batch, int64_t hq, int64_t hkv, int64_t d, const void* q,
+                             int64_t q_batch, int64_t q_head, const void* k_cache, const int64_t* kc,
+                             const void* v_cache, const int64_t* vc, int64_t n_pages, int64_t page_size,
+                             const int32_t* block_table, int64_t table_width, const int32_t* lengths, float scale,
+                             int64_t window, int64_t sinks, void* out, void* workspace, int64_t workspace_bytes,
+                             void* counters, int64_t counter_bytes, void* stream);
+
+/* Attention of `tokens` (1..64) new tokens of each sequence over a paged cache:
+ * q [batch, tokens, hq, d] (strides in elements), out contiguous.  lengths[b]
+ * tokens (0 for less) are in the cache before the new ones, new token i is token
+ * lengths[b] + i of the cache.  Token i sees the cached tokens t < lengths[b] and
+ * the new tokens j whose bit of ancestors[b * tokens + i] is set (bits from
+ * `tokens` on are not looked at; NULL: j <= i).  With a window > 0, only those
+ * whose position is above its own less the window, or below sinks: token t <
+ * lengths[b] has position t, new token i lengths[b] - 1 + the number of bits of
+ * its ancestors.  What a token does not see does not matter to it (NaN and
+ * infinity included); one that sees nothing gives zeros.  Otherwise as
+ * tp_paged_attention; workspace and counters likewise, of their own sizes. */
+int tp_paged_tree_attention(int dtype, int64_t batch, int64_t tokens, int64_t hq, int64_t hkv, int64_t d,
+                            const void* q, int64_t q_batch, int64_t q_token, int64_t q_head, const void* k_cache,
+                            const int64_t* kc, const void* v_cache, const int64_t* vc, int64_t n_pages,
+                            int64_t page_size, const int32_t* block_table, int64_t table_width,
+                            const int32_t* lengths, const int64_t* ancestors, float scale, int64_t window,
+                            int64_t sinks, void* out, void* workspace, int64_t workspace_bytes, void* counters,
+                            int64_t counter_bytes, void* stream);
+
+/* Bytes of workspace of a tp_paged_tree_attention call on the current device
+ * (-1: sizes it does not take), and of its counters. */
+int64_t tp_paged_tree_attention_workspace_bytes(int64_t batch, int64_t tokens, int64_t hq, int64_t hkv, int64_t d);
+int64_t tp_paged_tree_attention_counter_bytes(int64_t batch, int64_t tokens, int64_t hq, int64_t hkv, int64_t d);
+
+/* Of each row of logits [rows, vocab] (of `dtype`, rows ld elements apart), with
+ * p = softmax of it: logprobs[r] = log p[tokens[r]] (tokens may be NULL; a
+ * negative token gives 0, one >= vocab NaN), entropy[r] = -sum p log p, and the
+ * `top` (0..64, at most vocab) largest log probabilities [rows, top] with their
+ * tokens, in falling order, of equal ones the lower token first.  Sums are fp32.
+ * -infinity has log probability -infinity, also where the whole row is (entropy
+ * 0).  Where a row holds NaN or +infinity, its log probabilities and entropy are
+ * NaN, and its order is NaNs, then +infinity, then the rest.  The workspace
+ * (tp_token_logprobs_workspace_bytes, 16-byte aligned) may hold anything. */
+int tp_token_logprobs(int dtype, int64_t rows, int64_t vocab, const void* logits, int64_t ld, const int64_t* tokens,
+                      float* logprobs, float* entropy, int top, float* top_logprobs, int64_t* top_tokens,
+                      void* workspace, int64_t workspace_bytes, void* stream);
+int64_t tp_token_logprobs_workspace_bytes(int64_t rows, int64_t vocab, int top);
+
+/* out[r] = y[r] + scales[i] * (x[r] a_i^T) b_i^T with i = adapters[r]: x [rows,
+ * ldx >= k], y [rows, ldy >= n], a_i [rank, k] at a + i * a_adapter (rows a_row
+ * apart), b_i [n, rank] at b + i * b_adapter (rows b_row apart), all TP_F16 or
+ * all TP_BF16, out contiguous [rows, n] (not y itself), scales fp32 (NULL: 1).  An
+ * adapter outside [0, count) leaves the row y[r].  rank is 1..256.  Sums are
+ * fp32; out rounds once.  The workspace (tp_lora_workspace_bytes, 16-byte
+ * aligned) may hold anything. */
+int tp_lora_add(int dtype, int64_t rows, int64_t k, int64_t n, int64_t rank, int64_t count, const void* x, int64_t ldx,
+                const void* a, int64_t a_adapter, int64_t a_row, const void* b, int64_t b_adapter, int64_t b_row,
+                const int32_t* adapters, const float* scales, const void* y, int64_t ldy, void* out, void* workspace,
+                int64_t workspace_bytes, void* stream);
+int64_t tp_lora_workspace_bytes(int64_t rows, int64_t k, int64_t n, int64_t rank, int64_t count);
+
 #ifdef __cplusplus
 }
 #endif

@@ -32,6 +32,10 @@ _LAZY = {
     "rotary": ("turbopress_amd.paged", "rotary"),
     "rotary_append": ("turbopress_amd.paged", "rotary_append"),
     "paged_attention": ("turbopress_amd.paged", "paged_attention"),
+    "paged_tree_attention": ("turbopress_amd.paged", "paged_tree_attention"),
+    "tree_ancestors": ("turbopress_amd.paged", "tree_ancestors"),
+    "token_logprobs": ("turbopress_amd.logprobs", "token_logprobs"),
+    "lora_add": ("turbopress_amd.lora", "lora_add"),
     "PagedDecoder": ("turbopress_amd.paged_decode", "PagedDecoder"),
 }
 

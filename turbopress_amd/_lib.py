@@ -105,6 +105,27 @@ SIGNATURES.update({
     "tp_paged_attention_counter_bytes": (_I64, [_I64, _I64, _I64, _I64]),
 })
 
+# The operators of serving many requests: drafted tokens, windows with first
+# tokens that stay visible, log probabilities, adapters.
+SIGNATURES.update({
+    "tp_rotary_slots": (c_int, [c_int, _I64, _I64, _I64, _I64, _I64, c_int, _P, _I64, _I64, _P, _I64, _I64,
+                                _P, _I64, _P, _P, _P, _I64, _I64, _P, POINTER(c_int64), _P, POINTER(c_int64),
+                                _I64, _I64, _P, _I64, _I64, _P, _P, _P]),
+    "tp_paged_attention_sinks": (c_int, [c_int, _I64, _I64, _I64, _I64, _P, _I64, _I64, _P, POINTER(c_int64),
+                                         _P, POINTER(c_int64), _I64, _I64, _P, _I64, _P, c_float, _I64, _I64, _P,
+                                         _P, _I64, _P, _I64, _P]),
+    "tp_paged_tree_attention": (c_int, [c_int, _I64, _I64, _I64, _I64, _I64, _P, _I64, _I64, _I64, _P, POINTER(c_int64),
+                                        _P, POINTER(c_int64), _I64, _I64, _P, _I64, _P, _P, c_float, _I64, _I64, _P,
+                                        _P, _I64, _P, _I64, _P]),
+    "tp_paged_tree_attention_workspace_bytes": (_I64, [_I64, _I64, _I64, _I64, _I64]),
+    "tp_paged_tree_attention_counter_bytes": (_I64, [_I64, _I64, _I64, _I64, _I64]),
+    "tp_token_logprobs": (c_int, [c_int, _I64, _I64, _P, _I64, _P, _P, _P, c_int, _P, _P, _P, _I64, _P]),
+    "tp_token_logprobs_workspace_bytes": (_I64, [_I64, _I64, c_int]),
+    "tp_lora_add": (c_int, [c_int, _I64, _I64, _I64, _I64, _I64, _P, _I64, _P, _I64, _I64, _P, _I64, _I64, _P, _P,
+                            _P, _I64, _P, _P, _I64, _P]),
+    "tp_lora_workspace_bytes": (_I64, [_I64, _I64, _I64, _I64, _I64]),
+})
+
 _LIB: ctypes.CDLL | None = None
 _LOAD_ERROR: str | None = None
 

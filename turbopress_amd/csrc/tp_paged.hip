@@ -62,7 +62,7 @@ struct PagedArgs {
   float* parts;        // two states per workgroup
   uint32_t* counters;  // per (sequence, head tile): states left so far; zero between launches
   int64_t q_batch, q_head, kc_page, kc_slot, kc_head, vc_page, vc_slot, vc_head;
-  int64_t n_pages, table_width, window;
+  int64_t n_pages, table_width, window, sinks;
   int batch, hq, hkv, group, head_tiles, d, page_size;
   float scale;  // of the scores, in base 2
 };
@@ -132,9 +132,12 @@ struct TokenRows {
   uint64_t k, v;
 };
 
-// Tokens of a sequence that attention reads: [first, len); its first unit's base.
+// Tokens of a sequence that attention reads: [0, sinks) and [first, len).  They
+// are counted through in tiles from 0: the first `near` of the count are the
+// tokens themselves, those behind lie `shift` further on.
 struct Span {
-  int first, len, base, units;
+  int first, len, sinks, near, shift, units;
+  __device__ __forceinline__ int token(int at) const { return at + (at < near ? 0 : shift); }
 };
 
 template <int UNIT>
@@ -143,9 +146,12 @@ __device__ __forceinline__ Span span_of(const PagedArgs& a, int length) {
   // (room for the last unit's tokens below 2^31)
   s.len = (int)min(min((int64_t)max(length, 0), a.table_width * a.page_size), (int64_t)0x7ffff000);
   s.first = a.window > 0 && s.len > a.window ? (int)(s.len - a.window) : 0;
-  s.base = s.first & ~(kTile - 1);
+  const int base = s.first & ~(kTile - 1);
+  s.sinks = (int)min(a.sinks, (int64_t)s.first);
+  s.near = (s.sinks + kTile - 1) & ~(kTile - 1);
+  s.shift = max(base - s.near, 0);  // (sinks up to the window's own tiles: nothing lies between)
   // (an empty sequence is one unit too: its zeros have to be written)
-  s.units = max(1, (s.len - s.base + UNIT - 1) / UNIT);
+  s.units = max(1, (s.len - s.shift + UNIT - 1) / UNIT);
   return s;
 }
 
@@ -296,15 +302,17 @@ __global__ void __launch_bounds__(64 * paged_waves<DP>(), 1) paged_attention_ker
     }
 
     const int tiles = (j1 - j0) * W;
-    const int token0 = sp.base + j0 * UNIT;
+    auto token_of = [&](int i) __attribute__((always_inline)) {  // lane's of tile i
+      return sp.token(j0 * UNIT + i * kTile) + (lane & 31);
+    };
     auto page_of = [&](int i) __attribute__((always_inline)) {  // of lane's token of tile i; -1: masked
-      const int t = token0 + i * kTile + (lane & 31);
+      const int t = token_of(i);
       int page = -1;
-      if (i < tiles && t >= sp.first && t < sp.len) page = bt[(uint32_t)t / (uint32_t)a.page_size];
+      if (i < tiles && (t >= sp.first || t < sp.sinks) && t < sp.len) page = bt[(uint32_t)t / (uint32_t)a.page_size];
       return page;  // (looked at by put_rows, a step later: here it would be waited for)
     };
     auto put_rows = [&](int i, int page) __attribute__((always_inline)) {
-      const int t = token0 + i * kTile + (lane & 31);
+      const int t = token_of(i);
       const uint32_t slot = (uint32_t)t % (uint32_t)a.page_size;
       TokenRows r{(uint64_t)zeros, (uint64_t)zeros};
       if (page >= 0 && page < a.n_pages)
@@ -558,15 +566,15 @@ extern "C" int64_t tp_paged_attention_counter_bytes(int64_t batch, int64_t hq, i
   return batch * hkv * tiles * (int64_t)sizeof(uint32_t);
 }
 
-extern "C" int tp_paged_attention(int dtype, int64_t batch, int64_t hq, int64_t hkv, int64_t d, const void* q,
+static int paged_attention(int dtype, int64_t batch, int64_t hq, int64_t hkv, int64_t d, const void* q,
                                   int64_t q_batch, int64_t q_head, const void* k_cache, const int64_t* kc,
                                   const void* v_cache, const int64_t* vc, int64_t n_pages, int64_t page_size,
                                   const int32_t* block_table, int64_t table_width, const int32_t* lengths,
-                                  float scale, int64_t window, void* out, void* workspace,
+                                  float scale, int64_t window, int64_t sinks, void* out, void* workspace,
                                   int64_t workspace_bytes, void* counters, int64_t counter_bytes, void* stream) {
   if (dtype != TP_F16 && dtype != TP_BF16) return TP_ERR_BAD_TYPE;
   if (!paged_sizes_ok(batch, hq, hkv, d) || n_pages < 0 || n_pages > 0x7fffffff || page_size < 1 || page_size > (1 << 24) ||
-      table_width < 0 || table_width > (1 << 30) || window < 0)
+      table_width < 0 || table_width > (1 << 30) || window < 0 || sinks < 0)
     return TP_ERR_BAD_DIMS;
   if (batch == 0) return TP_OK;
   if (!q || !kc || !vc || !lengths || !out || (n_pages > 0 && (!k_cache || !v_cache)) || (table_width > 0 && !block_table))
@@ -583,10 +591,31 @@ extern "C" int tp_paged_attention(int dtype, int64_t batch, int64_t hq, int64_t 
   a.parts = static_cast<float*>(workspace), a.counters = static_cast<uint32_t*>(counters);
   a.q_batch = q_batch, a.q_head = q_head;
   a.kc_page = kc[0], a.kc_slot = kc[1], a.kc_head = kc[2], a.vc_page = vc[0], a.vc_slot = vc[1], a.vc_head = vc[2];
-  a.n_pages = n_pages, a.table_width = table_width, a.window = window;
+  a.n_pages = n_pages, a.table_width = table_width, a.window = window, a.sinks = sinks;
   a.batch = (int)batch, a.hq = (int)hq, a.hkv = (int)hkv, a.group = (int)(hq / hkv), a.d = (int)d;
   a.head_tiles = (a.group + kHeadTile - 1) / kHeadTile;
   a.page_size = (int)page_size, a.scale = scale * 1.44269504088896340736f;
   hipStream_t s = (hipStream_t)stream;
   return dtype == TP_F16 ? dispatch_paged<f16_t>(a, s) : dispatch_paged<bf16_t>(a, s);
+}
+
+extern "C" int tp_paged_attention(int dtype, int64_t batch, int64_t hq, int64_t hkv, int64_t d, const void* q,
+                                  int64_t q_batch, int64_t q_head, const void* k_cache, const int64_t* kc,
+                                  const void* v_cache, const int64_t* vc, int64_t n_pages, int64_t page_size,
+                                  const int32_t* block_table, int64_t table_width, const int32_t* lengths,
+                                  float scale, int64_t window, void* out, void* workspace,
+                                  int64_t workspace_bytes, void* counters, int64_t counter_bytes, void* stream) {
+  return paged_attention(dtype, batch, hq, hkv, d, q, q_batch, q_head, k_cache, kc, v_cache, vc, n_pages, page_size, block_table,
+                         table_width, lengths, scale, window, 0, out, workspace, workspace_bytes, counters, counter_bytes, stream);
+}
+
+extern "C" int tp_paged_attention_sinks(int dtype, int64_t batch, int64_t hq, int64_t hkv, int64_t d, const void* q,
+                                        int64_t q_batch, int64_t q_head, const void* k_cache, const int64_t* kc,
+                                        const void* v_cache, const int64_t* vc, int64_t n_pages, int64_t page_size,
+                                        const int32_t* block_table, int64_t table_width, const int32_t* lengths,
+                                        float scale, int64_t window, int64_t sinks, void* out, void* workspace,
+                                        int64_t workspace_bytes, void* counters, int64_t counter_bytes, void* stream) {
+  return paged_attention(dtype, batch, hq, hkv, d, q, q_batch, q_head, k_cache, kc, v_cache, vc, n_pages, page_size, block_table,
+                         table_width, lengths, scale, window, sinks, out, workspace, workspace_bytes, counters, counter_bytes,
+                         stream);
 }

@@ -19,7 +19,7 @@ struct RotaryArgs {
   const void *q, *k, *v;
   void *q_out, *k_out, *k_cache, *v_cache;
   const float* table;
-  const int64_t* positions;
+  const int64_t *positions, *slots;  // slots: where in the cache, if not at the position
   const int32_t *block_table, *sequences;
   int64_t q_token, q_head, k_token, k_head, v_token, v_head, kc_page, kc_slot, kc_head, vc_page, vc_slot, vc_head;
   int64_t tokens, n_positions, n_pages, page_size, table_width, n_sequences;
@@ -71,9 +71,11 @@ __global__ void __launch_bounds__(256) rotary_kernel(const RotaryArgs a) {
     if (a.k_cache) {
       if (padding || past) return;
       const int64_t seq = a.sequences ? (int64_t)a.sequences[t] : t;
-      const int64_t col = p / a.page_size;
+      const int64_t place = a.slots ? a.slots[t] : p;
+      if (place < 0) return;
+      const int64_t col = place / a.page_size;
       if (seq < 0 || seq >= a.n_sequences || col >= a.table_width) return;
-      const int64_t page = a.block_table[seq * a.table_width + col], slot = p - col * a.page_size;
+      const int64_t page = a.block_table[seq * a.table_width + col], slot = place - col * a.page_size;
       if (page < 0 || page >= a.n_pages) return;
       dst = is_v ? static_cast<T*>(a.v_cache) + page * a.vc_page + slot * a.vc_slot + head * a.vc_head
                  : static_cast<T*>(a.k_cache) + page * a.kc_page + slot * a.kc_slot + head * a.kc_head;
@@ -142,13 +144,13 @@ int launch_rotary(RotaryArgs a, hipStream_t s) {
 
 using namespace tp;
 
-extern "C" int tp_rotary(int dtype, int64_t tokens, int64_t hq, int64_t hk, int64_t d, int64_t rotary_dim,
+static int rotary(int dtype, int64_t tokens, int64_t hq, int64_t hk, int64_t d, int64_t rotary_dim,
                          int interleaved, const void* q, int64_t q_token, int64_t q_head, const void* k,
                          int64_t k_token, int64_t k_head, const float* table, int64_t n_positions,
                          const int64_t* positions, void* q_out, void* k_out, const void* v, int64_t v_token,
                          int64_t v_head, void* k_cache, const int64_t* kc, void* v_cache, const int64_t* vc,
                          int64_t n_pages, int64_t page_size, const int32_t* block_table, int64_t table_width,
-                         int64_t n_sequences, const int32_t* sequences, void* stream) {
+                         int64_t n_sequences, const int32_t* sequences, const int64_t* slots, void* stream) {
   if (!dtype_ok(dtype)) return TP_ERR_BAD_TYPE;
   if (tokens < 0 || hq < 0 || hk < 0 || hq > 65536 || hk > 65536 || d < 2 || d > 65536 || (d & 1) || rotary_dim < 2 ||
       rotary_dim > d || (rotary_dim & 1) || n_positions < 0 || tokens > ((int64_t)1 << 40))
@@ -167,10 +169,10 @@ extern "C" int tp_rotary(int dtype, int64_t tokens, int64_t hq, int64_t hk, int6
   const uintptr_t mask = dtype_bytes(dtype) - 1;
   if ((((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)q_out | (uintptr_t)k_out | (uintptr_t)k_cache |
         (uintptr_t)v_cache) & mask) || (((uintptr_t)table | (uintptr_t)block_table | (uintptr_t)sequences) & 3) ||
-      ((uintptr_t)positions & 7))
+      (((uintptr_t)positions | (uintptr_t)slots) & 7))
     return TP_ERR_MISALIGNED;
   a.q = q, a.k = k, a.v = v, a.q_out = q_out, a.k_out = k_out, a.k_cache = k_cache, a.v_cache = v_cache;
-  a.table = table, a.positions = positions, a.block_table = block_table, a.sequences = sequences;
+  a.table = table, a.positions = positions, a.slots = slots, a.block_table = block_table, a.sequences = sequences;
   a.q_token = q_token, a.q_head = q_head, a.k_token = k_token, a.k_head = k_head, a.v_token = v_token, a.v_head = v_head;
   a.tokens = tokens, a.n_positions = n_positions, a.n_pages = n_pages, a.page_size = page_size;
   a.table_width = table_width, a.n_sequences = n_sequences;
@@ -179,4 +181,29 @@ extern "C" int tp_rotary(int dtype, int64_t tokens, int64_t hq, int64_t hk, int6
   if (dtype == TP_F16) return launch_rotary<f16_t>(a, s);
   if (dtype == TP_BF16) return launch_rotary<bf16_t>(a, s);
   return launch_rotary<float>(a, s);
+}
+
+extern "C" int tp_rotary(int dtype, int64_t tokens, int64_t hq, int64_t hk, int64_t d, int64_t rotary_dim,
+                         int interleaved, const void* q, int64_t q_token, int64_t q_head, const void* k,
+                         int64_t k_token, int64_t k_head, const float* table, int64_t n_positions,
+                         const int64_t* positions, void* q_out, void* k_out, const void* v, int64_t v_token,
+                         int64_t v_head, void* k_cache, const int64_t* kc, void* v_cache, const int64_t* vc,
+                         int64_t n_pages, int64_t page_size, const int32_t* block_table, int64_t table_width,
+                         int64_t n_sequences, const int32_t* sequences, void* stream) {
+  return rotary(dtype, tokens, hq, hk, d, rotary_dim, interleaved, q, q_token, q_head, k, k_token, k_head, table, n_positions,
+                positions, q_out, k_out, v, v_token, v_head, k_cache, kc, v_cache, vc, n_pages, page_size, block_table,
+                table_width, n_sequences, sequences, nullptr, stream);
+}
+
+extern "C" int tp_rotary_slots(int dtype, int64_t tokens, int64_t hq, int64_t hk, int64_t d, int64_t rotary_dim,
+                               int interleaved, const void* q, int64_t q_token, int64_t q_head, const void* k,
+                               int64_t k_token, int64_t k_head, const float* table, int64_t n_positions,
+                               const int64_t* positions, void* q_out, const void* v, int64_t v_token, int64_t v_head,
+                               void* k_cache, const int64_t* kc, void* v_cache, const int64_t* vc, int64_t n_pages,
+                               int64_t page_size, const int32_t* block_table, int64_t table_width,
+                               int64_t n_sequences, const int32_t* sequences, const int64_t* slots, void* stream) {
+  if (tokens > 0 && (!k_cache || !slots)) return TP_ERR_NULL_POINTER;
+  return rotary(dtype, tokens, hq, hk, d, rotary_dim, interleaved, q, q_token, q_head, k, k_token, k_head, table, n_positions,
+                positions, q_out, nullptr, v, v_token, v_head, k_cache, kc, v_cache, vc, n_pages, page_size, block_table,
+                table_width, n_sequences, sequences, slots, stream);
 }

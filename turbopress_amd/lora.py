@@ -1,0 +1,91 @@
+"""Low-rank adapters of many requests beside a shared projection
+(csrc/tp_lora.hip): the packed weights stay one for all, and each row of a batch
+adds the product of its own request's adapter.  Inference only.
+"""
+
+from __future__ import annotations
+
+import torch
+from torch import Tensor
+
+from turbopress_amd import _lib
+from turbopress_amd.hip_kernel import raw_stream as _raw_stream
+from turbopress_amd.norm import DTYPE_CODES
+
+__all__ = ["lora_add", "MAX_RANK"]
+
+MAX_RANK = 256
+
+
+def _refuse(y, x, a, b, adapters, scales) -> None:
+    """Raise for arguments that lora_add does not take."""
+    if not y.is_cuda:
+        raise RuntimeError("y must be a CUDA (ROCm) tensor; turbopress_amd has no CPU path")
+    dt, dev = y.dtype, y.device
+
+    def expect(ok, name, t, what):
+        if not ok:
+            raise ValueError(f"{name} must be {what}, got {t.dtype} {list(t.shape)} on {t.device}")
+
+    expect(dt in (torch.float16, torch.bfloat16) and y.dim() >= 1 and y.shape[-1] >= 1, "y", y, "fp16 or bf16 [..., out]")
+    expect(x.dtype == dt and x.device == dev and x.dim() == y.dim() and x.shape[:-1] == y.shape[:-1] and x.shape[-1] >= 1, "x", x,
+           f"{dt} {[*y.shape[:-1], 'in']} on {dev}")
+    expect(a.dtype == dt and a.device == dev and a.dim() == 3 and a.shape[2] == x.shape[-1] and 1 <= a.shape[1] <= MAX_RANK, "a", a,
+           f"{dt} [adapters, 1 to {MAX_RANK} ranks, {x.shape[-1]}] on {dev}")
+    expect(b.dtype == dt and b.device == dev and b.shape == (a.shape[0], y.shape[-1], a.shape[1]), "b", b,
+           f"{dt} {[a.shape[0], y.shape[-1], a.shape[1]]} on {dev}")
+    expect(adapters.dtype == torch.int32 and adapters.device == dev and adapters.shape == y.shape[:-1], "adapters", adapters,
+           f"int32 {list(y.shape[:-1])} on {dev}")
+    expect(scales.dtype == torch.float32 and scales.device == dev and scales.shape == a.shape[:1], "scales", scales,
+           f"fp32 {list(a.shape[:1])} on {dev}")
+
+
+def _flat(t: Tensor, width: int) -> tuple:
+    """(tensor, elements from a row to the next) of [..., width] as rows."""
+    if t.dim() == 2 and (t.stride(1) == 1 or width == 1) and t.stride(0) >= 0:
+        return t, t.stride(0)
+    return (t if t.is_contiguous() else t.contiguous()), width
+
+
+def _weights(w: Tensor) -> Tensor:
+    return w if w.stride(2) == 1 or w.shape[2] == 1 else w.contiguous()
+
+
+def lora_add(y: Tensor, x: Tensor, a: Tensor, b: Tensor, adapters: Tensor, scales: Tensor | None = None) -> Tensor:
+    """``y + scales[i] * (x @ a[i]^T) @ b[i]^T`` with i = adapters of the row: y
+    [..., out], the shared projection's output of x [..., in] (fp16 or bf16, all
+    of one type); a [adapters, rank, in] and b [adapters, out, rank], the stacked
+    adapters (ranks up to 256; smaller ones are padded with zeros); adapters int32
+    [...], one per row, of which one that does not exist (-1) leaves its row as it
+    is; scales fp32 [adapters] (None: 1).  Returns a new tensor; both products are
+    summed in fp32, and the result rounds once."""
+    code, index = DTYPE_CODES.get(y.dtype, _lib.TP_F32), y.get_device()
+    lead = y.shape[:-1]
+    if code == _lib.TP_F32 or index < 0 or y.dim() < 1 or x.dtype is not y.dtype or x.get_device() != index or x.dim() != y.dim() \
+            or x.shape[:-1] != lead or a.dtype is not y.dtype or a.get_device() != index or a.dim() != 3 \
+            or a.shape[2] != x.shape[-1] or not 1 <= a.shape[1] <= MAX_RANK or b.dtype is not y.dtype or b.get_device() != index \
+            or b.shape != (a.shape[0], y.shape[-1], a.shape[1]) or adapters.dtype is not torch.int32 \
+            or adapters.get_device() != index or adapters.shape != lead or x.shape[-1] < 1 or y.shape[-1] < 1 \
+            or (scales is not None and (scales.dtype is not torch.float32 or scales.get_device() != index
+                                        or scales.shape != a.shape[:1])):
+        _refuse(y, x, a, b, adapters, scales)
+    k, n = x.shape[-1], y.shape[-1]
+    count, rank, _ = a.shape
+    out = torch.empty_like(y, memory_format=torch.contiguous_format)
+    rows = out.numel() // n
+    (x, ldx), (y, ldy), a, b = _flat(x, k), _flat(y, n), _weights(a), _weights(b)
+    if not adapters.is_contiguous():
+        adapters = adapters.contiguous()
+    if scales is not None and not scales.is_contiguous():
+        scales = scales.contiguous()
+    lib = _lib.lib()
+    need = lib.tp_lora_workspace_bytes(rows, k, n, rank, count)
+    ws = torch.empty(max(need, 16), dtype=torch.uint8, device=out.device)
+    a_adapter, a_row, _ = a.stride()
+    b_adapter, b_row, _ = b.stride()
+    st = lib.tp_lora_add(code, rows, k, n, rank, count, x.data_ptr(), ldx, a.data_ptr(), a_adapter, a_row, b.data_ptr(), b_adapter,
+                         b_row, adapters.data_ptr(), 0 if scales is None else scales.data_ptr(), y.data_ptr(), ldy,
+                         out.data_ptr(), ws.data_ptr(), need, _raw_stream(index))
+    if st:
+        _lib.check(st, "lora_add")
+    return out

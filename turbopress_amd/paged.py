@@ -1,5 +1,5 @@
-"""Rotary positions, the paged cache's writes, and attention of one new token
-over it (csrc/tp_rotary.hip, csrc/tp_paged.hip).
+"""Rotary positions, the paged cache's writes, and attention over it of one new
+token or of a tree of drafted ones (csrc/tp_rotary.hip, csrc/tp_paged.hip).
 
 A paged cache is two tensors ``k_cache`` and ``v_cache`` [n_pages, page_size,
 kv heads, head_dim] (any strides with contiguous head columns, so a [n_pages, kv
@@ -26,7 +26,10 @@ from turbopress_amd import hip_kernel as hk
 from turbopress_amd.hip_kernel import raw_stream as _raw_stream
 from turbopress_amd.norm import DTYPE_CODES
 
-__all__ = ["rotary_frequencies", "rotary_table", "rotary", "rotary_append", "paged_attention"]
+__all__ = ["rotary_frequencies", "rotary_table", "rotary", "rotary_append", "paged_attention", "paged_tree_attention",
+           "tree_ancestors", "TREE_TOKENS"]
+
+TREE_TOKENS = 64  # drafted tokens of a sequence: a bit of its ancestors each
 
 
 def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: dict | None = None) -> tuple:
@@ -212,21 +215,30 @@ def rotary(q: Tensor, k: Tensor | None, table: Tensor, positions: Tensor, interl
 
 
 def rotary_append(q: Tensor, k: Tensor, v: Tensor, table: Tensor, positions: Tensor, k_cache: Tensor, v_cache: Tensor,
-                  block_table: Tensor, sequences: Tensor | None = None, interleaved: bool = False) -> Tensor:
+                  block_table: Tensor, sequences: Tensor | None = None, interleaved: bool = False,
+                  slots: Tensor | None = None) -> Tensor:
     """``rotary`` with the rotated k and v written into a paged cache in the same
     launch; returns the rotated q.
 
     Token t goes to position positions[t] of sequence sequences[t] (int32
     [tokens]; None: token t is sequence t's).  Padding (a negative position), a
     position past the table or past block_table's width, and a page or a
-    sequence that does not exist write nothing."""
+    sequence that does not exist write nothing.
+
+    slots (int64 [tokens]): the key and value go to token slots[t] of the
+    sequence's cache in place of positions[t], for drafted tokens of a tree, which
+    share positions; a negative one writes nothing."""
     if k is None or v is None or k_cache is None or v_cache is None or block_table is None:
         raise ValueError("rotary_append needs k, v, k_cache, v_cache and block_table")
     code, index, tokens, hq, d, rd = _turn(q, k, table, positions)
     if v.dtype is not q.dtype or v.get_device() != index or v.shape != k.shape \
             or not _cached(k_cache, v_cache, block_table, q, index, d) or k_cache.shape[2] != k.shape[1] \
             or (sequences is None and tokens > block_table.shape[0]) or (sequences is not None and (
-                sequences.dtype is not torch.int32 or sequences.shape != (tokens,) or sequences.get_device() != index)):
+                sequences.dtype is not torch.int32 or sequences.shape != (tokens,) or sequences.get_device() != index)) \
+            or (slots is not None and (slots.dtype is not torch.int64 or slots.shape != (tokens,) or slots.get_device() != index)):
+        if slots is not None:
+            _expect(slots.dtype == torch.int64 and slots.device == q.device and slots.shape == (tokens,), "slots", slots,
+                    f"int64 [{tokens}] on {q.device}")
         _refuse(q, k, v, table, positions, k_cache, v_cache, block_table, sequences)
     q, k, v = _columns(q), _columns(k), _columns(v)
     q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
@@ -239,6 +251,17 @@ def rotary_append(q: Tensor, k: Tensor, v: Tensor, table: Tensor, positions: Ten
     q_token, q_head, _ = q.stride()
     k_token, k_head, _ = k.stride()
     v_token, v_head, _ = v.stride()
+    if slots is not None:
+        if not slots.is_contiguous():
+            slots = slots.contiguous()
+        st = _lib.lib().tp_rotary_slots(
+            code, tokens, hq, heads, d, rd, interleaved, q.data_ptr(), q_token, q_head, k.data_ptr(), k_token, k_head,
+            table.data_ptr(), table.shape[0], positions.data_ptr(), q_out.data_ptr(), v.data_ptr(), v_token, v_head,
+            k_cache.data_ptr(), _strides(k_cache), v_cache.data_ptr(), _strides(v_cache), pages, page_size, block_table.data_ptr(),
+            width, rows, 0 if sequences is None else sequences.data_ptr(), slots.data_ptr(), _raw_stream(index))
+        if st:
+            _lib.check(st, "rotary_append")
+        return q_out
     st = _lib.lib().tp_rotary(code, tokens, hq, heads, d, rd, interleaved, q.data_ptr(), q_token, q_head, k.data_ptr(),
                               k_token, k_head, table.data_ptr(), table.shape[0], positions.data_ptr(), q_out.data_ptr(), 0,
                               v.data_ptr(), v_token, v_head, k_cache.data_ptr(), _strides(k_cache), v_cache.data_ptr(),
@@ -281,10 +304,10 @@ def _workspace(index: int, stream: int, need: int, count: int) -> tuple:
 
 
 def paged_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, block_table: Tensor, lengths: Tensor,
-                    scale: float | None = None, window: int = 0) -> Tensor:
+                    scale: float | None = None, window: int = 0, sinks: int = 0) -> Tensor:
     """Attention of one new token per sequence, q [sequences, heads, d] (fp16 or
-    bf16), over its cached tokens [0, lengths[s]), or the last `window` of them:
-    [sequences, heads, d], contiguous.  Query head h reads cache head
+    bf16), over its cached tokens [0, lengths[s]), or the last `window` of them
+    and the first `sinks`: [sequences, heads, d], contiguous.  Query head h reads cache head
     h // (heads / kv heads); d is a multiple of 8 up to 256; lengths: int32
     [sequences], on the device (the host never waits for them), a length of 0
     gives zeros; scale: 1 / sqrt(d) by default.
@@ -296,6 +319,8 @@ def paged_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, block_table: Te
     code = DTYPE_CODES.get(q.dtype, _lib.TP_F32)
     if window < 0:
         raise ValueError(f"window must be 0 (none) or positive, got {window}")
+    if sinks < 0:
+        raise ValueError(f"sinks must be 0 (none) or positive, got {sinks}")
     if q.dim() != 3 or index < 0 or code == _lib.TP_F32 or not _cached(k_cache, v_cache, block_table, q, index, q.shape[2]) \
             or block_table.shape[0] != q.shape[0] or lengths.dtype is not torch.int32 or lengths.shape != q.shape[:1] \
             or lengths.get_device() != index:
@@ -318,10 +343,111 @@ def paged_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, block_table: Te
     stream = _raw_stream(index)
     need, count = _needs(index, b, hq, hkv, d)
     ws, counters, _held = _workspace(index, stream, need, count)
-    st = _lib.lib().tp_paged_attention(
-        code, b, hq, hkv, d, qp, q_row, q_head, k_cache.data_ptr(), _strides(k_cache), v_cache.data_ptr(), _strides(v_cache),
-        pages, page_size, block_table.data_ptr(), block_table.shape[1], lengths.data_ptr(),
-        d ** -0.5 if scale is None else scale, window, out.data_ptr(), ws, need, counters, count, stream)
+    if sinks:
+        st = _lib.lib().tp_paged_attention_sinks(
+            code, b, hq, hkv, d, qp, q_row, q_head, k_cache.data_ptr(), _strides(k_cache), v_cache.data_ptr(), _strides(v_cache),
+            pages, page_size, block_table.data_ptr(), block_table.shape[1], lengths.data_ptr(),
+            d ** -0.5 if scale is None else scale, window, sinks, out.data_ptr(), ws, need, counters, count, stream)
+    else:
+        st = _lib.lib().tp_paged_attention(
+            code, b, hq, hkv, d, qp, q_row, q_head, k_cache.data_ptr(), _strides(k_cache), v_cache.data_ptr(), _strides(v_cache),
+            pages, page_size, block_table.data_ptr(), block_table.shape[1], lengths.data_ptr(),
+            d ** -0.5 if scale is None else scale, window, out.data_ptr(), ws, need, counters, count, stream)
     if st:
         _lib.check(st, "paged_attention")
+    return out
+
+
+def tree_ancestors(parents: Tensor) -> Tensor:
+    """The ``ancestors`` of ``paged_tree_attention`` from the drafted tokens'
+    parents: int64 [..., tokens] of indices, each below its own (-1: it follows
+    the cache; -2: there is no token), on the host or the device.  Bit j of
+    token i is set where token j is i or one that it follows."""
+    if parents.dtype != torch.int64 or parents.dim() < 1 or not 1 <= parents.shape[-1] <= TREE_TOKENS:
+        raise ValueError(f"parents must be int64 [..., 1 to {TREE_TOKENS} tokens], got {parents.dtype} {list(parents.shape)}")
+    out = torch.zeros_like(parents, memory_format=torch.contiguous_format)
+    for i in range(parents.shape[-1]):
+        own = 1 << i if i < 63 else -1 << 63
+        p = parents[..., i:i + 1]
+        before = torch.where(p >= 0, out.gather(-1, p.clamp(0, max(0, i - 1))), 0)  # (nothing is in places i and on yet)
+        out[..., i:i + 1] = torch.where(p >= -1, before | own, 0)
+    return out
+
+
+@functools.lru_cache(maxsize=1024)
+def _tree_needs(index: int, batch: int, tokens: int, hq: int, hkv: int, d: int) -> tuple:
+    """(workspace bytes, counter bytes) of a call on a device."""
+    lib = _lib.lib()
+    return (lib.tp_paged_tree_attention_workspace_bytes(batch, tokens, hq, hkv, d),
+            lib.tp_paged_tree_attention_counter_bytes(batch, tokens, hq, hkv, d))
+
+
+def _refuse_tree(q, k_cache, v_cache, block_table, lengths, ancestors) -> None:
+    """Raise for the first argument that paged_tree_attention does not take."""
+    if not q.is_cuda:
+        raise RuntimeError("q must be a CUDA (ROCm) tensor; turbopress_amd has no CPU path")
+    _expect(q.dim() == 4 and 1 <= q.shape[1] <= TREE_TOKENS and q.dtype in (torch.float16, torch.bfloat16), "q", q,
+            f"fp16 or bf16 [sequences, 1 to {TREE_TOKENS} tokens, heads, head_dim]")
+    if ancestors is not None:
+        _expect(ancestors.dtype == torch.int64 and ancestors.device == q.device and ancestors.shape == q.shape[:2], "ancestors",
+                ancestors, f"int64 {list(q.shape[:2])} on {q.device}")
+    _refuse(q[:, 0], None, None, None, None, k_cache, v_cache, block_table, None, lengths)
+
+
+def paged_tree_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, block_table: Tensor, lengths: Tensor,
+                         ancestors: Tensor | None = None, scale: float | None = None, window: int = 0,
+                         sinks: int = 0) -> Tensor:
+    """Attention of several new tokens of each sequence at once, q [sequences,
+    tokens, heads, d] (fp16 or bf16, up to 64 tokens): [sequences, tokens, heads,
+    d], contiguous.  Heads, d, scale and the cache are as in ``paged_attention``.
+
+    lengths: int32 [sequences], the tokens in the cache *before* the new ones; new
+    token i's own key and value are at token lengths[s] + i of the cache
+    (``rotary_append`` with ``slots`` first).  ancestors: int64 [sequences,
+    tokens], bit j of entry i set where new token i sees new token j, itself among
+    them (``tree_ancestors``); None: a chain, each sees those up to itself.  Every
+    new token sees the cache before them; an entry of 0 sees only that (rows
+    behind a sequence's last token; with a length of 0 they give zeros).
+
+    window: a token at position p sees positions above p - window and the first
+    `sinks`; cached token t is at position t, new token i at lengths[s] - 1 + the
+    number of new tokens that it sees."""
+    index = q.get_device()
+    code = DTYPE_CODES.get(q.dtype, _lib.TP_F32)
+    if window < 0:
+        raise ValueError(f"window must be 0 (none) or positive, got {window}")
+    if sinks < 0:
+        raise ValueError(f"sinks must be 0 (none) or positive, got {sinks}")
+    if q.dim() != 4 or index < 0 or code == _lib.TP_F32 or not 1 <= q.shape[1] <= TREE_TOKENS \
+            or not _cached(k_cache, v_cache, block_table, q, index, q.shape[3]) \
+            or block_table.shape[0] != q.shape[0] or lengths.dtype is not torch.int32 or lengths.shape != q.shape[:1] \
+            or lengths.get_device() != index or (ancestors is not None and (
+                ancestors.dtype is not torch.int64 or ancestors.shape != q.shape[:2] or ancestors.get_device() != index)):
+        _refuse_tree(q, k_cache, v_cache, block_table, lengths, ancestors)
+    b, tokens, hq, d = q.shape
+    pages, page_size, hkv, _ = k_cache.shape
+    if d % 8 or not 8 <= d <= 256 or hq < 1 or hkv < 1 or hq % hkv:
+        _refuse_tree(q, k_cache, v_cache, block_table, lengths, ancestors)
+    q_row, q_token, q_head, q_column = q.stride()
+    qp = q.data_ptr()
+    if q_column != 1 or (qp | q_row << 1 | q_token << 1 | q_head << 1) & 15:  # (a row of 16-byte pieces)
+        q = q.clone(memory_format=torch.contiguous_format)
+        q_row, q_token, q_head, qp = tokens * hq * d, hq * d, d, q.data_ptr()
+    if not lengths.is_contiguous():
+        lengths = lengths.contiguous()
+    if ancestors is not None and not ancestors.is_contiguous():
+        ancestors = ancestors.contiguous()
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    if b == 0:
+        return out
+    stream = _raw_stream(index)
+    need, count = _tree_needs(index, b, tokens, hq, hkv, d)
+    ws, counters, _held = _workspace(index, stream, need, count)
+    st = _lib.lib().tp_paged_tree_attention(
+        code, b, tokens, hq, hkv, d, qp, q_row, q_token, q_head, k_cache.data_ptr(), _strides(k_cache), v_cache.data_ptr(),
+        _strides(v_cache), pages, page_size, block_table.data_ptr(), block_table.shape[1], lengths.data_ptr(),
+        0 if ancestors is None else ancestors.data_ptr(), d ** -0.5 if scale is None else scale, window, sinks, out.data_ptr(),
+        ws, need, counters, count, stream)
+    if st:
+        _lib.check(st, "paged_tree_attention")
     return out
