@@ -553,11 +553,18 @@ int64_t tp_paged_tree_attention_counter_bytes(int64_t batch, int64_t tokens, int
  * -infinity has log probability -infinity, also where the whole row is (entropy
  * 0).  Where a row holds NaN or +infinity, its log probabilities and entropy are
  * NaN, and its order is NaNs, then +infinity, then the rest.  The workspace
- * (tp_token_logprobs_workspace_bytes, 16-byte aligned) may hold anything. */
+ * (tp_token_logprobs_workspace_bytes, 16-byte aligned) may hold anything; the
+ * counters (tp_token_logprobs_counter_bytes, 4-byte aligned) are zero before and
+ * after every call, as tp_paged_attention's.  The 16-byte pieces of memory that
+ * hold a row's ends are read whole. */
 int tp_token_logprobs(int dtype, int64_t rows, int64_t vocab, const void* logits, int64_t ld, const int64_t* tokens,
                       float* logprobs, float* entropy, int top, float* top_logprobs, int64_t* top_tokens,
-                      void* workspace, int64_t workspace_bytes, void* stream);
+                      void* workspace, int64_t workspace_bytes, void* counters, int64_t counter_bytes, void* stream);
+
+/* Bytes of workspace of a tp_token_logprobs call (-1: sizes it does not take: up
+ * to 2^24 rows, vocab to 2^24 - 8), and of its counters. */
 int64_t tp_token_logprobs_workspace_bytes(int64_t rows, int64_t vocab, int top);
+int64_t tp_token_logprobs_counter_bytes(int64_t rows, int64_t vocab, int top);
 
 /* out[r] = y[r] + scales[i] * (x[r] a_i^T) b_i^T with i = adapters[r]: x [rows,
  * ldx >= k], y [rows, ldy >= n], a_i [rank, k] at a + i * a_adapter (rows a_row

@@ -119,8 +119,9 @@ SIGNATURES.update({
                                         _P, _I64, _P, _I64, _P]),
     "tp_paged_tree_attention_workspace_bytes": (_I64, [_I64, _I64, _I64, _I64, _I64]),
     "tp_paged_tree_attention_counter_bytes": (_I64, [_I64, _I64, _I64, _I64, _I64]),
-    "tp_token_logprobs": (c_int, [c_int, _I64, _I64, _P, _I64, _P, _P, _P, c_int, _P, _P, _P, _I64, _P]),
+    "tp_token_logprobs": (c_int, [c_int, _I64, _I64, _P, _I64, _P, _P, _P, c_int, _P, _P, _P, _I64, _P, _I64, _P]),
     "tp_token_logprobs_workspace_bytes": (_I64, [_I64, _I64, c_int]),
+    "tp_token_logprobs_counter_bytes": (_I64, [_I64, _I64, c_int]),
     "tp_lora_add": (c_int, [c_int, _I64, _I64, _I64, _I64, _I64, _P, _I64, _P, _I64, _I64, _P, _I64, _I64, _P, _P,
                             _P, _I64, _P, _P, _I64, _P]),
     "tp_lora_workspace_bytes": (_I64, [_I64, _I64, _I64, _I64, _I64]),

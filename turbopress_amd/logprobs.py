@@ -5,6 +5,7 @@ checks drafted ones.  Inference only: no gradient flows through.
 
 from __future__ import annotations
 
+import functools
 from typing import NamedTuple
 
 import torch
@@ -13,6 +14,7 @@ from torch import Tensor
 from turbopress_amd import _lib
 from turbopress_amd.hip_kernel import raw_stream as _raw_stream
 from turbopress_amd.norm import DTYPE_CODES
+from turbopress_amd.paged import _workspace
 
 __all__ = ["token_logprobs", "TokenLogprobs", "MAX_TOP"]
 
@@ -27,6 +29,13 @@ class TokenLogprobs(NamedTuple):
     entropy: Tensor
     top_logprobs: Tensor | None
     top_tokens: Tensor | None
+
+
+@functools.lru_cache(maxsize=1024)
+def _needs(rows: int, vocab: int, top: int) -> tuple:
+    """(workspace bytes, counter bytes) of a call."""
+    lib = _lib.lib()
+    return lib.tp_token_logprobs_workspace_bytes(rows, vocab, top), lib.tp_token_logprobs_counter_bytes(rows, vocab, top)
 
 
 def _refuse(logits: Tensor, tokens: Tensor | None, top: int) -> None:
@@ -66,12 +75,13 @@ def token_logprobs(logits: Tensor, tokens: Tensor | None = None, top: int = 0) -
     lib = _lib.lib()
     out = torch.empty(rows * (2 + top), dtype=torch.float32, device=logits.device)
     ids = torch.empty(rows, top, dtype=torch.int64, device=logits.device) if top else None
-    need = lib.tp_token_logprobs_workspace_bytes(rows, vocab, top)
-    ws = torch.empty(max(need, 16), dtype=torch.uint8, device=logits.device)
     p = out.data_ptr()
+    stream = _raw_stream(index)
+    need, count = _needs(rows, vocab, top)
+    ws, counters, _held = _workspace(index, stream, max(need, 16), count)
     st = lib.tp_token_logprobs(code, rows, vocab, logits.data_ptr(), ld, 0 if tokens is None else tokens.data_ptr(), p,
-                               p + 4 * rows, top, p + 8 * rows, 0 if ids is None else ids.data_ptr(), ws.data_ptr(), need,
-                               _raw_stream(index))
+                               p + 4 * rows, top, p + 8 * rows, 0 if ids is None else ids.data_ptr(), ws, need, counters,
+                               count, stream)
     if st:
         _lib.check(st, "token_logprobs")
     return TokenLogprobs(None if tokens is None else out[:rows], out[rows:2 * rows], out[2 * rows:].view(rows, top) if top else None,
