@@ -571,12 +571,15 @@ int64_t tp_token_logprobs_counter_bytes(int64_t rows, int64_t vocab, int top);
  * apart), b_i [n, rank] at b + i * b_adapter (rows b_row apart), all TP_F16 or
  * all TP_BF16, out contiguous [rows, n] (not y itself), scales fp32 (NULL: 1).  An
  * adapter outside [0, count) leaves the row y[r].  rank is 1..256.  Sums are
- * fp32; out rounds once.  The workspace (tp_lora_workspace_bytes, 16-byte
- * aligned) may hold anything. */
+ * fp32; out rounds once.  Rows of x and of a_i are at most 2^24 apart.  The
+ * workspace (tp_lora_workspace_bytes, 16-byte aligned) may hold anything. */
 int tp_lora_add(int dtype, int64_t rows, int64_t k, int64_t n, int64_t rank, int64_t count, const void* x, int64_t ldx,
                 const void* a, int64_t a_adapter, int64_t a_row, const void* b, int64_t b_adapter, int64_t b_row,
                 const int32_t* adapters, const float* scales, const void* y, int64_t ldy, void* out, void* workspace,
                 int64_t workspace_bytes, void* stream);
+
+/* Bytes of workspace of a tp_lora_add call (-1: sizes it does not take: up to 2^24
+ * rows and 2^20 columns). */
 int64_t tp_lora_workspace_bytes(int64_t rows, int64_t k, int64_t n, int64_t rank, int64_t count);
 
 #ifdef __cplusplus

@@ -2,7 +2,8 @@
 //
 //   out[r] = y[r] + scale_i (x[r] A_i^T) B_i^T,  i = adapters[r]
 //
-// in two launches, h = x A^T, then the rest.  2 rank flops for each element of x
+// in two launches, h = x A^T, then the rest (three where the first product's long
+// sum is cut).  2 rank flops for each element of x
 // and y: bound by HBM (x, y and out once, each used adapter's weights once), or by
 // latency for few rows.
 //
@@ -12,11 +13,11 @@
 // belongs to another adapter's rows is just not kept.  Of few rows the distinct
 // adapters are shared out over further workgroups (`slots`).
 //
-// The first product is cut along its long sum: parts of fp32, added in order by
-// the second launch, which takes h as two numbers of the weights' type, its
-// leading bits and what they leave (2^-16 of it are lost in bf16, in fp16, whose
-// row is scaled by a power of two to the type's range, 2^-21 of the row's
-// largest): one number would lose as much as the output's rounding.
+// h is left in the order of the second product's operands, as two numbers of the
+// weights' type, its leading bits and what they leave (2^-16 of it are lost in
+// bf16, in fp16, where 32 ranks of a row are scaled by a power of two to the type's
+// range, 2^-21 of their largest): one number would lose as much as the output's
+// rounding.
 #include "tp_ops_common.h"
 
 #include <algorithm>
@@ -49,22 +50,30 @@ struct LoraArgs {
   void* out;
   const int32_t* adapters;
   const float* scales;
-  float* h;  // [parts][rows][hr]
+  float* parts_h;     // [parts][rows][hr], where there are several
+  void *lead, *rest;  // h's two numbers: [16 rows][step of 32 ranks][lane] operands
+  int* power;         // fp16: [rows][step], the power of two of h
   int64_t ldx, ldy, a_adapter, a_row, b_adapter, b_row, rows;
   int k, n, rank, count;
-  int parts, slots, hr, steps;  // steps: of 32 columns of x
+  int parts, slots, hr, lines, steps;  // lines: of 64 columns of a row of x
 };
 
-// 8 elements at any alignment, those from `left` on zeros.
+// 8 elements at any alignment.
+template <typename V, typename T>
+__device__ __forceinline__ V load_eight(const T* p) {
+  V v;
+  __builtin_memcpy(&v, p, sizeof(v));
+  return v;
+}
+// Those from `left` on zeros; the row's last element, at left - 1, may be read in
+// their place (left may be 0 and less: no branch, the loads are in flight together).
 template <typename V, typename T>
 __device__ __forceinline__ V load_upto(const T* p, int left) {
-  V v{};
-  if (left >= 8) {
-    __builtin_memcpy(&v, p, sizeof(v));
-  } else {
+  V v;
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
-      if (e < left) v[e] = p[e];
+  for (int e = 0; e < 8; ++e) {
+    const T x = p[min(e, left - 1)];
+    v[e] = e < left ? x : (T)0.0f;
   }
   return v;
 }
@@ -83,173 +92,223 @@ __device__ __forceinline__ void each_adapter(int id, uint64_t pending, int slot,
   }
 }
 
+// 8 ranks from 8 c on of a row's h (its sums v, unscaled), by four lanes a step of
+// 32 (aligned in their wave, all of them active).
+template <typename T>
+__device__ __forceinline__ void leave_h(const LoraArgs& p, int64_t row, int c, f32x4 (&v)[2], float scale) {
+  typedef typename LoraMma<T>::v8 v8;
+  float most = 0.0f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float f = 8 * c + e < p.rank ? v[e / 4][e % 4] * scale : 0.0f;
+    v[e / 4][e % 4] = f;
+    most = fmaxf(most, fabsf(f));
+  }
+  int up = 0;
+  if constexpr (__is_same(T, f16_t)) {
+    most = fmaxf(most, __shfl_xor(most, 1));
+    most = fmaxf(most, __shfl_xor(most, 2));
+    if (most > 0.0f && most < INFINITY) up = 15 - __builtin_amdgcn_frexp_expf(most);
+    if (c % 4 == 0 && c / 4 < p.steps) p.power[row * p.steps + c / 4] = -up;
+  }
+  if (c / 4 >= p.steps) return;
+  v8 a, b;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    float f = v[e / 4][e % 4];
+    if constexpr (__is_same(T, f16_t)) f = __builtin_ldexpf(f, up);
+    a[e] = (T)f;
+    const float r = f - (float)a[e];
+    b[e] = (T)(r - r == 0.0f ? r : 0.0f);  // (of infinity and NaN nothing is left)
+  }
+  const int64_t to = ((row / 16 * p.steps + c / 4) * 4 + c % 4) * 16 + row % 16;
+  static_cast<v8*>(p.lead)[to] = a, static_cast<v8*>(p.rest)[to] = b;
+}
+
+// Columns of x that a wave takes at once: a row's are a line of 128 bytes.
+constexpr int kLine = 64;
+
 // h of 16 NT rows and 16 RT ranks over a part of the columns, which W waves share.
+// A wave loads whole lines, 8 lanes each (operands straight from memory would be 64
+// accesses of 16 bytes: 2047 x 9728 of rank 64 30 us), and turns them into operands
+// in LDS of its own: piece c of row r lies at c ^ (r & 7), so that 16 rows' pieces
+// are on distinct banks.
 template <typename T, int NT, int RT, int W>
 __global__ void __launch_bounds__(64 * W) lora_shrink_kernel(const LoraArgs p) {
   typedef typename LoraMma<T>::v8 v8;
-  constexpr int ROWS = 16 * NT, U = 4;  // steps whose loads are in flight together
-  __shared__ f32x4 sums[W][ROWS][4 * RT];
+  constexpr int ROWS = 16 * NT, LINES = 16 * (NT + RT);  // lines: of x's rows, then of A's
+  constexpr int kSums = ROWS * (4 * RT + 1);             // (a piece more a row: 16 rows' pieces on distinct banks)
+  constexpr int kWave = kSums > LINES * 8 ? kSums : LINES * 8;
+  constexpr int PIECES = RT < 2 ? 4 : 2 * RT;  // of 8 ranks that a row leaves
+  static_assert(ROWS * PIECES <= 64 * W, "a thread has one piece at most");
+  __shared__ f32x4 lds[W][kWave];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lr = lane & 15, lg = lane >> 4;
   const int64_t row0 = (int64_t)blockIdx.x * ROWS;
   const int slot = blockIdx.z % p.slots, rank0 = blockIdx.z / p.slots * 16 * RT;
   const int id = lane < ROWS && row0 + lane < p.rows ? p.adapters[row0 + lane] : -1;
-  const int from = (int)((int64_t)p.steps * blockIdx.y / p.parts), to = (int)((int64_t)p.steps * (blockIdx.y + 1) / p.parts);
+  const int from = (int)((int64_t)p.lines * blockIdx.y / p.parts), to = (int)((int64_t)p.lines * (blockIdx.y + 1) / p.parts);
   const int s0 = from + (to - from) * wave / W, s1 = from + (to - from) * (wave + 1) / W;
-  const T* x[NT];
-#pragma unroll
-  for (int t = 0; t < NT; ++t) x[t] = static_cast<const T*>(p.x) + min(row0 + 16 * t + lr, p.rows - 1) * p.ldx + 8 * lg;
+  const int whole = min(s1, p.k / kLine);  // lines of 64 columns up to here
+  const int at = lane >> 3, piece = lane & 7;  // of what the lane loads
+  v8* staged = reinterpret_cast<v8*>(lds[wave]);
+  const int own_row = threadIdx.x / PIECES, own_piece = threadIdx.x % PIECES;  // of h
+  const int own_id = __shfl(id, own_row < ROWS ? own_row : 0);
+  const T* x = static_cast<const T*>(p.x) + row0 * p.ldx;
 
   each_adapter(id, __ballot(id >= 0 && id < p.count), slot, p.slots, [&](int who, uint64_t same) __attribute__((always_inline)) {
-    const T* a[RT];
-#pragma unroll
-    for (int r = 0; r < RT; ++r)
-      a[r] = static_cast<const T*>(p.a) + who * p.a_adapter + min(rank0 + 16 * r + lr, p.rank - 1) * p.a_row + 8 * lg;
+    const T* a = static_cast<const T*>(p.a) + who * p.a_adapter + rank0 * p.a_row;
+    // the lane's eight columns of line 8 i + at (rows are at most 2^24 apart: 32 bits)
+    auto line = [&](int i, int s) __attribute__((always_inline)) {
+      const int l = 8 * i + at;
+      const int to = i < 2 * NT ? l * (int)p.ldx : min(l - ROWS, p.rank - 1 - rank0) * (int)p.a_row;
+      return (i < 2 * NT ? x : a) + kLine * s + (to + 8 * piece);
+    };
+    // (rows of other adapters are not read: what lies in LDS there is not kept)
+    auto wanted = [&](int i) __attribute__((always_inline)) { return i >= 2 * NT || (same >> (8 * i + at) & 1); };
     f32x4 acc[NT][RT];
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
       for (int r = 0; r < RT; ++r) acc[t][r] = f32x4{0, 0, 0, 0};
-    for (int s = s0; s < s1; s += U) {
-      v8 xv[U][NT], av[U][RT];
+    auto multiply = [&]() __attribute__((always_inline)) {
+      wave_lds_fence();
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int c = 32 * (s + u);
-        if (s + u < s1 && c + 32 <= p.k) {
+      for (int u = 0; u < 2; ++u) {
+        v8 xv[NT];
 #pragma unroll
-          for (int t = 0; t < NT; ++t) __builtin_memcpy(&xv[u][t], x[t] + c, 16);
+        for (int t = 0; t < NT; ++t) xv[t] = staged[(16 * t + lr) * 8 + ((4 * u + lg) ^ (lr & 7))];
 #pragma unroll
-          for (int r = 0; r < RT; ++r) __builtin_memcpy(&av[u][r], a[r] + c, 16);
-        } else {
-          const int left = s + u < s1 ? p.k - c - 8 * lg : 0;
+        for (int r = 0; r < RT; ++r) {
+          const v8 w = staged[(ROWS + 16 * r + lr) * 8 + ((4 * u + lg) ^ (lr & 7))];
 #pragma unroll
-          for (int t = 0; t < NT; ++t) xv[u][t] = load_upto<v8>(x[t] + c, left);
-#pragma unroll
-          for (int r = 0; r < RT; ++r) av[u][r] = load_upto<v8>(a[r] + c, left);
+          for (int t = 0; t < NT; ++t) acc[t][r] = LoraMma<T>::mul(w, xv[t], acc[t][r]);
         }
       }
+      wave_lds_fence();
+    };
+    v8 v[2 * (NT + RT)];
+    auto load = [&](int s) __attribute__((always_inline)) {
 #pragma unroll
-      for (int u = 0; u < U; ++u)
+      for (int i = 0; i < 2 * (NT + RT); ++i)
+        if (wanted(i)) v[i] = load_eight<v8>(line(i, s));
+    };
+    if (s0 < whole) load(s0);
+    for (int s = s0; s < whole; ++s) {
 #pragma unroll
-        for (int t = 0; t < NT; ++t)
-#pragma unroll
-          for (int r = 0; r < RT; ++r) acc[t][r] = LoraMma<T>::mul(av[u][r], xv[u][t], acc[t][r]);
+      for (int i = 0; i < 2 * (NT + RT); ++i) staged[(8 * i + at) * 8 + (piece ^ at)] = v[i];
+      if (s + 1 < whole) load(s + 1);
+      multiply();
+    }
+    if (whole < s1) {  // the row's end
+#pragma unroll 1
+      for (int i = 0; i < 2 * (NT + RT); ++i)
+        if (wanted(i))
+          staged[(8 * i + at) * 8 + (piece ^ at)] = load_upto<v8>(line(i, whole), p.k - kLine * whole - 8 * piece);
+      multiply();
     }
     // lane: row 16 t + lr, ranks 16 r + 4 lg .. + 3
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
-      for (int r = 0; r < RT; ++r) sums[wave][16 * t + lr][4 * r + lg] = acc[t][r];
+      for (int r = 0; r < RT; ++r) lds[wave][(16 * t + lr) * (4 * RT + 1) + 4 * r + lg] = acc[t][r];
     __syncthreads();
-    for (int i = threadIdx.x; i < ROWS * 4 * RT; i += 64 * W) {
-      const int row = i / (4 * RT), c = i - row * (4 * RT);
-      if (same >> row & 1) {
-        f32x4 sum = sums[0][row][c];
+    if (own_row < ROWS && same >> own_row & 1) {
+      f32x4 sum[2] = {f32x4{0, 0, 0, 0}, f32x4{0, 0, 0, 0}};
+      if (own_piece < 2 * RT) {
 #pragma unroll
-        for (int w = 1; w < W; ++w) sum += sums[w][row][c];
-        *reinterpret_cast<f32x4*>(p.h + (blockIdx.y * p.rows + row0 + row) * p.hr + rank0 + 4 * c) = sum;
+        for (int c = 0; c < 2; ++c) {
+          sum[c] = lds[0][own_row * (4 * RT + 1) + 2 * own_piece + c];
+#pragma unroll
+          for (int w = 1; w < W; ++w) sum[c] += lds[w][own_row * (4 * RT + 1) + 2 * own_piece + c];
+        }
+      }
+      if (p.parts == 1) {
+        leave_h<T>(p, row0 + own_row, rank0 / 8 + own_piece, sum, p.scales ? p.scales[own_id] : 1.0f);
+      } else if (own_piece < 2 * RT) {
+        f32x4* q = reinterpret_cast<f32x4*>(p.parts_h + (blockIdx.y * p.rows + row0 + own_row) * p.hr + rank0 + 8 * own_piece);
+        q[0] = sum[0], q[1] = sum[1];
       }
     }
     __syncthreads();
   });
 }
 
-// The outputs of 16 NT rows and 256 columns.  LDS: h as two operands [step of 32
-// ranks][16 rows][lane], then each row's power of two.
-template <typename T, int NT>
+// The parts' sums, added in order: a thread per row and 8 ranks.
+template <typename T>
+__global__ void __launch_bounds__(256) lora_join_kernel(const LoraArgs p) {
+  const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x, row = at / (4 * p.steps);
+  const int c = (int)(at - row * (4 * p.steps));
+  if (row >= p.rows) return;
+  const int who = p.adapters[row];
+  if (who < 0 || who >= p.count) return;
+  f32x4 sum[2] = {f32x4{0, 0, 0, 0}, f32x4{0, 0, 0, 0}};
+  // (h has room for whole pieces of 16 ranks: past those nothing is read)
+  const float* h = p.parts_h + row * p.hr + 8 * min(c, (p.rank - 1) / 8);
+  for (int part = 0; part < p.parts; part += 4) {
+    f32x4 q[4][2];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const f32x4* from = reinterpret_cast<const f32x4*>(h + min(part + u, p.parts - 1) * p.rows * p.hr);
+      q[u][0] = from[0], q[u][1] = from[1];
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if (part + u < p.parts) sum[0] += q[u][0], sum[1] += q[u][1];
+  }
+  leave_h<T>(p, row, c, sum, p.scales ? p.scales[who] : 1.0f);
+}
+
+// The outputs of 16 NT rows and 256 columns.  PLAIN: a rank that is a
+// multiple of 8 and 64 columns and more, of which the last wave takes the last 64.
+// Loads that need no other's result are issued together: the ids, then y, h and the
+// first weights; the next step's while one is multiplied.
+template <typename T, int NT, bool PLAIN>
 __global__ void __launch_bounds__(256) lora_expand_kernel(const LoraArgs p) {
   typedef typename LoraMma<T>::v8 v8;
   constexpr int ROWS = 16 * NT;
-  extern __shared__ __attribute__((aligned(16))) char lds[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lr = lane & 15, lg = lane >> 4;
   const int64_t row0 = (int64_t)blockIdx.x * ROWS;
-  const int slot = blockIdx.z, steps = (p.rank + 31) / 32;
-  v8* lead = reinterpret_cast<v8*>(lds);
-  v8* rest = lead + steps * NT * 64;
-  int* power = reinterpret_cast<int*>(rest + steps * NT * 64);
-  const int id = lane < ROWS && row0 + lane < p.rows ? p.adapters[row0 + lane] : -1;
-  const uint64_t valid = __ballot(id >= 0 && id < p.count);
-  const uint64_t here = __ballot(lane < ROWS && row0 + lane < p.rows);
-  // this workgroup's rows
-  uint64_t mine = 0;
-  each_adapter(id, valid, slot, p.slots, [&](int, uint64_t same) __attribute__((always_inline)) { mine |= same; });
-  const uint64_t plain = slot == 0 ? here & ~valid : 0;  // rows without an adapter
-  if (!(mine | plain)) return;
-
-  // their h, 8 threads a row, 8 ranks at a time
-  for (int row = threadIdx.x / 8; row < ROWS; row += 32) {
-    if (!(mine >> row & 1)) continue;
-    const int l8 = threadIdx.x & 7;
-    const int who = p.adapters[row0 + row];
-    const float scale = p.scales ? p.scales[who] : 1.0f;
-    const float* h = p.h + (row0 + row) * p.hr;
-    float most = 0.0f;
-    for (int pass = 0; pass < 2; ++pass) {  // (fp16: its largest first)
-      int up = 0;
-      if constexpr (__is_same(T, f16_t)) {
-        if (pass == 1) {
-#pragma unroll
-          for (int o = 1; o < 8; o *= 2) most = fmaxf(most, __shfl_xor(most, o));
-          if (most > 0.0f && most < INFINITY) up = 15 - __builtin_amdgcn_frexp_expf(most);
-          if (l8 == 0) power[row] = -up;
-        }
-      } else if (pass == 0) {
-        continue;
-      }
-      for (int c = l8; c < 4 * steps; c += 8) {
-        f32x4 v[2] = {f32x4{0, 0, 0, 0}, f32x4{0, 0, 0, 0}};
-        if (8 * c < p.rank) {
-          for (int part = 0; part < p.parts; ++part) {
-            const f32x4* q = reinterpret_cast<const f32x4*>(h + part * p.rows * p.hr + 8 * c);
-            v[0] += q[0];
-            v[1] += q[1];
-          }
-        }
-        v8 a, b;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          float f = 8 * c + e < p.rank ? v[e / 4][e % 4] * scale : 0.0f;
-          if constexpr (__is_same(T, f16_t)) {
-            if (pass == 0) most = fmaxf(most, fabsf(f));
-            f = __builtin_ldexpf(f, up);
-          }
-          a[e] = (T)f;
-          const float r = f - (float)a[e];
-          b[e] = (T)(r - r == 0.0f ? r : 0.0f);  // (of infinity and NaN nothing is left)
-        }
-        if (pass == 1) {
-          const int at = ((c / 4 * NT + row / 16) * 4 + c % 4) * 16 + row % 16;
-          lead[at] = a, rest[at] = b;
-        }
-      }
-    }
-  }
-  __syncthreads();
-
+  const int slot = blockIdx.z;
   // A lane has 16 columns of a row: tile t's row 4 g + e of the matrix instruction
   // is column 16 g + 4 t + e.
-  const int column0 = blockIdx.y * 256 + wave * 64, column = column0 + 16 * lg;
-  if (column0 >= p.n) return;
-  auto put = [&](int t, uint64_t rows, const f32x4 (&acc)[4], int up) __attribute__((always_inline)) {
-    const int row = 16 * t + lr;
-    if (!(rows >> row & 1)) return;
-    const T* y = static_cast<const T*>(p.y) + (row0 + row) * p.ldy + column;
-    T* out = static_cast<T*>(p.out) + (row0 + row) * p.n + column;
-    struct {
-      T v[16];
-    } r;
-    if (column + 16 <= p.n) {
-      __builtin_memcpy(&r, y, sizeof(r));
+  if (blockIdx.y * 256 + wave * 64 >= (uint32_t)p.n) return;
+  const int column0 = PLAIN ? min((int)blockIdx.y * 256 + wave * 64, p.n - 64) : (int)blockIdx.y * 256 + wave * 64;
+  const int column = column0 + 16 * lg;
+  const int id = lane < ROWS && row0 + lane < p.rows ? p.adapters[row0 + lane] : -1;
+  const uint64_t valid = __ballot(id >= 0 && id < p.count);
+  // this workgroup's rows
+  uint64_t mine = slot == 0 ? __ballot(lane < ROWS && row0 + lane < p.rows) & ~valid : 0;  // rows without an adapter
+  const uint64_t plain = mine;
+  each_adapter(id, valid, slot, p.slots, [&](int, uint64_t same) __attribute__((always_inline)) { mine |= same; });
+  if (!mine) return;
+
+  struct Sixteen {
+    T v[16];
+  } y[NT];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    const T* at = static_cast<const T*>(p.y) + min(row0 + 16 * t + lr, p.rows - 1) * p.ldy;
+    if (!(mine >> (16 * t + lr) & 1)) {  // (another slot's)
+    } else if (PLAIN || column0 + 64 <= p.n) {
+      __builtin_memcpy(&y[t], at + column, sizeof(Sixteen));
     } else {
 #pragma unroll
-      for (int e = 0; e < 16; ++e) r.v[e] = column + e < p.n ? y[e] : (T)0.0f;
+      for (int e = 0; e < 16; ++e) y[t].v[e] = at[min(column + e, p.n - 1)];
     }
+  }
+  auto put = [&](int t, uint64_t rows, const f32x4 (&sum)[4]) __attribute__((always_inline)) {
+    const int row = 16 * t + lr;
+    if (!(rows >> row & 1)) return;
+    T* out = static_cast<T*>(p.out) + (row0 + row) * p.n + column;
+    // (opaque: else y is waited for and turned into floats before the products)
+    u32x4 raw[2];
+    __builtin_memcpy(raw, &y[t], sizeof(raw));
+    asm volatile("" : "+v"(raw[0]), "+v"(raw[1]));
+    Sixteen r;
+    __builtin_memcpy(&r, raw, sizeof(r));
 #pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      float f = acc[e / 4][e % 4];
-      if constexpr (__is_same(T, f16_t)) f = __builtin_ldexpf(f, up);
-      r.v[e] = (T)((float)r.v[e] + f);
-    }
-    if (column + 16 <= p.n) {
+    for (int e = 0; e < 16; ++e) r.v[e] = (T)((float)r.v[e] + sum[e / 4][e % 4]);
+    if (PLAIN || column0 + 64 <= p.n) {
       __builtin_memcpy(out, &r, sizeof(r));
     } else {
 #pragma unroll
@@ -257,42 +316,73 @@ __global__ void __launch_bounds__(256) lora_expand_kernel(const LoraArgs p) {
         if (column + e < p.n) out[e] = r.v[e];
     }
   };
+  const v8* lead = static_cast<const v8*>(p.lead) + row0 / 16 * p.steps * 64 + lane;
+  const v8* rest = static_cast<const v8*>(p.rest) + row0 / 16 * p.steps * 64 + lane;
   each_adapter(id, valid, slot, p.slots, [&](int who, uint64_t same) __attribute__((always_inline)) {
     const T* b[4];
 #pragma unroll
-    for (int t = 0; t < 4; ++t)
-      b[t] = static_cast<const T*>(p.b) + who * p.b_adapter + min(column0 + 16 * (lr >> 2) + 4 * t + (lr & 3), p.n - 1) * p.b_row + 8 * lg;
-    f32x4 acc[NT][4];
+    for (int c = 0; c < 4; ++c)
+      b[c] = static_cast<const T*>(p.b) + who * p.b_adapter + min(column0 + 16 * (lr >> 2) + 4 * c + (lr & 3), p.n - 1) * p.b_row + 8 * lg;
+    v8 w[4], h0[NT], h1[NT];
+    int power[NT];  // of the step
+    auto load = [&](int s) __attribute__((always_inline)) {
+      const int left = p.rank - 32 * s - 8 * lg;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        if constexpr (PLAIN) w[c] = left > 0 ? load_eight<v8>(b[c] + 32 * s) : v8{};
+        else w[c] = load_upto<v8>(b[c] + 32 * s, left);
+      }
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        // (past the last rows there are no operands)
+        const int64_t at = (int64_t)min(t, (int)((p.rows - 1 - row0) / 16)) * p.steps * 64 + s * 64;
+        h0[t] = lead[at], h1[t] = rest[at];
+        if constexpr (__is_same(T, f16_t)) power[t] = p.power[min(row0 + 16 * t + lr, p.rows - 1) * p.steps + s];
+      }
+    };
+    f32x4 sum[NT][4];
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
-      for (int c = 0; c < 4; ++c) acc[t][c] = f32x4{0, 0, 0, 0};
-    for (int s = 0; s < steps; ++s) {
-      v8 w[4];
+      for (int c = 0; c < 4; ++c) sum[t][c] = f32x4{0, 0, 0, 0};
+    load(0);
+#pragma unroll 1
+    for (int s = 0; s < p.steps; ++s) {
+      v8 w_[4], h0_[NT], h1_[NT];
+      int power_[NT];
 #pragma unroll
-      for (int c = 0; c < 4; ++c) w[c] = load_upto<v8>(b[c] + 32 * s, p.rank - 32 * s - 8 * lg);
+      for (int c = 0; c < 4; ++c) w_[c] = w[c];
 #pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        const v8 h0 = lead[(s * NT + t) * 64 + lane], h1 = rest[(s * NT + t) * 64 + lane];
+      for (int t = 0; t < NT; ++t) h0_[t] = h0[t], h1_[t] = h1[t], power_[t] = power[t];
+      if (s + 1 < p.steps) load(s + 1);
+      f32x4 acc[NT][4];  // (of a step: each has a power of two of its own)
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          acc[t][c] = LoraMma<T>::mul(w[c], h0, acc[t][c]);
-          acc[t][c] = LoraMma<T>::mul(w[c], h1, acc[t][c]);
+          acc[t][c] = LoraMma<T>::mul(w_[c], h0_[t], f32x4{0, 0, 0, 0});
+          acc[t][c] = LoraMma<T>::mul(w_[c], h1_[t], acc[t][c]);
         }
-      }
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) sum[t][c][e] += __is_same(T, f16_t) ? __builtin_ldexpf(acc[t][c][e], power_[t]) : acc[t][c][e];
     }
 #pragma unroll
-    for (int t = 0; t < NT; ++t) put(t, same, acc[t], __is_same(T, f16_t) ? power[16 * t + lr] : 0);
+    for (int t = 0; t < NT; ++t) put(t, same, sum[t]);
   });
-  const f32x4 zero[4] = {f32x4{0, 0, 0, 0}, f32x4{0, 0, 0, 0}, f32x4{0, 0, 0, 0}, f32x4{0, 0, 0, 0}};
   if (plain) {
+    const f32x4 zero[4] = {f32x4{0, 0, 0, 0}, f32x4{0, 0, 0, 0}, f32x4{0, 0, 0, 0}, f32x4{0, 0, 0, 0}};
 #pragma unroll
-    for (int t = 0; t < NT; ++t) put(t, plain, zero, 0);
+    for (int t = 0; t < NT; ++t) put(t, plain, zero);
   }
 }
 
 struct LoraPlan {
-  int tiles, parts, slots, hr, steps;  // tiles: of 16 rows of a workgroup
+  int tiles, parts, slots, hr, lines, steps;  // tiles: of 16 rows of a workgroup
+  int64_t parts_bytes, operand_bytes, power_bytes;
 };
 
 inline LoraPlan lora_plan(int64_t rows, int64_t k, int64_t rank) {
@@ -300,11 +390,19 @@ inline LoraPlan lora_plan(int64_t rows, int64_t k, int64_t rank) {
   q.tiles = rows > 256 ? 4 : 1;
   q.slots = q.tiles == 1 ? 16 : 1;
   q.hr = (int)(rank + 63) / 64 * 64;
-  q.steps = (int)(k + 31) / 32;
-  const int64_t groups = (rows + 16 * q.tiles - 1) / (16 * q.tiles), waves = q.tiles == 1 ? 4 : 8;
-  int64_t parts = (q.steps + 5 * waves - 1) / (5 * waves);
-  if (q.tiles > 1) parts = std::min(parts, std::max((int64_t)1, (256 + groups - 1) / groups));
+  q.lines = (int)((k + kLine - 1) / kLine);
+  q.steps = (int)(rank + 31) / 32;
+  int64_t parts;
+  if (q.tiles == 1) {
+    parts = (q.lines + 95) / 96;
+  } else {
+    const int64_t groups = (rows + 63) / 64;
+    parts = std::min((int64_t)(q.lines + 15) / 16, (256 + groups - 1) / groups);
+  }
   q.parts = (int)std::min(parts, (int64_t)16);
+  q.parts_bytes = q.parts > 1 ? rows * q.parts * q.hr * 4 : 0;
+  q.operand_bytes = (rows + 15) / 16 * q.steps * 1024;
+  q.power_bytes = (rows * q.steps * 4 + 15) / 16 * 16;
   return q;
 }
 
@@ -314,23 +412,24 @@ void launch_shrink(const LoraArgs& p, hipStream_t s) {
   hipLaunchKernelGGL((lora_shrink_kernel<T, NT, RT, W>), grid, dim3(64 * W), 0, s, p);
 }
 
-template <typename T, int NT, int W>
+template <typename T, int NT, int W, int NE>
 int launch_lora(const LoraArgs& p, hipStream_t s) {
   if (p.count > 0) {
     if (p.rank <= 16) launch_shrink<T, NT, 1, W>(p, s);
-    else if (p.rank <= 32) launch_shrink<T, NT, 2, W>(p, s);
-    else launch_shrink<T, NT, 4, W>(p, s);
+    else if (NT == 1 || p.rank <= 32) launch_shrink<T, NT, 2, W>(p, s);
+    else if constexpr (NT > 1) launch_shrink<T, NT, 4, W>(p, s);
+    if (p.parts > 1)
+      hipLaunchKernelGGL((lora_join_kernel<T>), dim3((uint32_t)((p.rows * 4 * p.steps + 255) / 256)), dim3(256), 0, s, p);
   }
-  const int steps = (p.rank + 31) / 32, bytes = steps * NT * 2048 + NT * 64;
-  allow_dynamic_lds(reinterpret_cast<const void*>(lora_expand_kernel<T, NT>), 0);
-  const dim3 grid((uint32_t)((p.rows + 16 * NT - 1) / (16 * NT)), (p.n + 255) / 256, p.slots);
-  hipLaunchKernelGGL((lora_expand_kernel<T, NT>), grid, dim3(256), bytes, s, p);
+  const dim3 grid((uint32_t)((p.rows + 16 * NE - 1) / (16 * NE)), (p.n + 255) / 256, p.slots);
+  if (p.rank % 8 == 0 && p.n >= 64) hipLaunchKernelGGL((lora_expand_kernel<T, NE, true>), grid, dim3(256), 0, s, p);
+  else hipLaunchKernelGGL((lora_expand_kernel<T, NE, false>), grid, dim3(256), 0, s, p);
   return launch_status();
 }
 
 inline bool lora_sizes_ok(int64_t rows, int64_t k, int64_t n, int64_t rank, int64_t count) {
   return rows >= 0 && rows <= (1 << 24) && k >= 1 && k <= (1 << 20) && n >= 1 && n <= (1 << 20) && rank >= 1 && rank <= 256 &&
-         count >= 0 && count <= (1 << 20) && grid_fits((rows + 63) / 64 * ((n + 255) / 256), 256);
+         count >= 0 && count <= (1 << 20) && grid_fits((rows + 31) / 32 * ((n + 255) / 256), 256);
 }
 
 }  // namespace tp
@@ -340,7 +439,7 @@ using namespace tp;
 extern "C" int64_t tp_lora_workspace_bytes(int64_t rows, int64_t k, int64_t n, int64_t rank, int64_t count) {
   if (!lora_sizes_ok(rows, k, n, rank, count)) return -1;
   const LoraPlan q = lora_plan(rows, k, rank);
-  return count ? rows * q.parts * q.hr * (int64_t)sizeof(float) : 0;
+  return count ? q.parts_bytes + 2 * q.operand_bytes + q.power_bytes : 0;
 }
 
 extern "C" int tp_lora_add(int dtype, int64_t rows, int64_t k, int64_t n, int64_t rank, int64_t count, const void* x,
@@ -349,7 +448,7 @@ extern "C" int tp_lora_add(int dtype, int64_t rows, int64_t k, int64_t n, int64_
                            const void* y, int64_t ldy, void* out, void* workspace, int64_t workspace_bytes,
                            void* stream) {
   if (dtype != TP_F16 && dtype != TP_BF16) return TP_ERR_BAD_TYPE;
-  if (!lora_sizes_ok(rows, k, n, rank, count) || ldx < 0 || ldy < 0) return TP_ERR_BAD_DIMS;
+  if (!lora_sizes_ok(rows, k, n, rank, count) || ldx < 0 || ldx > (1 << 24) || a_row < 0 || a_row > (1 << 24) || ldy < 0) return TP_ERR_BAD_DIMS;
   if (rows == 0) return TP_OK;
   if (!x || !y || !out || !adapters || (count && (!a || !b))) return TP_ERR_NULL_POINTER;
   if ((((uintptr_t)x | (uintptr_t)a | (uintptr_t)b | (uintptr_t)y | (uintptr_t)out) & 1) || (((uintptr_t)adapters | (uintptr_t)scales) & 3))
@@ -359,11 +458,16 @@ extern "C" int tp_lora_add(int dtype, int64_t rows, int64_t k, int64_t n, int64_
   if ((uintptr_t)workspace & 15) return TP_ERR_MISALIGNED;
   const LoraPlan q = lora_plan(rows, k, rank);
   LoraArgs p{};
-  p.x = x, p.a = a, p.b = b, p.y = y, p.out = out, p.adapters = adapters, p.scales = scales, p.h = static_cast<float*>(workspace);
+  p.x = x, p.a = a, p.b = b, p.y = y, p.out = out, p.adapters = adapters, p.scales = scales;
+  char* ws = static_cast<char*>(workspace);
+  if (need) {
+    p.parts_h = reinterpret_cast<float*>(ws), p.lead = ws + q.parts_bytes, p.rest = ws + q.parts_bytes + q.operand_bytes;
+    p.power = reinterpret_cast<int*>(ws + q.parts_bytes + 2 * q.operand_bytes);
+  }
   p.ldx = ldx, p.ldy = ldy, p.a_adapter = a_adapter, p.a_row = a_row, p.b_adapter = b_adapter, p.b_row = b_row;
   p.rows = rows, p.k = (int)k, p.n = (int)n, p.rank = (int)rank, p.count = (int)count;
-  p.parts = q.parts, p.slots = q.slots, p.hr = q.hr, p.steps = q.steps;
+  p.parts = q.parts, p.slots = q.slots, p.hr = q.hr, p.lines = q.lines, p.steps = q.steps;
   hipStream_t s = (hipStream_t)stream;
-  if (q.tiles == 1) return dtype == TP_F16 ? launch_lora<f16_t, 1, 4>(p, s) : launch_lora<bf16_t, 1, 4>(p, s);
-  return dtype == TP_F16 ? launch_lora<f16_t, 4, 8>(p, s) : launch_lora<bf16_t, 4, 8>(p, s);
+  if (q.tiles == 1) return dtype == TP_F16 ? launch_lora<f16_t, 1, 8, 1>(p, s) : launch_lora<bf16_t, 1, 8, 1>(p, s);
+  return dtype == TP_F16 ? launch_lora<f16_t, 4, 8, 2>(p, s) : launch_lora<bf16_t, 4, 8, 2>(p, s);
 }

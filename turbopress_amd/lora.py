@@ -5,16 +5,26 @@ adds the product of its own request's adapter.  Inference only.
 
 from __future__ import annotations
 
+import functools
+
 import torch
 from torch import Tensor
 
 from turbopress_amd import _lib
 from turbopress_amd.hip_kernel import raw_stream as _raw_stream
 from turbopress_amd.norm import DTYPE_CODES
+from turbopress_amd.paged import _workspace
 
 __all__ = ["lora_add", "MAX_RANK"]
 
 MAX_RANK = 256
+_FAR = 1 << 24  # elements that rows may lie apart without a copy
+
+
+@functools.lru_cache(maxsize=1024)
+def _needs(rows: int, k: int, n: int, rank: int, count: int) -> int:
+    """Workspace bytes of a call."""
+    return _lib.lib().tp_lora_workspace_bytes(rows, k, n, rank, count)
 
 
 def _refuse(y, x, a, b, adapters, scales) -> None:
@@ -42,13 +52,13 @@ def _refuse(y, x, a, b, adapters, scales) -> None:
 
 def _flat(t: Tensor, width: int) -> tuple:
     """(tensor, elements from a row to the next) of [..., width] as rows."""
-    if t.dim() == 2 and (t.stride(1) == 1 or width == 1) and t.stride(0) >= 0:
+    if t.dim() == 2 and (t.stride(1) == 1 or width == 1) and t.stride(0) <= _FAR:
         return t, t.stride(0)
     return (t if t.is_contiguous() else t.contiguous()), width
 
 
 def _weights(w: Tensor) -> Tensor:
-    return w if w.stride(2) == 1 or w.shape[2] == 1 else w.contiguous()
+    return w if (w.stride(2) == 1 or w.shape[2] == 1) and w.stride(1) <= _FAR else w.contiguous()
 
 
 def lora_add(y: Tensor, x: Tensor, a: Tensor, b: Tensor, adapters: Tensor, scales: Tensor | None = None) -> Tensor:
@@ -78,14 +88,14 @@ def lora_add(y: Tensor, x: Tensor, a: Tensor, b: Tensor, adapters: Tensor, scale
         adapters = adapters.contiguous()
     if scales is not None and not scales.is_contiguous():
         scales = scales.contiguous()
-    lib = _lib.lib()
-    need = lib.tp_lora_workspace_bytes(rows, k, n, rank, count)
-    ws = torch.empty(max(need, 16), dtype=torch.uint8, device=out.device)
+    stream = _raw_stream(index)
+    need = _needs(rows, k, n, rank, count)
+    ws, _, _held = _workspace(index, stream, max(need, 16), 0)
     a_adapter, a_row, _ = a.stride()
     b_adapter, b_row, _ = b.stride()
-    st = lib.tp_lora_add(code, rows, k, n, rank, count, x.data_ptr(), ldx, a.data_ptr(), a_adapter, a_row, b.data_ptr(), b_adapter,
+    st = _lib.lib().tp_lora_add(code, rows, k, n, rank, count, x.data_ptr(), ldx, a.data_ptr(), a_adapter, a_row, b.data_ptr(), b_adapter,
                          b_row, adapters.data_ptr(), 0 if scales is None else scales.data_ptr(), y.data_ptr(), ldy,
-                         out.data_ptr(), ws.data_ptr(), need, _raw_stream(index))
+                         out.data_ptr(), ws, need, stream)
     if st:
         _lib.check(st, "lora_add")
     return out
