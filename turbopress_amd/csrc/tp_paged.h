@@ -1,4 +1,5 @@
-// Attention of one new token per sequence over a paged cache.  With the running
+// Attention of one new token per sequence over a paged cache, or of a tree of up
+// to 64 that are drafted (TREE).  With the running
 // maximum m and sum l of a softmax, a block of tokens takes a state (m, l, o) to
 //
 //   m' = max(m, max_t s_t),  l' = l e^(m - m') + sum_t e^(s_t - m'),
@@ -25,6 +26,17 @@
 // the probabilities from the registers where S^T left them, and V through a
 // wave's own piece of LDS, read transposed.  Loads of the next 32 tokens are in
 // flight meanwhile.
+//
+// TREE: new token j of a sequence is token length + j of its cache, and sees those
+// before the length and, of the new ones, the bits of its mask.  A row is a (new
+// token, query head) of the cache head, up to 64 rows share what a workgroup reads,
+// and which of them see a token is asked only in the tiles where they differ.  4
+// flops for each element and row: at 64 rows the exponentials, products and the
+// waits between them bound it, not HBM (16 new tokens, 32 query heads on 8 of 128
+// columns: 131072 tokens 135 + 8 us of the join = 3.8 TB/s; 13 of 32 sequences of 0 to
+// 8191 152 + 10; 64 new tokens of 16 sequences of 4096, 4 groups of rows 263 + 9).
+// Up to 16 rows are a wave's as above, 32 or 64 two waves' on each piece of tokens:
+// one loads keys, the other values, for both.
 #pragma once
 
 #include "tp_ops_common.h"
@@ -52,9 +64,9 @@ constexpr int kRowTile = 16;  // query rows: columns of a matrix instruction
 // More only add starts and joins: 64 x 8192 tokens, 8 heads of 128, 4 waves, 1 / 2
 // / 3 workgroups per CU 354 / 392 / 362 us, 1 x 131072 104 / 117 / 117; 8 waves
 // 357 and 107, and 12.3 us for 1 x 577 against 9.7 (fewer, longer units).
-template <int DP, int RT>
+template <int DP, int H>
 __host__ __device__ constexpr int paged_waves() {
-  return DP <= 64 && RT < 4 ? 8 : 4;
+  return DP <= 64 && H == 1 ? 8 : 4;
 }
 
 struct PagedArgs {
@@ -74,10 +86,11 @@ struct PagedArgs {
 __device__ const uint4 kZeros[32] = {};
 
 // A 16-byte load from global memory (said so: of a pointer chosen from two, the
-// compiler would make a flat load, whose wait covers LDS too).
-template <typename V>
+// compiler would make a flat load, whose wait covers LDS too).  ONCE: past the caches.
+template <bool ONCE, typename V>
 __device__ __forceinline__ V load16(const void* p) {
-  return __builtin_nontemporal_load((const __attribute__((address_space(1))) V*)p);
+  const auto at = (const __attribute__((address_space(1))) V*)p;
+  return ONCE ? __builtin_nontemporal_load(at) : *at;
 }
 
 // kUnit: of the probabilities, the sums and the outputs of a state (a power of
@@ -91,6 +104,9 @@ __device__ __forceinline__ V load16(const void* p) {
 // second products run under the loads (64 x 8192 tokens 351 us with and without,
 // 1 x 577 9.1 and 9.2).  What a probability above 0 leaves is not 0 (a unit that
 // the sum does not feel): 0 times a value that is infinite would be NaN.
+//
+// cut_above: the same where the leading bits are those of a little less, so that
+// what they leave is above 0 by itself (2^-16 or 2^-21 of it are lost).
 template <typename T>
 struct Mma;
 template <>
@@ -103,6 +119,11 @@ struct Mma<f16_t> {
     p[e] = (f16_t)lead[0], p[e + 1] = (f16_t)lead[1];
     rest[e] = (f16_t)fmaxf(x - (float)lead[0], fminf(x, 0x1p-24f));
     rest[e + 1] = (f16_t)fmaxf(y - (float)lead[1], fminf(y, 0x1p-24f));
+  }
+  __device__ __forceinline__ static void cut_above(float x, float y, v8& p, v8& rest, int e) {
+    const auto lead = __builtin_amdgcn_cvt_pkrtz(x * (1.0f - 0x1p-11f), y * (1.0f - 0x1p-11f));
+    p[e] = (f16_t)lead[0], p[e + 1] = (f16_t)lead[1];
+    rest[e] = (f16_t)(x - (float)lead[0]), rest[e + 1] = (f16_t)(y - (float)lead[1]);
   }
   __device__ __forceinline__ static f32x4 mul(v8 a, v8 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
@@ -121,10 +142,24 @@ struct Mma<bf16_t> {
     rest[e] = (bf16_t)fmaxf(x - __builtin_bit_cast(float, xb & 0xffff0000u), fminf(x, 0x1p-100f));
     rest[e + 1] = (bf16_t)fmaxf(y - __builtin_bit_cast(float, yb & 0xffff0000u), fminf(y, 0x1p-100f));
   }
+  __device__ __forceinline__ static void cut_above(float x, float y, v8& p, v8& rest, int e) {
+    const uint32_t xb = __builtin_bit_cast(uint32_t, x * (1.0f - 0x1p-8f)), yb = __builtin_bit_cast(uint32_t, y * (1.0f - 0x1p-8f));
+    const auto both = __builtin_bit_cast(bf16x2, __builtin_amdgcn_perm(yb, xb, 0x07060302));
+    p[e] = both[0], p[e + 1] = both[1];
+    rest[e] = (bf16_t)(x - __builtin_bit_cast(float, xb & 0xffff0000u));
+    rest[e + 1] = (bf16_t)(y - __builtin_bit_cast(float, yb & 0xffff0000u));
+  }
   __device__ __forceinline__ static f32x4 mul(v8 a, v8 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
   }
 };
+
+// TREE: exponents above the largest that they are about, at most, and the unit's
+// exponent: fp16 probabilities go up to 2^15 (those down to 2^-35 of that largest
+// count).
+constexpr float kSlack = 4.0f;
+template <typename T>
+constexpr float kTreeUnit = __is_same(T, f16_t) ? 11.0f : 0.0f;
 
 // Floats of a state: per row its maximum and sum, then the (unnormalised) outputs.
 template <int DP, int RT>
@@ -143,6 +178,11 @@ struct RowSight {
   int first, unused;
 };
 
+// (13 new tokens of 32 sequences of 0 to 8191 tokens, 8 cache heads of 128: 0 / 1 / 2
+// / 3 / 4 / 6 units 247 / 194 / 173 / 165 / 155 / 156 us, of 61 such 468 / 353 / 351 /
+// 326 / 309 / 303; 32 of 4096 tokens each 139 / 135 / 136 / 137 / 137 / 137)
+constexpr int kLead = 4;
+
 // Tokens of a sequence that attention reads: [0, sinks) and [first, len).  They
 // are counted through in tiles from 0: the first `near` of the count are the
 // tokens themselves, those behind lie `shift` further on.
@@ -153,7 +193,9 @@ struct Span {
   __device__ __forceinline__ int token(int at) const { return at + (at < near ? 0 : shift); }
 };
 
-template <int UNIT, bool TREE>
+// LEAD: units without tokens that a (sequence, cache head, row group) begins with, for
+// what its beginning and end cost: a workgroup of several short ones takes fewer tokens.
+template <int UNIT, bool TREE, int LEAD>
 __device__ __forceinline__ Span span_of(const PagedArgs& a, int length) {
   Span s;
   // (room for the last unit's tokens below 2^31)
@@ -172,7 +214,7 @@ __device__ __forceinline__ Span span_of(const PagedArgs& a, int length) {
   s.near = (s.sinks + kTile - 1) & ~(kTile - 1);
   s.shift = max(base - s.near, 0);  // (sinks up to the window's own tiles: nothing lies between)
   // (an empty sequence is one unit too: its zeros have to be written)
-  s.units = max(1, (s.len - s.shift + UNIT - 1) / UNIT);
+  s.units = LEAD + max(1, (s.len - s.shift + UNIT - 1) / UNIT);
   return s;
 }
 
@@ -198,13 +240,13 @@ __device__ __forceinline__ int64_t uniform(int64_t v) {
 }
 
 // The first `states` waves' states joined: f(row, column, 4 outputs, maximum, sum) for each
-// row and 4 columns.  Wave w's outputs are floats [row][DP] at lds + w * pitch,
-// its maxima and sums ml[0][w] and ml[1][w].
-template <int DP, int W, int R, typename F>
-__device__ __forceinline__ void join_waves(int tid, int rows, int states, const float (&ml)[2][W][R],
-                                           const char* lds, int pitch, F f) {
-  for (int i = tid; i < rows * (DP / 4); i += 64 * W) {
-    const int h = i / (DP / 4), c = 4 * (i - h * (DP / 4));
+// of `rows` rows, row_of(0) and on, below `end` and 4 columns.  Wave w's outputs of the j-th
+// are DP floats at `at(w, j)`, its maxima and sums ml[0][w] and ml[1][w].
+template <int DP, int W, int R, int THREADS, typename A, typename O, typename F>
+__device__ __forceinline__ void join_waves(int tid, int rows, int end, int states, const float (&ml)[2][W][R], A at, O row_of, F f) {
+  for (int i = tid; i < rows * (DP / 4); i += THREADS) {
+    const int j = i / (DP / 4), c = 4 * (i - j * (DP / 4)), h = row_of(j);
+    if (h >= end) continue;
     float top = kLeastScore;
 #pragma unroll
     for (int w = 0; w < W; ++w)
@@ -216,7 +258,7 @@ __device__ __forceinline__ void join_waves(int tid, int rows, int states, const 
       if (w < states) {
         const float e = __builtin_amdgcn_exp2f(ml[0][w][h] - top);
         sum += e * ml[1][w][h];
-        y += e * *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(lds + w * pitch) + h * DP + c);
+        y += e * *reinterpret_cast<const f32x4*>(at(w, j) + c);
       }
     f(h, c, y, top, sum);
   }
@@ -244,42 +286,61 @@ __device__ __forceinline__ f32x2 get_device(const float* p) {
   return f32x2{__builtin_bit_cast(float, (uint32_t)v), __builtin_bit_cast(float, (uint32_t)(v >> 32))};
 }
 
-// RT tiles of 16 query rows share the keys and values that a workgroup reads.  A row
-// is a query head of the cache head; TREE: row r is new token r / group's head
-// r % group.
-template <typename T, int DP, bool EXACT, int RT, bool TREE>
-__global__ void __launch_bounds__((64 * paged_waves<DP, RT>()), 1) paged_attention_kernel(const PagedArgs a) {
-  constexpr int W = paged_waves<DP, RT>(), UNIT = W * kTile, ROWS = RT * kRowTile;
+// H RT tiles of 16 query rows share the keys and values that a workgroup reads: its H
+// sets of W waves each take the same tokens for RT tiles of their own (two waves on a
+// SIMD, one of whose matrix instructions run under the other's exponentials: 16 new
+// tokens over 131072 170 us with one wave of 64 rows).  A row is a query head of the
+// cache head; TREE: row r is new token r / group's head r % group.
+template <typename T, int DP, bool EXACT, int RT, int H, bool TREE>
+__global__ void __launch_bounds__((64 * H * paged_waves<DP, H>()), 1) paged_attention_kernel(const PagedArgs a) {
+  constexpr int W = paged_waves<DP, H>(), UNIT = W * kTile, MINE = RT * kRowTile, ROWS = H * MINE;
   typedef typename Mma<T>::v8 v8;
   typedef int16_t i16x8 __attribute__((ext_vector_type(8)));
+  constexpr int LEAD = H > 1 ? kLead : 0;
   constexpr int KS = DP / 32;        // k steps of S^T
   constexpr int DT = DP / 16;        // row tiles of O^T
   constexpr int C = DP / 8;          // 16-byte chunks of a row
   constexpr int VL = C / 2;          // V loads per lane and tile
   constexpr int kRow = 2 * DP + 32;  // LDS bytes of a V row: 16 rows' 32-byte pieces fall on distinct banks
-  // a wave's values, then its outputs
-  constexpr int kPiece = kTile * kRow > ROWS * DP * 4 ? kTile * kRow : ROWS * DP * 4;
-  __shared__ __attribute__((aligned(16))) char v_lds[W][kPiece];
-  __shared__ TokenRows rows[W][2][kTile];
+  // H > 1: of two waves of the same tokens the first loads keys, the other values, past
+  // LDS for both; rows of keys lie 16 bytes further apart than they are long, so that
+  // 16 rows' pieces are on distinct banks.
+  constexpr bool SHARED = H > 1;
+  static_assert(H <= 2, "");
+  constexpr int kRowK = 2 * DP + 16;
+  // a wave's values (or keys), then its outputs of a tile of rows
+  constexpr int kPiece = kTile * kRow;
+  static_assert(kPiece >= kTile * kRowK && kPiece >= kRowTile * DP * 4 && H * W * kPiece >= ROWS * DP * 4, "");
+  __shared__ __attribute__((aligned(16))) char v_lds[H * W][kPiece];
+  __shared__ TokenRows rows[H * W][2][kTile];
   __shared__ float ml[2][W][ROWS];
   __shared__ uint32_t ticket;
-  __shared__ RowSight sight[TREE ? W : 1][TREE ? ROWS : 1];  // (a wave's own copy: read where a tile is hidden from some)
+  __shared__ RowSight sight[TREE ? H * W : 1][TREE ? MINE : 1];  // (a wave's own copy: read where a tile is hidden from some)
+  // TREE: outputs that are +infinity (1), -infinity (2) or NaN (3) by a value that is,
+  // 16 in a word; whether there are any.
+  __shared__ uint32_t odd_out[TREE ? ROWS : 1][TREE ? DP / 16 : 1], odd_any;
+  if constexpr (TREE) {
+    for (int x = threadIdx.x; x < ROWS * (DP / 16); x += 64 * H * W) odd_out[x / (DP / 16)][x % (DP / 16)] = 0;
+    if (threadIdx.x == 0) odd_any = 0;
+    __syncthreads();
+  }
   // Many rows' queries are read from LDS at each tile, in the order of the
   // operands: registers hold no more beside the outputs.
-  constexpr bool Q_LDS = RT * KS >= 12;
-  // 32 rows of 256 columns: the next keys' registers are free only behind the values' products.
-  constexpr bool K_LATE = RT * DP > 256 && DP > 192;
-  __shared__ __attribute__((aligned(16))) v8 q_lds[Q_LDS ? RT : 1][KS][64];
+  constexpr bool Q_LDS = H * RT > 1;
+  // 256 columns: the next keys' registers are free only behind the values' products.
+  constexpr bool K_LATE = RT > 1 && DP > 192;
+  __shared__ __attribute__((aligned(16))) v8 q_lds[Q_LDS ? H * RT : 1][KS][64];
 
   const int lane0 = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int half = H > 1 ? wave / W : 0, first_tile = wave - half * W;  // its set, and its tile of each W
   const int per_seq = a.hkv * a.row_groups;  // (cache head, row group) pairs of a sequence
   const int all_rows = TREE ? a.tokens * a.group : a.group;
 
   // All units, and this workgroup's run of them.
-  const int units0 = span_of<UNIT, TREE>(a, lane0 < a.batch ? a.lengths[lane0] : 0).units;
+  const int units0 = span_of<UNIT, TREE, LEAD>(a, lane0 < a.batch ? a.lengths[lane0] : 0).units;
   auto units_of = [&](int b0) __attribute__((always_inline)) {
     const int x = b0 + lane0;
-    const int u = b0 == 0 ? units0 : span_of<UNIT, TREE>(a, x < a.batch ? a.lengths[x] : 0).units;
+    const int u = b0 == 0 ? units0 : span_of<UNIT, TREE, LEAD>(a, x < a.batch ? a.lengths[x] : 0).units;
     return x < a.batch ? (int64_t)u * per_seq : (int64_t)0;
   };
   const int64_t upto0 = wave_scan(units_of(0), lane0);  // inclusive, of the first 64 sequences
@@ -307,7 +368,15 @@ __global__ void __launch_bounds__((64 * paged_waves<DP, RT>()), 1) paged_attenti
   }
   b = __builtin_amdgcn_readfirstlane(b);
   seq0 = uniform(seq0);
-  Span sp = span_of<UNIT, TREE>(a, a.lengths[b]);
+  Span sp = span_of<UNIT, TREE, LEAD>(a, a.lengths[b]);
+
+  // TREE: scores are scaled behind their maximum, so a negative scale's sign goes
+  // to the queries (and a scale of 0 is next to it: 0 times a masked -infinity).
+  const float scale = TREE ? fmaxf(fabsf(a.scale), 1e-30f) : a.scale;
+  const uint32_t q_sign = TREE && a.scale < 0.0f ? 0x80008000u : 0u;
+  auto signed_q = [&](v8 q) __attribute__((always_inline)) {
+    return TREE ? __builtin_bit_cast(v8, __builtin_bit_cast(u32x4, q) ^ q_sign) : q;
+  };
 
   while (at < end) {
     // a segment: units [j0, j1) of one (sequence, cache head, row group)
@@ -326,12 +395,24 @@ __global__ void __launch_bounds__((64 * paged_waves<DP, RT>()), 1) paged_attenti
     const T* vbase = static_cast<const T*>(a.v) + kvh * a.vc_head;
     const T* zeros = reinterpret_cast<const T*>(kZeros);
 
+    const int unit0 = LEAD ? max(j0 - LEAD, 0) : j0;  // first of tokens
+    const int tiles = (LEAD ? max(j1 - LEAD, 0) - unit0 : j1 - j0) * W;
+    auto first_of = [&](int i) __attribute__((always_inline)) { return sp.token(unit0 * UNIT + i * kTile); };  // token of tile i
+    auto page_of = [&](int i) __attribute__((always_inline)) {  // of lane's token of tile i; -1: masked
+      const int t = first_of(i) + (lane & 31);
+      int page = -1;
+      if (i < tiles && (t >= sp.first || t < sp.sinks) && t < sp.len) page = bt[(uint32_t)t / (uint32_t)a.page_size];
+      return page;  // (looked at by put_rows, a step later: here it would be waited for)
+    };
+    int page0 = -1, page = -1;  // TREE: ahead of the queries and their sights
+    if constexpr (TREE) page0 = page_of(first_tile), page = page_of(first_tile + W);
+
     // Q^T: a lane holds columns 32 s + 8 lg .. + 7 of row 16 r + lr
     v8 q[Q_LDS ? 1 : RT][KS];
     int all_first = 0;  // TREE: where the last row's window begins
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
-      const int row = row0 + kRowTile * r + lr;
+      const int row = row0 + half * MINE + kRowTile * r + lr;
       const T* p = static_cast<const T*>(a.q) + b * a.q_batch;
       if constexpr (TREE) {
         const int token = min(row, all_rows - 1) / a.group;
@@ -358,9 +439,9 @@ __global__ void __launch_bounds__((64 * paged_waves<DP, RT>()), 1) paged_attenti
       }
 #pragma unroll
       for (int s = 0; s < KS; ++s) {
-        const bool in = kRowTile * r + lr < heads && (EXACT || 32 * s + 8 * lg < a.d);
-        if constexpr (!Q_LDS) q[r][s] = load16<v8>(in ? p + 32 * s + 8 * lg : zeros);
-        else if (wave == (r * KS + s) % W) q_lds[r][s][lane] = load16<v8>(in ? p + 32 * s + 8 * lg : zeros);
+        const bool in = row - row0 < heads && (EXACT || 32 * s + 8 * lg < a.d);
+        if constexpr (!Q_LDS) q[r][s] = signed_q(load16<!TREE, v8>(in ? p + 32 * s + 8 * lg : zeros));
+        else if (first_tile == (r * KS + s) % W) q_lds[half * RT + r][s][lane] = signed_q(load16<!TREE, v8>(in ? p + 32 * s + 8 * lg : zeros));
       }
     }
     if constexpr (TREE) {
@@ -373,14 +454,6 @@ __global__ void __launch_bounds__((64 * paged_waves<DP, RT>()), 1) paged_attenti
 
     if constexpr (Q_LDS) __syncthreads();
 
-    const int tiles = (j1 - j0) * W;
-    auto first_of = [&](int i) __attribute__((always_inline)) { return sp.token(j0 * UNIT + i * kTile); };  // token of tile i
-    auto page_of = [&](int i) __attribute__((always_inline)) {  // of lane's token of tile i; -1: masked
-      const int t = first_of(i) + (lane & 31);
-      int page = -1;
-      if (i < tiles && (t >= sp.first || t < sp.sinks) && t < sp.len) page = bt[(uint32_t)t / (uint32_t)a.page_size];
-      return page;  // (looked at by put_rows, a step later: here it would be waited for)
-    };
     auto put_rows = [&](int i, int page) __attribute__((always_inline)) {
       const int t = first_of(i) + (lane & 31);
       const uint32_t slot = (uint32_t)t % (uint32_t)a.page_size;
@@ -389,13 +462,13 @@ __global__ void __launch_bounds__((64 * paged_waves<DP, RT>()), 1) paged_attenti
         r = TokenRows{(uint64_t)(kbase + page * a.kc_page + slot * a.kc_slot), (uint64_t)(vbase + page * a.vc_page + slot * a.vc_slot)};
       if (lane < kTile) rows[wave][(i / W) & 1][lane] = r;
     };
-    v8 k[2][KS], v[VL];
+    v8 k[SHARED ? 1 : 2][KS], v[VL];
     auto load_k = [&](int i) __attribute__((always_inline)) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const T* r = reinterpret_cast<const T*>(rows[wave][(i / W) & 1][16 * h + lr].k) + 8 * lg;
 #pragma unroll
-        for (int s = 0; s < KS; ++s) k[h][s] = load16<v8>(EXACT || 32 * s + 8 * lg < a.d ? r + 32 * s : zeros);
+        for (int s = 0; s < KS; ++s) k[h][s] = load16<!TREE, v8>(EXACT || 32 * s + 8 * lg < a.d ? r + 32 * s : zeros);
       }
     };
     // chunk c of a lane: 16-byte piece v_piece(c) of token v_token(c)
@@ -404,8 +477,9 @@ __global__ void __launch_bounds__((64 * paged_waves<DP, RT>()), 1) paged_attenti
     auto load_v = [&](int i) __attribute__((always_inline)) {
 #pragma unroll
       for (int c = 0; c < VL; ++c) {
-        const T* r = reinterpret_cast<const T*>(rows[wave][(i / W) & 1][v_token(c)].v) + 8 * v_piece(c);
-        v[c] = load16<v8>(EXACT || 8 * v_piece(c) < a.d ? r : zeros);
+        const TokenRows& at = rows[wave][(i / W) & 1][v_token(c)];
+        const T* r = reinterpret_cast<const T*>(SHARED && half == 0 ? at.k : at.v) + 8 * v_piece(c);
+        v[c] = load16<!TREE, v8>(EXACT || 8 * v_piece(c) < a.d ? r : zeros);
       }
     };
 
@@ -418,190 +492,304 @@ __global__ void __launch_bounds__((64 * paged_waves<DP, RT>()), 1) paged_attenti
       m[r] = kLeastScore, l[r] = 0.0f;
     }
 
-    put_rows(wave, page_of(wave));
+    put_rows(first_tile, TREE ? page0 : page_of(first_tile));
     wave_lds_fence();
     // (in the loop's order, next pages, keys, values: its waits count loads)
-    int page = page_of(wave + W);
+    if constexpr (!TREE) page = page_of(first_tile + W);
     __builtin_amdgcn_sched_barrier(0);
-    load_k(wave);
-    __builtin_amdgcn_sched_barrier(0);
-    load_v(wave);
-    __builtin_amdgcn_sched_barrier(0);
-    for (int i = wave; i < tiles; i += W) {
-      // rows of the next tile, pages of the one after
-      const uint64_t masked = __ballot(rows[wave][(i / W) & 1][lane & 31].k == (uint64_t)zeros);
-      put_rows(i + W, page);
-      wave_lds_fence();
-      page = page_of(i + 2 * W);
-
-      f32x4 s[RT][2];
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-#pragma unroll
-        for (int r = 0; r < RT; ++r) s[r][h] = f32x4{0, 0, 0, 0};
-#pragma unroll
-        for (int c = 0; c < KS; ++c)
-#pragma unroll
-          for (int r = 0; r < RT; ++r) s[r][h] = Mma<T>::mul(k[h][c], Q_LDS ? q_lds[r][c][lane] : q[r][c], s[r][h]);
-      }
-      // (sched_barrier: moved up, the loads would take registers of their own)
+    if constexpr (!SHARED) {
+      load_k(first_tile);
       __builtin_amdgcn_sched_barrier(0);
-      if (!K_LATE) load_k(i + W);
-
-      // lane: row 16 r + lr, tokens 16 h + 4 lg + e
+    }
+    load_v(first_tile);
+    __builtin_amdgcn_sched_barrier(0);
+    const int v_wave = SHARED ? W + first_tile : wave;  // whose piece holds the values
+    auto put_v = [&]() __attribute__((always_inline)) {
 #pragma unroll
-      for (int r = 0; r < RT; ++r)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) s[r][h] *= a.scale;
-      if (masked) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (masked >> (16 * h + 4 * lg + e) & 1) {
-#pragma unroll
-              for (int r = 0; r < RT; ++r) s[r][h][e] = -INFINITY;
-            }
-      }
-      // TREE: tokens that some rows see and others do not
+      for (int c = 0; c < VL; ++c) *reinterpret_cast<v8*>(v_lds[wave] + v_token(c) * kRow + 16 * v_piece(c)) = v[c];
+    };
+    // TREE: a value that is not finite may meet only the rows that see it.  In tiles
+    // that are hidden from some it is noted for those that do, and zero in LDS.
+    auto clean_v = [&](int i) __attribute__((always_inline)) {
       const int t0 = first_of(i);
-      const bool some = TREE && !(t0 + kTile <= sp.before && (t0 >= all_first || t0 + kTile <= a.sinks));
-      uint32_t seen[RT];  // of those the lane's, as bits
-      if (TREE && some) {
+      if (t0 + kTile <= sp.before && (a.window <= 0 || t0 >= sp.before + a.tokens - a.window || t0 + kTile <= a.sinks)) return;
+      bool found = false;
 #pragma unroll
-        for (int r = 0; r < RT; ++r) {
-          seen[r] = 0;
-          const RowSight mine = sight[wave][kRowTile * r + lr];
+      for (int c = 0; c < VL; ++c) {
+        const i16x8 w = __builtin_bit_cast(i16x8, v[c]);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) found |= ((uint32_t)w[e] & Mma<T>::kExponent) == Mma<T>::kExponent;
+      }
+      if (!__any(found)) return;
+      wave_lds_fence();
+#pragma unroll 1
+      for (int c = lane; c < kTile * DP; c += 64) {
+        T* at = reinterpret_cast<T*>(v_lds[wave] + c / DP * kRow) + c % DP;
+        const uint32_t w = __builtin_bit_cast(uint16_t, *at);
+        if ((w & Mma<T>::kExponent) != Mma<T>::kExponent) continue;
+        *at = (T)0.0f;
+        const uint32_t is = w & (0x7fff & ~Mma<T>::kExponent) ? 3 : w >> 15 ? 2 : 1;
+        const int t = t0 + c / DP, j = t - sp.before;
+        for (int r = 0; r < ROWS; ++r) {
+          const RowSight mine = sight[H == 1 ? wave : r / MINE * W + first_tile][r % MINE];
+          if (j < 0 ? t >= mine.first || t < a.sinks : j < a.tokens && (mine.bits >> (j & 63) & 1))
+            atomicOr(&odd_out[r][c % DP / 16], is << (2 * (c % 16)));
+        }
+      }
+      if (lane == 0) odd_any = 1;
+      wave_lds_fence();
+    };
+    // V^T: a lane takes column 16 t + lr of tokens 16 h + 4 lg .. + 3
+    auto read_v = [&](int t) __attribute__((always_inline)) {
+      i16x4 part[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        part[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            (__attribute__((address_space(3))) i16x4*)(v_lds[v_wave] + (16 * h + 4 * lg + (lr >> 2)) * kRow + 32 * t +
+                                                       8 * (lr & 3)));
+      return (i16x8)__builtin_shufflevector(part[0], part[1], 0, 1, 2, 3, 4, 5, 6, 7);
+    };
+    if constexpr (!TREE) {
+      for (int i = first_tile; i < tiles; i += W) {
+        // rows of the next tile, pages of the one after
+        const uint64_t masked = __ballot(rows[wave][(i / W) & 1][lane & 31].k == (uint64_t)zeros);
+        put_rows(i + W, page);
+        wave_lds_fence();
+        page = page_of(i + 2 * W);
+
+        f32x4 s[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          s[h] = f32x4{0, 0, 0, 0};
+#pragma unroll
+          for (int c = 0; c < KS; ++c) s[h] = Mma<T>::mul(k[h][c], q[0][c], s[h]);
+        }
+        // (sched_barrier: moved up, the loads would take registers of their own)
+        __builtin_amdgcn_sched_barrier(0);
+        load_k(i + W);
+
+        // lane: row lr, tokens 16 h + 4 lg + e
+#pragma unroll
+        for (int h = 0; h < 2; ++h) s[h] *= a.scale;
+        if (masked) {
 #pragma unroll
           for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int t = t0 + 16 * h + 4 * lg + e, j = t - sp.before;
-              const bool sees = j < 0 ? t >= mine.first || t < a.sinks : j < a.tokens && (mine.bits >> (j & 63) & 1);
-              if (sees) seen[r] |= 1u << (4 * h + e);
-              else s[r][h][e] = -INFINITY;
-            }
+            for (int e = 0; e < 4; ++e)
+              if (masked >> (16 * h + 4 * lg + e) & 1) s[h][e] = -INFINITY;
         }
-      }
-      v8 p[RT], rest[RT];
-#pragma unroll
-      for (int r = 0; r < RT; ++r) {
-        float top = m[r];  // (a NaN is not its maximum, but makes its exponential, so the sums, NaN)
+        float top = m[0];  // (a NaN is not its maximum, but makes its exponential, so the sums, NaN)
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) top = fmaxf(top, s[r][h][e]);
+          for (int e = 0; e < 4; ++e) top = fmaxf(top, s[h][e]);
         top = combine32<MaxOp>(combine16<MaxOp>(top));
-        const float keep = __builtin_amdgcn_exp2f(m[r] - top);
-        m[r] = top;
-        l[r] *= keep;
+        const float keep = __builtin_amdgcn_exp2f(m[0] - top);
+        m[0] = top;
+        l[0] *= keep;
         float x8[8];
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const float x = __builtin_amdgcn_exp2f(s[r][h][e] - top) * Mma<T>::kUnit;
-            l[r] += x;
+            const float x = __builtin_amdgcn_exp2f(s[h][e] - top) * Mma<T>::kUnit;
+            l[0] += x;
             x8[4 * h + e] = x;
           }
+        v8 p, rest;
 #pragma unroll
-        for (int e = 0; e < 8; e += 2) Mma<T>::cut(x8[e], x8[e + 1], p[r], rest[r], e);
+        for (int e = 0; e < 8; e += 2) Mma<T>::cut(x8[e], x8[e + 1], p, rest, e);
 #pragma unroll
-        for (int t = 0; t < DT; ++t) o[r][t] *= keep;
-      }
+        for (int t = 0; t < DT; ++t) o[0][t] *= keep;
 
-      // TREE: a value that is not finite may meet only the rows that see it
-      bool odd = false;
-      if (TREE && some) {
-        bool found = false;
-#pragma unroll
-        for (int c = 0; c < VL; ++c) {
-          const i16x8 w = __builtin_bit_cast(i16x8, v[c]);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) found |= ((uint32_t)w[e] & Mma<T>::kExponent) == Mma<T>::kExponent;
-        }
-        odd = __any(found);
-      }
-#pragma unroll
-      for (int c = 0; c < VL; ++c) {
-        *reinterpret_cast<v8*>(v_lds[wave] + v_token(c) * kRow + 16 * v_piece(c)) = v[c];
-      }
-      wave_lds_fence();
-      __builtin_amdgcn_sched_barrier(0);
-      load_v(i + W);
-      __builtin_amdgcn_sched_barrier(0);
-      // V^T: a lane takes column 16 t + lr of tokens 16 h + 4 lg .. + 3
-      auto read_v = [&](int t) __attribute__((always_inline)) {
-        i16x4 part[2];
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-          part[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-              (__attribute__((address_space(3))) i16x4*)(v_lds[wave] + (16 * h + 4 * lg + (lr >> 2)) * kRow + 32 * t +
-                                                         8 * (lr & 3)));
-        return (i16x8)__builtin_shufflevector(part[0], part[1], 0, 1, 2, 3, 4, 5, 6, 7);
-      };
-      if (!TREE || !odd) {
+        put_v();
+        wave_lds_fence();
+        __builtin_amdgcn_sched_barrier(0);
+        load_v(i + W);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int t = 0; t < DT; ++t) {
           const v8 both = __builtin_bit_cast(v8, read_v(t));
-#pragma unroll
-          for (int r = 0; r < RT; ++r) {
-            o[r][t] = Mma<T>::mul(both, p[r], o[r][t]);
-            o[r][t] = Mma<T>::mul(both, rest[r], o[r][t]);
-          }
+          o[0][t] = Mma<T>::mul(both, p, o[0][t]);
+          o[0][t] = Mma<T>::mul(both, rest, o[0][t]);
           if (t % 4 == 3) __builtin_amdgcn_sched_barrier(0);  // (eight reads at a time: registers)
         }
-      } else {
-        // Finite values as ever; those that are not are counted by a product of
-        // their own, of 1 (+infinity), 64 (-infinity) and 4096 (NaN) with 1 where
-        // the row sees the token (4096 where it does without weight: 0 x infinity).
+        wave_lds_fence();
+      }
+    } else {
+      // The largest that exponents are about is moved only where one is above it by
+      // more than kSlack, outside the loop over the tiles: within, the outputs are
+      // the matrix instructions' alone and stay in their registers (64 rows of 128
+      // columns: 128 products and 400 copies a tile otherwise).
+      int i = first_tile;
+      bool staged = false;  // SHARED: the tile is in LDS
+      while (i < tiles) {
+        float top[RT];
+        bool above = false;
+        for (; i < tiles; i += W) {
+          if constexpr (SHARED) {
+            if (!staged) {
+              // this tile past LDS, the next one's loads behind it
+              if (half == 0) {
 #pragma unroll
-        for (int r = 0; r < RT; ++r) {
-          v8 sees;
-#pragma unroll
-          for (int e = 0; e < 8; ++e)
-            sees[e] = (T)(!(seen[r] >> e & 1) ? 0.0f : (float)p[r][e] + (float)rest[r][e] > 0.0f ? 1.0f : 4096.0f);
-#pragma unroll
-          for (int t = 0; t < DT; ++t) {
-            const i16x8 both = read_v(t);
-            i16x8 finite;
-            v8 kind;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              const uint32_t w = (uint16_t)both[e];
-              const bool is = (w & Mma<T>::kExponent) != Mma<T>::kExponent;
-              finite[e] = is ? both[e] : (int16_t)0;
-              kind[e] = (T)(is ? 0.0f : w & (0x7fff & ~Mma<T>::kExponent) ? 4096.0f : w >> 15 ? 64.0f : 1.0f);
+                for (int c = 0; c < VL; ++c) *reinterpret_cast<v8*>(v_lds[wave] + v_token(c) * kRowK + 16 * v_piece(c)) = v[c];
+              } else {
+                put_v();
+                clean_v(i);
+              }
+              __syncthreads();
+              put_rows(i + W, page);
+              wave_lds_fence();
+              page = page_of(i + 2 * W);
+              __builtin_amdgcn_sched_barrier(0);
+              load_v(i + W);
+              __builtin_amdgcn_sched_barrier(0);
             }
-            o[r][t] = Mma<T>::mul(__builtin_bit_cast(v8, finite), p[r], o[r][t]);
-            o[r][t] = Mma<T>::mul(__builtin_bit_cast(v8, finite), rest[r], o[r][t]);
-            const f32x4 n = Mma<T>::mul(kind, sees, f32x4{0, 0, 0, 0});
+            staged = true;
+          }
+          f32x4 s[RT][2];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const uint32_t c = (uint32_t)n[e];  // (at most 32 of each)
-              const bool plus = c & 63, minus = c >> 6 & 63;
-              if (c >= 4096 || (plus && minus)) o[r][t][e] = __builtin_nanf("");
-              else if (plus || minus) o[r][t][e] += plus ? INFINITY : -INFINITY;
+          for (int h = 0; h < 2; ++h) {
+#pragma unroll
+            for (int r = 0; r < RT; ++r) s[r][h] = f32x4{0, 0, 0, 0};
+#pragma unroll
+            for (int c = 0; c < KS; ++c) {
+              const v8 kc = SHARED ? *reinterpret_cast<const v8*>(v_lds[first_tile] + (16 * h + lr) * kRowK + 64 * c + 16 * lg) : k[SHARED ? 0 : h][c];
+#pragma unroll
+              for (int r = 0; r < RT; ++r) s[r][h] = Mma<T>::mul(kc, Q_LDS ? q_lds[half * RT + r][c][lane] : q[r][c], s[r][h]);
             }
+          }
+          // lane: row 16 r + lr, tokens 16 h + 4 lg + e
+          const uint64_t masked = __ballot(rows[wave][(i / W) & 1][lane & 31].k == (uint64_t)zeros);
+          if (masked) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                if (masked >> (16 * h + 4 * lg + e) & 1) {
+#pragma unroll
+                  for (int r = 0; r < RT; ++r) s[r][h][e] = -INFINITY;
+                }
+          }
+          // tokens that some rows see and others do not
+          const int t0 = first_of(i);
+          const bool some = !(t0 + kTile <= sp.before && (t0 >= all_first || t0 + kTile <= a.sinks));
+          if (some) {
+#pragma unroll
+            for (int r = 0; r < RT; ++r) {
+              const RowSight mine = sight[wave][kRowTile * r + lr];
+#pragma unroll
+              for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  const int t = t0 + 16 * h + 4 * lg + e, j = t - sp.before;
+                  const bool sees = j < 0 ? t >= mine.first || t < a.sinks : j < a.tokens && (mine.bits >> (j & 63) & 1);
+                  if (!sees) s[r][h][e] = -INFINITY;
+                }
+            }
+          }
+          above = false;
+#pragma unroll
+          for (int r = 0; r < RT; ++r) {
+            top[r] = -INFINITY;
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) top[r] = fmaxf(top[r], s[r][h][e]);
+            top[r] = combine32<MaxOp>(combine16<MaxOp>(top[r])) * scale;
+            above |= top[r] > m[r] + kSlack;
+          }
+          if (__any(above)) {  // (the tile is begun again)
+            above = true;
+            break;
+          }
+          if constexpr (!SHARED) {
+            // rows of the next tile, pages of the one after
+            put_rows(i + W, page);
+            wave_lds_fence();
+            page = page_of(i + 2 * W);
+            __builtin_amdgcn_sched_barrier(0);
+            if (!K_LATE) load_k(i + W);
+          }
+
+          v8 p[RT], rest[RT];
+#pragma unroll
+          for (int r = 0; r < RT; ++r) {
+            const float about = kTreeUnit<T> - m[r];
+            float x8[8];
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r][h][e], scale, about));
+                l[r] += x;
+                x8[4 * h + e] = x;
+              }
+#pragma unroll
+            for (int e = 0; e < 8; e += 2) Mma<T>::cut_above(x8[e], x8[e + 1], p[r], rest[r], e);
+          }
+          // a value that is not finite may meet only the rows that see it
+          if constexpr (!SHARED) {
+            put_v();
+            clean_v(i);
+            wave_lds_fence();
+            __builtin_amdgcn_sched_barrier(0);
+            load_v(i + W);
             __builtin_amdgcn_sched_barrier(0);
           }
+#pragma unroll
+          for (int t = 0; t < DT; ++t) {
+            const v8 both = __builtin_bit_cast(v8, read_v(t));
+#pragma unroll
+            for (int r = 0; r < RT; ++r) {
+              o[r][t] = Mma<T>::mul(both, p[r], o[r][t]);
+              o[r][t] = Mma<T>::mul(both, rest[r], o[r][t]);
+            }
+            if (t % 4 == 3) __builtin_amdgcn_sched_barrier(0);  // (eight reads at a time: registers)
+          }
+          if constexpr (SHARED) {
+            staged = false;
+            __syncthreads();  // (both waves have read the tile)
+          } else {
+            wave_lds_fence();
+            if (K_LATE) load_k(i + W);
+          }
+        }
+        if (!above) break;
+#pragma unroll
+        for (int r = 0; r < RT; ++r) {
+          const float to = top[r] > m[r] + kSlack ? top[r] : m[r], keep = __builtin_amdgcn_exp2f(m[r] - to);
+          m[r] = to;
+          l[r] *= keep;
+#pragma unroll
+          for (int t = 0; t < DT; ++t) o[r][t] *= keep;
         }
       }
-      wave_lds_fence();
-      if (K_LATE) load_k(i + W);
     }
 
     // the waves' states, through LDS
     const int tid = opaque((int)threadIdx.x);
-    float* ow = reinterpret_cast<float*>(v_lds[wave]);
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
       l[r] = combine32<AddOp>(combine16<AddOp>(l[r]));
-#pragma unroll
-      for (int t = 0; t < DT; ++t) *reinterpret_cast<f32x4*>(ow + (kRowTile * r + lr) * DP + 16 * t + 4 * lg) = o[r][t];
-      if (lane < kRowTile) ml[0][wave][kRowTile * r + lane] = m[r], ml[1][wave][kRowTile * r + lane] = l[r];
+      if (lane < kRowTile) {
+        const int row = half * MINE + kRowTile * r + lane;
+        ml[0][first_tile][row] = m[r], ml[1][first_tile][row] = l[r];
+      }
     }
-    __syncthreads();
+    auto with_odd = [&](int h, int c, f32x4 y) __attribute__((always_inline)) {
+      if constexpr (TREE) {
+        if (odd_any) {
+          const uint32_t word = odd_out[h][c / 16] >> (2 * (c % 16));
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const uint32_t is = word >> (2 * e) & 3;
+            if (is) y[e] += is == 3 ? __builtin_nanf("") : is == 1 ? INFINITY : -INFINITY;
+          }
+        }
+      }
+      return y;
+    };
     auto put_out = [&](int h, int c, f32x4 y, float, float sum) __attribute__((always_inline)) {
       int64_t at_row = (int64_t)b * a.hq + kvh * a.group + row0 + h;
       if constexpr (TREE) {
@@ -610,8 +798,27 @@ __global__ void __launch_bounds__((64 * paged_waves<DP, RT>()), 1) paged_attenti
       }
       store_out(static_cast<T*>(a.out) + at_row * a.d, a.d, c, y, sum);
     };
+    // (each set's r-th tile of rows)
+    auto join = [&](auto f) __attribute__((always_inline)) {
+      float* ow = reinterpret_cast<float*>(v_lds[wave]);
+#pragma unroll
+      for (int r = 0; r < RT; ++r) {
+        if (r > 0) __syncthreads();
+#pragma unroll
+        for (int t = 0; t < DT; ++t) *reinterpret_cast<f32x4*>(ow + lr * DP + 16 * t + 4 * lg) = o[r][t];
+        __syncthreads();
+        join_waves<DP, W, ROWS, 64 * H * W>(
+            tid, H == 1 ? min(kRowTile, heads - kRowTile * r) : H * kRowTile, heads, W, ml,
+            [&](int w, int j) __attribute__((always_inline)) {
+              return reinterpret_cast<const float*>(v_lds[(H == 1 ? 0 : j / kRowTile * W) + w]) + (H == 1 ? j : j % kRowTile) * DP;
+            },
+            [&](int j) __attribute__((always_inline)) { return H == 1 ? kRowTile * r + j : j / kRowTile * MINE + kRowTile * r + j % kRowTile; }, f);
+      }
+    };
     if (j0 == 0 && j1 == sp.units) {
-      join_waves<DP, W, ROWS>(tid, heads, W, ml, v_lds[0], kPiece, put_out);
+      join([&](int h, int c, f32x4 y, float top, float sum) __attribute__((always_inline)) {
+        put_out(h, c, with_odd(h, c, y), top, sum);
+      });
     } else {
       // The state goes to the workspace, and the last workgroup of this head
       // joins them all.  They belong to consecutive workgroups g0 .. g1; each
@@ -621,73 +828,151 @@ __global__ void __launch_bounds__((64 * paged_waves<DP, RT>()), 1) paged_attenti
       // needs no fence, only the stores' completion: a fence writes back the
       // whole L2 (64 sequences x 8192 tokens of one cache head: 186 us with a
       // fence per workgroup).
-      constexpr int STATE = state_floats<DP, RT>();
+      constexpr int STATE = state_floats<DP, H * RT>();
       float* part = a.parts + ((int64_t)blockIdx.x * 2 + (at != start)) * STATE;
-      join_waves<DP, W, ROWS>(tid, heads, W, ml, v_lds[0], kPiece, [&](int h, int c, f32x4 y, float top, float sum) {
-        put_device(part + 2 * ROWS + h * DP + c, y[0], y[1]);
-        put_device(part + 2 * ROWS + h * DP + c + 2, y[2], y[3]);
-        if (c == 0) put_device(part + 2 * h, top, sum);
-      });
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-      __syncthreads();
-      const int64_t u0 = seq0 + (int64_t)pair * sp.units, u1 = u0 + sp.units;
-      const int64_t g0 = ((u0 + 1) * wgs - 1) / total, g1 = (u1 * wgs - 1) / total;
-      const int n = (int)(g1 - g0 + 1);
-      uint32_t* counter = a.counters + (int64_t)b * per_seq + pair;
-      if (tid == 0) ticket = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      __syncthreads();
-      if (ticket == (uint32_t)n - 1) {
-        if (tid == 0) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        const int later = g0 * total / wgs < u0;  // g0's state is its second
-        const float* parts = a.parts + (g0 * 2 + later) * STATE;
-        const int64_t next = (2 - later) * STATE;  // g0 + 1's, from g0's
-        // 64 pieces (a row, 4 columns) of the states are a wave's, or, of few
-        // pieces, every PG-th of their states; its loads are in flight together
-        const int pieces = heads * (DP / 4), groups = (pieces + 63) / 64, pg = max(1, W / groups);
-        auto gather = [&](auto ahead) __attribute__((always_inline)) {
-          constexpr int A = decltype(ahead)::value;
-          for (int x = wave; x < groups * pg; x += W) {
-            const int part = x / groups, i = (x - part * groups) * 64 + lane;
-            if (i >= pieces) continue;
-            const int h = i / (DP / 4), c = 4 * (i - h * (DP / 4));
-            float top = kLeastScore, sum = 0.0f;
-            f32x4 y{0, 0, 0, 0};
-            for (int g = part; g < n; g += pg * A) {
-              f32x2 pm[A], po[A][2];
-#pragma unroll
-              for (int z = 0; z < A; ++z) {
-                const int gz = min(g + z * pg, n - 1);
-                const float* p = parts + (gz == 0 ? 0 : next + (int64_t)(gz - 1) * 2 * STATE);
-                pm[z] = get_device(p + 2 * h);
-                po[z][0] = get_device(p + 2 * ROWS + h * DP + c);
-                po[z][1] = get_device(p + 2 * ROWS + h * DP + c + 2);
-              }
-#pragma unroll
-              for (int z = 0; z < A; ++z)
-                if (g + z * pg < n) {
-                  const float m2 = MaxOp::of(top, pm[z][0]);
-                  const float f = __builtin_amdgcn_exp2f(top - m2), fz = __builtin_amdgcn_exp2f(pm[z][0] - m2);
-                  sum = sum * f + pm[z][1] * fz;
-                  y = y * f + f32x4{po[z][0][0], po[z][0][1], po[z][1][0], po[z][1][1]} * fz;
-                  top = m2;
-                }
-            }
-            *reinterpret_cast<f32x4*>(reinterpret_cast<float*>(v_lds[part]) + h * DP + c) = y;
-            if (c == 0) ml[0][part][h] = top, ml[1][part][h] = sum;
-          }
-        };
-        if (n <= 4 * pg) gather(std::integral_constant<int, 4>{});
-        else gather(std::integral_constant<int, 16>{});
+      if constexpr (H > 1) {
+        // (of many rows a state is 33 KB: another launch joins them on all CUs)
+        join([&](int h, int c, f32x4 y, float top, float sum) __attribute__((always_inline)) {
+          *reinterpret_cast<f32x4*>(part + 2 * ROWS + h * DP + c) = with_odd(h, c, y);
+          if (c == 0) part[2 * h] = top, part[2 * h + 1] = sum;
+        });
+      } else {
+        join([&](int h, int c, f32x4 y, float top, float sum) __attribute__((always_inline)) {
+          y = with_odd(h, c, y);
+          put_device(part + 2 * ROWS + h * DP + c, y[0], y[1]);
+          put_device(part + 2 * ROWS + h * DP + c + 2, y[2], y[3]);
+          if (c == 0) put_device(part + 2 * h, top, sum);
+        });
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
-        join_waves<DP, W, ROWS>(tid, heads, pg, ml, v_lds[0], kPiece, put_out);
+        const int64_t u0 = seq0 + (int64_t)pair * sp.units, u1 = u0 + sp.units;
+        const int64_t g0 = ((u0 + 1) * wgs - 1) / total, g1 = (u1 * wgs - 1) / total;
+        const int n = (int)(g1 - g0 + 1);
+        uint32_t* counter = a.counters + (int64_t)b * per_seq + pair;
+        if (tid == 0) ticket = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        __syncthreads();
+        if (ticket == (uint32_t)n - 1) {
+          if (tid == 0) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+          const int later = g0 * total / wgs < u0;  // g0's state is its second
+          const float* parts = a.parts + (g0 * 2 + later) * STATE;
+          const int64_t next = (2 - later) * STATE;  // g0 + 1's, from g0's
+          // 64 pieces (a row, 4 columns) of the states are a wave's, or, of few
+          // pieces, every PG-th of their states; its loads are in flight together
+          const int pieces = heads * (DP / 4), groups = (pieces + 63) / 64, pg = max(1, W / groups);
+          float* joined = reinterpret_cast<float*>(v_lds[0]);  // [pg][groups * 64 pieces]
+          auto gather = [&](auto ahead) __attribute__((always_inline)) {
+            constexpr int A = decltype(ahead)::value;
+            for (int x = wave; x < groups * pg; x += H * W) {
+              const int part = x / groups, i = (x - part * groups) * 64 + lane;
+              if (i >= pieces) continue;
+              const int h = i / (DP / 4), c = 4 * (i - h * (DP / 4));
+              float top = kLeastScore, sum = 0.0f;
+              f32x4 y{0, 0, 0, 0};
+              for (int g = part; g < n; g += pg * A) {
+                f32x2 pm[A], po[A][2];
+  #pragma unroll
+                for (int z = 0; z < A; ++z) {
+                  const int gz = min(g + z * pg, n - 1);
+                  const float* p = parts + (gz == 0 ? 0 : next + (int64_t)(gz - 1) * 2 * STATE);
+                  pm[z] = get_device(p + 2 * h);
+                  po[z][0] = get_device(p + 2 * ROWS + h * DP + c);
+                  po[z][1] = get_device(p + 2 * ROWS + h * DP + c + 2);
+                }
+  #pragma unroll
+                for (int z = 0; z < A; ++z)
+                  if (g + z * pg < n) {
+                    const float m2 = MaxOp::of(top, pm[z][0]);
+                    const float f = __builtin_amdgcn_exp2f(top - m2), fz = __builtin_amdgcn_exp2f(pm[z][0] - m2);
+                    sum = sum * f + pm[z][1] * fz;
+                    y = y * f + f32x4{po[z][0][0], po[z][0][1], po[z][1][0], po[z][1][1]} * fz;
+                    top = m2;
+                  }
+              }
+              *reinterpret_cast<f32x4*>(joined + part * groups * 256 + h * DP + c) = y;
+              if (c == 0) ml[0][part][h] = top, ml[1][part][h] = sum;
+            }
+          };
+          if (n <= 4 * pg) gather(std::integral_constant<int, 4>{});
+          else gather(std::integral_constant<int, 16>{});
+          __syncthreads();
+          join_waves<DP, W, ROWS, 64 * H * W>(
+              tid, heads, heads, pg, ml,
+              [&](int w, int j) __attribute__((always_inline)) { return joined + w * groups * 256 + j * DP; },
+              [&](int j) __attribute__((always_inline)) { return j; }, put_out);
+        }
       }
     }
     __syncthreads();
+    if constexpr (TREE) {
+      if (odd_any) {  // (the next segment has none yet)
+        __syncthreads();
+        for (int x = threadIdx.x; x < ROWS * (DP / 16); x += 64 * H * W) odd_out[x / (DP / 16)][x % (DP / 16)] = 0;
+        if (threadIdx.x == 0) odd_any = 0;
+        __syncthreads();
+      }
+    }
     at += j1 - j0;
     if (at - seq0 == (int64_t)sp.units * per_seq) {
       seq0 = at;
-      if (++b < a.batch) sp = span_of<UNIT, TREE>(a, a.lengths[b]);
+      if (++b < a.batch) sp = span_of<UNIT, TREE, LEAD>(a, a.lengths[b]);
     }
+  }
+}
+
+// The states that the tree kernel's workgroups (of W waves of tokens) left of a
+// (sequence, cache head, row group), joined: blockIdx.x of those, blockIdx.y 4 rows
+// (131072 tokens, 8 cache heads of 128 and 64 rows: 7.7 us, 16 rows 14).
+template <typename T, int DP, int W, int ROWS>
+__global__ void __launch_bounds__(128) paged_join_kernel(const PagedArgs a, int grid) {
+  constexpr int UNIT = W * kTile, STATE = ROWS * (DP + 2), A = 8;
+  const int lane = threadIdx.x & 63, per_seq = a.hkv * a.row_groups;
+  const int b = blockIdx.x / per_seq, pair = blockIdx.x - b * per_seq;
+  // units of all sequences, and those before this one
+  int64_t total = 0, before = 0;
+  for (int b0 = 0; b0 < a.batch; b0 += 64) {
+    const int x = b0 + lane;
+    const int64_t u = x < a.batch ? (int64_t)span_of<UNIT, true, kLead>(a, a.lengths[x]).units * per_seq : 0;
+    total += __shfl(wave_scan(u, lane), 63);
+    before += __shfl(wave_scan(x < b ? u : 0, lane), 63);
+  }
+  const int units = span_of<UNIT, true, kLead>(a, a.lengths[b]).units;
+  const int64_t wgs = min((int64_t)grid, total);
+  const int64_t u0 = before + (int64_t)pair * units, u1 = u0 + units;
+  const int64_t g0 = ((u0 + 1) * wgs - 1) / total, g1 = (u1 * wgs - 1) / total;
+  const int n = (int)(g1 - g0 + 1);
+  if (n == 1) return;  // (its outputs are written)
+  const int later = g0 * total / wgs < u0;  // g0's state is its second
+  const float* parts = a.parts + (g0 * 2 + later) * STATE;
+  const int64_t next = (2 - later) * STATE;  // g0 + 1's, from g0's
+  const int kvh = pair / a.row_groups, row0 = (pair - kvh * a.row_groups) * ROWS, all_rows = a.tokens * a.group;
+  for (int i = threadIdx.x; i < 4 * (DP / 4); i += 128) {
+    const int h = blockIdx.y * 4 + i / (DP / 4), c = 4 * (i % (DP / 4));
+    if (row0 + h >= all_rows) continue;
+    float top = kLeastScore, sum = 0.0f;
+    f32x4 y{0, 0, 0, 0};
+    for (int g = 0; g < n; g += A) {
+      f32x2 pm[A];
+      f32x4 po[A];
+#pragma unroll
+      for (int z = 0; z < A; ++z) {
+        const int gz = min(g + z, n - 1);
+        const float* p = parts + (gz == 0 ? 0 : next + (int64_t)(gz - 1) * 2 * STATE);
+        pm[z] = *reinterpret_cast<const f32x2*>(p + 2 * h);
+        po[z] = *reinterpret_cast<const f32x4*>(p + 2 * ROWS + h * DP + c);
+      }
+#pragma unroll
+      for (int z = 0; z < A; ++z)
+        if (g + z < n) {
+          const float m2 = MaxOp::of(top, pm[z][0]);
+          const float f = __builtin_amdgcn_exp2f(top - m2), fz = __builtin_amdgcn_exp2f(pm[z][0] - m2);
+          sum = sum * f + pm[z][1] * fz;
+          y = y * f + po[z] * fz;
+          top = m2;
+        }
+    }
+    const int token = (row0 + h) / a.group;
+    const int64_t at_row = ((int64_t)b * a.tokens + token) * a.hq + kvh * a.group + row0 + h - token * a.group;
+    store_out(static_cast<T*>(a.out) + at_row * a.d, a.d, c, y, sum);
   }
 }
 
@@ -697,11 +982,11 @@ inline int padded_d(int64_t d) { return d <= 64 ? 64 : d <= 96 ? 96 : d <= 128 ?
 // Tiles of rows that share a workgroup's keys and values.
 inline int tree_row_tiles(int64_t rows, int dp) { return rows <= kRowTile ? 1 : rows <= 2 * kRowTile || dp > 128 ? 2 : 4; }
 
-template <typename T, int DP, int RT, bool TREE>
+template <typename T, int DP, int RT, int H, bool TREE>
 void launch_rows(const PagedArgs& a, hipStream_t s) {
   const dim3 grid((uint32_t)device_cu_count());
-  if (a.d == DP) hipLaunchKernelGGL((paged_attention_kernel<T, DP, true, RT, TREE>), grid, dim3(64 * paged_waves<DP, RT>()), 0, s, a);
-  else hipLaunchKernelGGL((paged_attention_kernel<T, DP, false, RT, TREE>), grid, dim3(64 * paged_waves<DP, RT>()), 0, s, a);
+  if (a.d == DP) hipLaunchKernelGGL((paged_attention_kernel<T, DP, true, RT, H, TREE>), grid, dim3(64 * H * paged_waves<DP, H>()), 0, s, a);
+  else hipLaunchKernelGGL((paged_attention_kernel<T, DP, false, RT, H, TREE>), grid, dim3(64 * H * paged_waves<DP, H>()), 0, s, a);
 }
 
 // Trees are compiled apart, a type in a file.
@@ -711,9 +996,20 @@ int dispatch_tree_bf16(const PagedArgs& a, hipStream_t s);
 template <typename T, int DP>
 void launch_tree(const PagedArgs& a, hipStream_t s) {
   const int tiles = tree_row_tiles((int64_t)a.tokens * a.group, DP);
-  if (tiles == 1) return launch_rows<T, DP, 1, true>(a, s);
-  if (tiles == 2) return launch_rows<T, DP, 2, true>(a, s);
-  if constexpr (DP <= 128) launch_rows<T, DP, 4, true>(a, s);
+  if (tiles == 1) return launch_rows<T, DP, 1, 1, true>(a, s);
+  if constexpr (DP <= 128) {
+    const dim3 grid((uint32_t)(a.batch * a.hkv * a.row_groups), tiles * kRowTile / 4);
+    constexpr int W = paged_waves<DP, 2>();
+    if (tiles == 2) {
+      launch_rows<T, DP, 1, 2, true>(a, s);
+      hipLaunchKernelGGL((paged_join_kernel<T, DP, W, 2 * kRowTile>), grid, dim3(128), 0, s, a, device_cu_count());
+    } else {
+      launch_rows<T, DP, 2, 2, true>(a, s);
+      hipLaunchKernelGGL((paged_join_kernel<T, DP, W, 4 * kRowTile>), grid, dim3(128), 0, s, a, device_cu_count());
+    }
+  } else {  // (registers and LDS hold no two waves a SIMD)
+    launch_rows<T, DP, 2, 1, true>(a, s);
+  }
 }
 
 template <typename T>

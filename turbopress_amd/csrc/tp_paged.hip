@@ -10,11 +10,11 @@ bool paged_sizes_ok(int64_t batch, int64_t hq, int64_t hkv, int64_t d) {
 template <typename T>
 int dispatch_paged(const PagedArgs& a, hipStream_t s) {
   switch (padded_d(a.d)) {
-    case 64: launch_rows<T, 64, 1, false>(a, s); break;
-    case 96: launch_rows<T, 96, 1, false>(a, s); break;
-    case 128: launch_rows<T, 128, 1, false>(a, s); break;
-    case 192: launch_rows<T, 192, 1, false>(a, s); break;
-    default: launch_rows<T, 256, 1, false>(a, s); break;
+    case 64: launch_rows<T, 64, 1, 1, false>(a, s); break;
+    case 96: launch_rows<T, 96, 1, 1, false>(a, s); break;
+    case 128: launch_rows<T, 128, 1, 1, false>(a, s); break;
+    case 192: launch_rows<T, 192, 1, 1, false>(a, s); break;
+    default: launch_rows<T, 256, 1, 1, false>(a, s); break;
   }
   return launch_status();
 }
