@@ -36,6 +36,7 @@ _LAZY = {
     "tree_ancestors": ("turbopress_amd.paged", "tree_ancestors"),
     "token_logprobs": ("turbopress_amd.logprobs", "token_logprobs"),
     "lora_add": ("turbopress_amd.lora", "lora_add"),
+    "LoraAdapters": ("turbopress_amd.lora", "LoraAdapters"),
     "PagedDecoder": ("turbopress_amd.paged_decode", "PagedDecoder"),
 }
 

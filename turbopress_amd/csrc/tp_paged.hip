@@ -93,7 +93,9 @@ extern "C" int tp_paged_attention_sinks(int dtype, int64_t batch, int64_t hq, in
 }
 
 static bool tree_sizes_ok(int64_t batch, int64_t tokens, int64_t hq, int64_t hkv, int64_t d) {
-  return tokens >= 1 && tokens <= 64 && paged_sizes_ok(batch, hq, hkv, d);
+  if (tokens < 1 || tokens > 64 || !paged_sizes_ok(batch, hq, hkv, d)) return false;
+  const int64_t all = tokens * (hq / hkv), rows = kRowTile * tree_row_tiles(all, padded_d(d));
+  return batch * hkv * ((all + rows - 1) / rows) <= (1 << 24);  // (the joins' workgroups)
 }
 
 extern "C" int64_t tp_paged_tree_attention_workspace_bytes(int64_t batch, int64_t tokens, int64_t hq, int64_t hkv, int64_t d) {

@@ -6,6 +6,10 @@ adds the product of its own request's adapter.  Inference only.
 from __future__ import annotations
 
 import functools
+import json
+import math
+from collections.abc import Mapping, Sequence
+from pathlib import Path
 
 import torch
 from torch import Tensor
@@ -15,7 +19,7 @@ from turbopress_amd.hip_kernel import raw_stream as _raw_stream
 from turbopress_amd.norm import DTYPE_CODES
 from turbopress_amd.paged import _workspace
 
-__all__ = ["lora_add", "MAX_RANK"]
+__all__ = ["lora_add", "LoraAdapters", "MAX_RANK"]
 
 MAX_RANK = 256
 _FAR = 1 << 24  # elements that rows may lie apart without a copy
@@ -99,3 +103,83 @@ def lora_add(y: Tensor, x: Tensor, a: Tensor, b: Tensor, adapters: Tensor, scale
     if st:
         _lib.check(st, "lora_add")
     return out
+
+
+class LoraAdapters:
+    """Adapters of one model, stacked by the projections that they change.
+
+    adapters: of each, {module name: (a [rank, in], b [out, rank])}; scales: of
+    each, what its products are multiplied by.  Adapters may have ranks and
+    modules of their own: what one has not is zeros beside the others'."""
+
+    def __init__(self, adapters: Sequence[Mapping], scales: Sequence[float], dtype: torch.dtype, device="cuda") -> None:
+        if not adapters or len(adapters) != len(scales):
+            raise ValueError(f"{len(adapters)} adapters and {len(scales)} scales: as many are needed, one at least")
+        if dtype not in (torch.float16, torch.bfloat16):
+            raise ValueError(f"dtype must be fp16 or bf16, got {dtype}")
+        self.count = len(adapters)
+        self.scales = torch.tensor([float(s) for s in scales], dtype=torch.float32, device=device)
+        self.stacks: dict = {}
+        for name in dict.fromkeys(n for one in adapters for n in one):
+            pairs = [one.get(name) for one in adapters]
+            for pair in pairs:
+                if pair is not None and (pair[0].dim() != 2 or pair[1].dim() != 2 or pair[0].shape[0] != pair[1].shape[1]
+                                         or not 1 <= pair[0].shape[0] <= MAX_RANK):
+                    raise ValueError(f"{name}: a must be [rank, in] and b [out, rank] with 1 to {MAX_RANK} ranks, got "
+                                     f"{list(pair[0].shape)} and {list(pair[1].shape)}")
+            have = [pair for pair in pairs if pair is not None]
+            sizes = {(pair[0].shape[1], pair[1].shape[0]) for pair in have}
+            if len(sizes) != 1:
+                raise ValueError(f"{name}: adapters of different (in, out): {sorted(sizes)}")
+            (k, n), = sizes
+            rank = max(pair[0].shape[0] for pair in have)
+            a = torch.zeros(self.count, rank, k, dtype=dtype)
+            b = torch.zeros(self.count, n, rank, dtype=dtype)
+            for i, pair in enumerate(pairs):
+                if pair is not None:
+                    a[i, :pair[0].shape[0]] = pair[0]
+                    b[i, :, :pair[0].shape[0]] = pair[1]
+            self.stacks[name] = (a.to(device), b.to(device))
+
+    @classmethod
+    def load(cls, directories: Sequence, dtype: torch.dtype, device="cuda") -> "LoraAdapters":
+        """From directories of ``adapter_config.json`` (r, lora_alpha, use_rslora)
+        and ``adapter_model.safetensors`` (``base_model.model.<module>.lora_A.weight``
+        [rank, in] and ``.lora_B.weight`` [out, rank]).  What such an adapter may have
+        beside its two products is refused."""
+        from safetensors.torch import load_file
+        adapters, scales = [], []
+        for directory in map(Path, directories):
+            cfg = json.loads((directory / "adapter_config.json").read_text())
+            for key in ("use_dora", "rank_pattern", "alpha_pattern", "modules_to_save", "fan_in_fan_out"):
+                if cfg.get(key):
+                    raise ValueError(f"{directory}: {key} = {cfg[key]!r} is not supported")
+            if cfg.get("bias", "none") != "none" or cfg.get("peft_type", "LORA") != "LORA":
+                raise ValueError(f"{directory}: not a low-rank adapter without biases")
+            parts: dict = {}
+            for key, t in load_file(directory / "adapter_model.safetensors").items():
+                name, _, kind = key.removeprefix("base_model.model.").rpartition(".lora_")
+                if kind not in ("A.weight", "B.weight") or not name:
+                    raise ValueError(f"{directory}: {key} is not supported")
+                parts.setdefault(name, {})[kind[0]] = t
+            if any(len(pair) != 2 for pair in parts.values()) or not parts:
+                raise ValueError(f"{directory}: a module needs lora_A and lora_B")
+            adapters.append({name: (pair["A"], pair["B"]) for name, pair in parts.items()})
+            scales.append(cfg["lora_alpha"] / (math.sqrt(cfg["r"]) if cfg.get("use_rslora") else cfg["r"]))
+        return cls(adapters, scales, dtype, device)
+
+    def check(self, shapes: Mapping, dtype: torch.dtype, device) -> None:
+        """Raise where these are not adapters of modules {name: (out, in)}."""
+        for name, (a, b) in self.stacks.items():
+            if name not in shapes:
+                raise ValueError(f"an adapter changes {name}, which is no projection of the model")
+            if (b.shape[1], a.shape[2]) != tuple(shapes[name]):
+                raise ValueError(f"{name} is {list(shapes[name])}, its adapters {[b.shape[1], a.shape[2]]}")
+            if a.dtype != dtype or a.device != device:
+                raise ValueError(f"adapters are {a.dtype} on {a.device}, the model {dtype} on {device}")
+
+    def add(self, name: str, y: Tensor, x: Tensor, rows: Tensor) -> Tensor:
+        """``lora_add`` of module `name`, rows: each row's adapter; y where none
+        changes the module."""
+        stack = self.stacks.get(name)
+        return y if stack is None else lora_add(y, x, *stack, rows, self.scales)
