@@ -31,12 +31,11 @@
 // before the length and, of the new ones, the bits of its mask.  A row is a (new
 // token, query head) of the cache head, up to 64 rows share what a workgroup reads,
 // and which of them see a token is asked only in the tiles where they differ.  4
-// flops for each element and row: at 64 rows the exponentials, products and the
+// flops for each element and row: from 64 rows on the exponentials, products and the
 // waits between them bound it, not HBM (16 new tokens, 32 query heads on 8 of 128
-// columns: 131072 tokens 135 + 8 us of the join = 3.8 TB/s; 13 of 32 sequences of 0 to
-// 8191 152 + 10; 64 new tokens of 16 sequences of 4096, 4 groups of rows 263 + 9).
-// Up to 16 rows are a wave's as above, 32 or 64 two waves' on each piece of tokens:
-// one loads keys, the other values, for both.
+// columns: 131072 tokens 139 + 8 us of the join = 3.8 TB/s; 13 of 32 sequences of 0 to
+// 8191 152 + 10; 64 new tokens of 16 sequences of 4096, 256 rows a group 174 + 16 =
+// 0.40 PFLOP/s, matrix units busy for a third and vector units for half of it).
 #pragma once
 
 #include "tp_ops_common.h"
@@ -67,6 +66,11 @@ constexpr int kRowTile = 16;  // query rows: columns of a matrix instruction
 template <int DP, int H>
 __host__ __device__ constexpr int paged_waves() {
   return DP <= 64 && H == 1 ? 8 : 4;
+}
+
+template <int DP, int H>
+__host__ __device__ constexpr int paged_threads() {
+  return 64 * (H > 1 ? 2 : 1) * paged_waves<DP, H>();
 }
 
 struct PagedArgs {
@@ -180,8 +184,12 @@ struct RowSight {
 
 // (13 new tokens of 32 sequences of 0 to 8191 tokens, 8 cache heads of 128: 0 / 1 / 2
 // / 3 / 4 / 6 units 247 / 194 / 173 / 165 / 155 / 156 us, of 61 such 468 / 353 / 351 /
-// 326 / 309 / 303; 32 of 4096 tokens each 139 / 135 / 136 / 137 / 137 / 137)
-constexpr int kLead = 4;
+// 326 / 309 / 303; 32 of 4096 tokens each 139 / 135 / 136 / 137 / 137 / 137.  256 rows,
+// whose units take longer: 64 new tokens of 16 sequences of 0 to 8191, 0 / 1 / 2 / 3 / 4
+// units 353 / 222 / 187 / 173 / 172 us, of 16 of 4096 each 167 / 175 / 179 / 174 / 182)
+template <int H>
+constexpr int kLead = H == 1 ? 0 : H == 2 ? 4 : 3;
+
 
 // Tokens of a sequence that attention reads: [0, sinks) and [first, len).  They
 // are counted through in tiles from 0: the first `near` of the count are the
@@ -286,53 +294,55 @@ __device__ __forceinline__ f32x2 get_device(const float* p) {
   return f32x2{__builtin_bit_cast(float, (uint32_t)v), __builtin_bit_cast(float, (uint32_t)(v >> 32))};
 }
 
-// H RT tiles of 16 query rows share the keys and values that a workgroup reads: its H
-// sets of W waves each take the same tokens for RT tiles of their own (two waves on a
-// SIMD, one of whose matrix instructions run under the other's exponentials: 16 new
-// tokens over 131072 170 us with one wave of 64 rows).  A row is a query head of the
-// cache head; TREE: row r is new token r / group's head r % group.
+// H RT tiles of 16 query rows share the keys and values that a workgroup reads.  H > 1:
+// of its eight waves four load keys and four values, past LDS for all; H sets of 8 / H
+// waves each take RT tiles of rows, and the waves of a set every (8 / H)-th of the four
+// tiles of tokens.  (Two waves on a SIMD, one of whose matrix instructions run under the
+// other's exponentials: 16 new tokens over 131072 170 us with one wave of 64 rows.)  A
+// row is a query head of the cache head; TREE: row r is new token r / group's head r %
+// group.
 template <typename T, int DP, bool EXACT, int RT, int H, bool TREE>
-__global__ void __launch_bounds__((64 * H * paged_waves<DP, H>()), 1) paged_attention_kernel(const PagedArgs a) {
+__global__ void __launch_bounds__((paged_threads<DP, H>()), 1) paged_attention_kernel(const PagedArgs a) {
   constexpr int W = paged_waves<DP, H>(), UNIT = W * kTile, MINE = RT * kRowTile, ROWS = H * MINE;
+  constexpr int THREADS = paged_threads<DP, H>(), WAVES = THREADS / 64, G = WAVES / H;  // G: waves of a set
   typedef typename Mma<T>::v8 v8;
   typedef int16_t i16x8 __attribute__((ext_vector_type(8)));
-  constexpr int LEAD = H > 1 ? kLead : 0;
+  constexpr int LEAD = kLead<H>;
   constexpr int KS = DP / 32;        // k steps of S^T
   constexpr int DT = DP / 16;        // row tiles of O^T
   constexpr int C = DP / 8;          // 16-byte chunks of a row
   constexpr int VL = C / 2;          // V loads per lane and tile
   constexpr int kRow = 2 * DP + 32;  // LDS bytes of a V row: 16 rows' 32-byte pieces fall on distinct banks
-  // H > 1: of two waves of the same tokens the first loads keys, the other values, past
-  // LDS for both; rows of keys lie 16 bytes further apart than they are long, so that
-  // 16 rows' pieces are on distinct banks.
+  // H > 1: rows of keys lie 16 bytes further apart in LDS than they are long, so that 16
+  // rows' pieces are on distinct banks.
   constexpr bool SHARED = H > 1;
-  static_assert(H <= 2, "");
   constexpr int kRowK = 2 * DP + 16;
   // a wave's values (or keys), then its outputs of a tile of rows
   constexpr int kPiece = kTile * kRow;
-  static_assert(kPiece >= kTile * kRowK && kPiece >= kRowTile * DP * 4 && H * W * kPiece >= ROWS * DP * 4, "");
-  __shared__ __attribute__((aligned(16))) char v_lds[H * W][kPiece];
-  __shared__ TokenRows rows[H * W][2][kTile];
-  __shared__ float ml[2][W][ROWS];
+  static_assert(kPiece >= kTile * kRowK && kPiece >= kRowTile * DP * 4 && (H > 1 || W * kPiece >= ROWS * DP * 4), "");
+  __shared__ __attribute__((aligned(16))) char v_lds[WAVES][kPiece];
+  __shared__ TokenRows rows[WAVES][2][kTile];
+  __shared__ float ml[2][G][ROWS];
   __shared__ uint32_t ticket;
-  __shared__ RowSight sight[TREE ? H * W : 1][TREE ? MINE : 1];  // (a wave's own copy: read where a tile is hidden from some)
+  __shared__ RowSight sight[TREE ? WAVES : 1][TREE ? MINE : 1];  // (a wave's own copy: read where a tile is hidden from some)
   // TREE: outputs that are +infinity (1), -infinity (2) or NaN (3) by a value that is,
   // 16 in a word; whether there are any.
   __shared__ uint32_t odd_out[TREE ? ROWS : 1][TREE ? DP / 16 : 1], odd_any;
   if constexpr (TREE) {
-    for (int x = threadIdx.x; x < ROWS * (DP / 16); x += 64 * H * W) odd_out[x / (DP / 16)][x % (DP / 16)] = 0;
+    for (int x = threadIdx.x; x < ROWS * (DP / 16); x += THREADS) odd_out[x / (DP / 16)][x % (DP / 16)] = 0;
     if (threadIdx.x == 0) odd_any = 0;
     __syncthreads();
   }
-  // Many rows' queries are read from LDS at each tile, in the order of the
-  // operands: registers hold no more beside the outputs.
-  constexpr bool Q_LDS = H * RT > 1;
+  // Many rows' queries are read from LDS at each tile, in the order of the operands:
+  // registers hold no more beside the outputs.  (256 rows' would fill it.)
+  constexpr bool Q_LDS = H * RT > 1 && H <= 2;
   // 256 columns: the next keys' registers are free only behind the values' products.
   constexpr bool K_LATE = RT > 1 && DP > 192;
   __shared__ __attribute__((aligned(16))) v8 q_lds[Q_LDS ? H * RT : 1][KS][64];
 
   const int lane0 = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int half = H > 1 ? wave / W : 0, first_tile = wave - half * W;  // its set, and its tile of each W
+  const int half = SHARED ? wave / W : 0, first_tile = wave - half * W;  // of keys or values, its tile of each W to load
+  const int set = SHARED ? wave / G : 0, first_seen = wave - set * G;    // its rows, and its first tile of each W
   const int per_seq = a.hkv * a.row_groups;  // (cache head, row group) pairs of a sequence
   const int all_rows = TREE ? a.tokens * a.group : a.group;
 
@@ -412,7 +422,7 @@ __global__ void __launch_bounds__((64 * H * paged_waves<DP, H>()), 1) paged_atte
     int all_first = 0;  // TREE: where the last row's window begins
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
-      const int row = row0 + half * MINE + kRowTile * r + lr;
+      const int row = row0 + set * MINE + kRowTile * r + lr;
       const T* p = static_cast<const T*>(a.q) + b * a.q_batch;
       if constexpr (TREE) {
         const int token = min(row, all_rows - 1) / a.group;
@@ -441,7 +451,7 @@ __global__ void __launch_bounds__((64 * H * paged_waves<DP, H>()), 1) paged_atte
       for (int s = 0; s < KS; ++s) {
         const bool in = row - row0 < heads && (EXACT || 32 * s + 8 * lg < a.d);
         if constexpr (!Q_LDS) q[r][s] = signed_q(load16<!TREE, v8>(in ? p + 32 * s + 8 * lg : zeros));
-        else if (first_tile == (r * KS + s) % W) q_lds[half * RT + r][s][lane] = signed_q(load16<!TREE, v8>(in ? p + 32 * s + 8 * lg : zeros));
+        else if (first_seen == (r * KS + s) % G) q_lds[set * RT + r][s][lane] = signed_q(load16<!TREE, v8>(in ? p + 32 * s + 8 * lg : zeros));
       }
     }
     if constexpr (TREE) {
@@ -452,7 +462,7 @@ __global__ void __launch_bounds__((64 * H * paged_waves<DP, H>()), 1) paged_atte
       }
     }
 
-    if constexpr (Q_LDS) __syncthreads();
+    if constexpr (Q_LDS || SHARED) __syncthreads();
 
     auto put_rows = [&](int i, int page) __attribute__((always_inline)) {
       const int t = first_of(i) + (lane & 31);
@@ -503,7 +513,6 @@ __global__ void __launch_bounds__((64 * H * paged_waves<DP, H>()), 1) paged_atte
     }
     load_v(first_tile);
     __builtin_amdgcn_sched_barrier(0);
-    const int v_wave = SHARED ? W + first_tile : wave;  // whose piece holds the values
     auto put_v = [&]() __attribute__((always_inline)) {
 #pragma unroll
       for (int c = 0; c < VL; ++c) *reinterpret_cast<v8*>(v_lds[wave] + v_token(c) * kRow + 16 * v_piece(c)) = v[c];
@@ -530,8 +539,9 @@ __global__ void __launch_bounds__((64 * H * paged_waves<DP, H>()), 1) paged_atte
         *at = (T)0.0f;
         const uint32_t is = w & (0x7fff & ~Mma<T>::kExponent) ? 3 : w >> 15 ? 2 : 1;
         const int t = t0 + c / DP, j = t - sp.before;
+#pragma unroll 1
         for (int r = 0; r < ROWS; ++r) {
-          const RowSight mine = sight[H == 1 ? wave : r / MINE * W + first_tile][r % MINE];
+          const RowSight mine = sight[H == 1 ? wave : r / MINE * G][r % MINE];
           if (j < 0 ? t >= mine.first || t < a.sinks : j < a.tokens && (mine.bits >> (j & 63) & 1))
             atomicOr(&odd_out[r][c % DP / 16], is << (2 * (c % 16)));
         }
@@ -540,7 +550,7 @@ __global__ void __launch_bounds__((64 * H * paged_waves<DP, H>()), 1) paged_atte
       wave_lds_fence();
     };
     // V^T: a lane takes column 16 t + lr of tokens 16 h + 4 lg .. + 3
-    auto read_v = [&](int t) __attribute__((always_inline)) {
+    auto read_v = [&](int v_wave, int t) __attribute__((always_inline)) {  // (whose piece holds the values)
       i16x4 part[2];
 #pragma unroll
       for (int h = 0; h < 2; ++h)
@@ -609,7 +619,7 @@ __global__ void __launch_bounds__((64 * H * paged_waves<DP, H>()), 1) paged_atte
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int t = 0; t < DT; ++t) {
-          const v8 both = __builtin_bit_cast(v8, read_v(t));
+          const v8 both = __builtin_bit_cast(v8, read_v(wave, t));
           o[0][t] = Mma<T>::mul(both, p, o[0][t]);
           o[0][t] = Mma<T>::mul(both, rest, o[0][t]);
           if (t % 4 == 3) __builtin_amdgcn_sched_barrier(0);  // (eight reads at a time: registers)
@@ -622,11 +632,12 @@ __global__ void __launch_bounds__((64 * H * paged_waves<DP, H>()), 1) paged_atte
       // the matrix instructions' alone and stay in their registers (64 rows of 128
       // columns: 128 products and 400 copies a tile otherwise).
       int i = first_tile;
-      bool staged = false;  // SHARED: the tile is in LDS
+      bool staged = false;  // SHARED: W tiles are in LDS, of which a wave takes every G-th
+      int seen = first_seen, step = W;
       while (i < tiles) {
         float top[RT];
         bool above = false;
-        for (; i < tiles; i += W) {
+        for (; i < tiles; i += G < W ? step : W) {
           if constexpr (SHARED) {
             if (!staged) {
               // this tile past LDS, the next one's loads behind it
@@ -647,20 +658,27 @@ __global__ void __launch_bounds__((64 * H * paged_waves<DP, H>()), 1) paged_atte
             }
             staged = true;
           }
+          const int piece = !SHARED ? wave : G == W ? first_seen : seen, tile = SHARED ? i - first_tile + piece : i;
           f32x4 s[RT][2];
+          v8 kc[2][KS];
+          const bool mine_masked = rows[piece][(i / W) & 1][lane & 31].k == (uint64_t)zeros;
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
+          for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int r = 0; r < RT; ++r) s[r][h] = f32x4{0, 0, 0, 0};
+            for (int c = 0; c < KS; ++c)
+              kc[h][c] = SHARED ? *reinterpret_cast<const v8*>(v_lds[piece] + (16 * h + lr) * kRowK + 64 * c + 16 * lg) : k[SHARED ? 0 : h][c];
+          if constexpr (SHARED) __builtin_amdgcn_sched_barrier(0);  // (all reads from LDS in flight)
 #pragma unroll
-            for (int c = 0; c < KS; ++c) {
-              const v8 kc = SHARED ? *reinterpret_cast<const v8*>(v_lds[first_tile] + (16 * h + lr) * kRowK + 64 * c + 16 * lg) : k[SHARED ? 0 : h][c];
+          for (int c = 0; c < KS; ++c)
 #pragma unroll
-              for (int r = 0; r < RT; ++r) s[r][h] = Mma<T>::mul(kc, Q_LDS ? q_lds[half * RT + r][c][lane] : q[r][c], s[r][h]);
-            }
-          }
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+              for (int r = 0; r < RT; ++r) {
+                if (c == 0) s[r][h] = f32x4{0, 0, 0, 0};
+                s[r][h] = Mma<T>::mul(kc[h][c], Q_LDS ? q_lds[set * RT + r][c][lane] : q[r][c], s[r][h]);
+              }
           // lane: row 16 r + lr, tokens 16 h + 4 lg + e
-          const uint64_t masked = __ballot(rows[wave][(i / W) & 1][lane & 31].k == (uint64_t)zeros);
+          const uint64_t masked = __ballot(mine_masked);
           if (masked) {
 #pragma unroll
             for (int h = 0; h < 2; ++h)
@@ -672,7 +690,7 @@ __global__ void __launch_bounds__((64 * H * paged_waves<DP, H>()), 1) paged_atte
                 }
           }
           // tokens that some rows see and others do not
-          const int t0 = first_of(i);
+          const int t0 = first_of(tile);
           const bool some = !(t0 + kTile <= sp.before && (t0 >= all_first || t0 + kTile <= a.sinks));
           if (some) {
 #pragma unroll
@@ -712,6 +730,18 @@ __global__ void __launch_bounds__((64 * H * paged_waves<DP, H>()), 1) paged_atte
             if (!K_LATE) load_k(i + W);
           }
 
+          // values are read from LDS two tiles of columns ahead of their products, the
+          // first ones ahead of the exponentials
+          v8 both[2][2];
+          auto read_two = [&](int t) __attribute__((always_inline)) {
+#pragma unroll
+            for (int u = 0; u < 2; ++u) both[t / 2 & 1][u] = __builtin_bit_cast(v8, read_v(SHARED ? W + piece : wave, t + u));
+          };
+          if constexpr (SHARED) {
+            read_two(0);
+            __builtin_amdgcn_sched_barrier(0);
+          }
+
           v8 p[RT], rest[RT];
 #pragma unroll
           for (int r = 0; r < RT; ++r) {
@@ -736,20 +766,29 @@ __global__ void __launch_bounds__((64 * H * paged_waves<DP, H>()), 1) paged_atte
             __builtin_amdgcn_sched_barrier(0);
             load_v(i + W);
             __builtin_amdgcn_sched_barrier(0);
+            read_two(0);
           }
 #pragma unroll
-          for (int t = 0; t < DT; ++t) {
-            const v8 both = __builtin_bit_cast(v8, read_v(t));
+          for (int t = 0; t < DT; t += 2) {
+            if (t + 2 < DT) read_two(t + 2);
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int r = 0; r < RT; ++r) {
-              o[r][t] = Mma<T>::mul(both, p[r], o[r][t]);
-              o[r][t] = Mma<T>::mul(both, rest[r], o[r][t]);
-            }
-            if (t % 4 == 3) __builtin_amdgcn_sched_barrier(0);  // (eight reads at a time: registers)
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+              for (int r = 0; r < RT; ++r) o[r][t + u] = Mma<T>::mul(both[t / 2 & 1][u], p[r], o[r][t + u]);
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+              for (int r = 0; r < RT; ++r) o[r][t + u] = Mma<T>::mul(both[t / 2 & 1][u], rest[r], o[r][t + u]);
+            __builtin_amdgcn_sched_barrier(0);
           }
           if constexpr (SHARED) {
-            staged = false;
-            __syncthreads();  // (both waves have read the tile)
+            if constexpr (G < W) seen += G, step = 0;
+            if (G == W || seen >= W) {
+              staged = false;
+              if constexpr (G < W) seen = first_seen, step = W;
+              __syncthreads();  // (all waves have read the tiles)
+            }
           } else {
             wave_lds_fence();
             if (K_LATE) load_k(i + W);
@@ -773,8 +812,8 @@ __global__ void __launch_bounds__((64 * H * paged_waves<DP, H>()), 1) paged_atte
     for (int r = 0; r < RT; ++r) {
       l[r] = combine32<AddOp>(combine16<AddOp>(l[r]));
       if (lane < kRowTile) {
-        const int row = half * MINE + kRowTile * r + lane;
-        ml[0][first_tile][row] = m[r], ml[1][first_tile][row] = l[r];
+        const int row = set * MINE + kRowTile * r + lane;
+        ml[0][first_seen][row] = m[r], ml[1][first_seen][row] = l[r];
       }
     }
     auto with_odd = [&](int h, int c, f32x4 y) __attribute__((always_inline)) {
@@ -807,10 +846,10 @@ __global__ void __launch_bounds__((64 * H * paged_waves<DP, H>()), 1) paged_atte
 #pragma unroll
         for (int t = 0; t < DT; ++t) *reinterpret_cast<f32x4*>(ow + lr * DP + 16 * t + 4 * lg) = o[r][t];
         __syncthreads();
-        join_waves<DP, W, ROWS, 64 * H * W>(
-            tid, H == 1 ? min(kRowTile, heads - kRowTile * r) : H * kRowTile, heads, W, ml,
+        join_waves<DP, G, ROWS, THREADS>(
+            tid, H == 1 ? min(kRowTile, heads - kRowTile * r) : H * kRowTile, heads, G, ml,
             [&](int w, int j) __attribute__((always_inline)) {
-              return reinterpret_cast<const float*>(v_lds[(H == 1 ? 0 : j / kRowTile * W) + w]) + (H == 1 ? j : j % kRowTile) * DP;
+              return reinterpret_cast<const float*>(v_lds[(H == 1 ? 0 : j / kRowTile * G) + w]) + (H == 1 ? j : j % kRowTile) * DP;
             },
             [&](int j) __attribute__((always_inline)) { return H == 1 ? kRowTile * r + j : j / kRowTile * MINE + kRowTile * r + j % kRowTile; }, f);
       }
@@ -862,7 +901,7 @@ __global__ void __launch_bounds__((64 * H * paged_waves<DP, H>()), 1) paged_atte
           float* joined = reinterpret_cast<float*>(v_lds[0]);  // [pg][groups * 64 pieces]
           auto gather = [&](auto ahead) __attribute__((always_inline)) {
             constexpr int A = decltype(ahead)::value;
-            for (int x = wave; x < groups * pg; x += H * W) {
+            for (int x = wave; x < groups * pg; x += WAVES) {
               const int part = x / groups, i = (x - part * groups) * 64 + lane;
               if (i >= pieces) continue;
               const int h = i / (DP / 4), c = 4 * (i - h * (DP / 4));
@@ -895,7 +934,7 @@ __global__ void __launch_bounds__((64 * H * paged_waves<DP, H>()), 1) paged_atte
           if (n <= 4 * pg) gather(std::integral_constant<int, 4>{});
           else gather(std::integral_constant<int, 16>{});
           __syncthreads();
-          join_waves<DP, W, ROWS, 64 * H * W>(
+          join_waves<DP, W, ROWS, THREADS>(
               tid, heads, heads, pg, ml,
               [&](int w, int j) __attribute__((always_inline)) { return joined + w * groups * 256 + j * DP; },
               [&](int j) __attribute__((always_inline)) { return j; }, put_out);
@@ -906,7 +945,7 @@ __global__ void __launch_bounds__((64 * H * paged_waves<DP, H>()), 1) paged_atte
     if constexpr (TREE) {
       if (odd_any) {  // (the next segment has none yet)
         __syncthreads();
-        for (int x = threadIdx.x; x < ROWS * (DP / 16); x += 64 * H * W) odd_out[x / (DP / 16)][x % (DP / 16)] = 0;
+        for (int x = threadIdx.x; x < ROWS * (DP / 16); x += THREADS) odd_out[x / (DP / 16)][x % (DP / 16)] = 0;
         if (threadIdx.x == 0) odd_any = 0;
         __syncthreads();
       }
@@ -919,23 +958,29 @@ __global__ void __launch_bounds__((64 * H * paged_waves<DP, H>()), 1) paged_atte
   }
 }
 
-// The states that the tree kernel's workgroups (of W waves of tokens) left of a
-// (sequence, cache head, row group), joined: blockIdx.x of those, blockIdx.y 4 rows
-// (131072 tokens, 8 cache heads of 128 and 64 rows: 7.7 us, 16 rows 14).
-template <typename T, int DP, int W, int ROWS>
+// Rows of a joining workgroup.
+template <int RT, int H>
+__host__ __device__ constexpr int join_rows() {
+  return RT * H > 4 ? 8 : 4;
+}
+
+// The states that the tree kernel's workgroups left of a (sequence, cache head, row
+// group), joined: blockIdx.x of those, blockIdx.y EACH rows (131072 tokens, 8 cache
+// heads of 128 and 64 rows: 4 a workgroup 7.7 us, 16 14).
+template <typename T, int DP, int RT, int H>
 __global__ void __launch_bounds__(128) paged_join_kernel(const PagedArgs a, int grid) {
-  constexpr int UNIT = W * kTile, STATE = ROWS * (DP + 2), A = 8;
+  constexpr int ROWS = H * RT * kRowTile, EACH = join_rows<RT, H>(), UNIT = paged_waves<DP, H>() * kTile, STATE = ROWS * (DP + 2), A = 8;
   const int lane = threadIdx.x & 63, per_seq = a.hkv * a.row_groups;
   const int b = blockIdx.x / per_seq, pair = blockIdx.x - b * per_seq;
   // units of all sequences, and those before this one
   int64_t total = 0, before = 0;
   for (int b0 = 0; b0 < a.batch; b0 += 64) {
     const int x = b0 + lane;
-    const int64_t u = x < a.batch ? (int64_t)span_of<UNIT, true, kLead>(a, a.lengths[x]).units * per_seq : 0;
+    const int64_t u = x < a.batch ? (int64_t)span_of<UNIT, true, kLead<H>>(a, a.lengths[x]).units * per_seq : 0;
     total += __shfl(wave_scan(u, lane), 63);
     before += __shfl(wave_scan(x < b ? u : 0, lane), 63);
   }
-  const int units = span_of<UNIT, true, kLead>(a, a.lengths[b]).units;
+  const int units = span_of<UNIT, true, kLead<H>>(a, a.lengths[b]).units;
   const int64_t wgs = min((int64_t)grid, total);
   const int64_t u0 = before + (int64_t)pair * units, u1 = u0 + units;
   const int64_t g0 = ((u0 + 1) * wgs - 1) / total, g1 = (u1 * wgs - 1) / total;
@@ -945,8 +990,8 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const PagedArgs a, int 
   const float* parts = a.parts + (g0 * 2 + later) * STATE;
   const int64_t next = (2 - later) * STATE;  // g0 + 1's, from g0's
   const int kvh = pair / a.row_groups, row0 = (pair - kvh * a.row_groups) * ROWS, all_rows = a.tokens * a.group;
-  for (int i = threadIdx.x; i < 4 * (DP / 4); i += 128) {
-    const int h = blockIdx.y * 4 + i / (DP / 4), c = 4 * (i % (DP / 4));
+  for (int i = threadIdx.x; i < EACH * (DP / 4); i += 128) {
+    const int h = blockIdx.y * EACH + i / (DP / 4), c = 4 * (i % (DP / 4));
     if (row0 + h >= all_rows) continue;
     float top = kLeastScore, sum = 0.0f;
     f32x4 y{0, 0, 0, 0};
@@ -979,34 +1024,40 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const PagedArgs a, int 
 // Columns that the kernel's instance for d holds.
 inline int padded_d(int64_t d) { return d <= 64 ? 64 : d <= 96 ? 96 : d <= 128 ? 128 : d <= 192 ? 192 : 256; }
 
-// Tiles of rows that share a workgroup's keys and values.
-inline int tree_row_tiles(int64_t rows, int dp) { return rows <= kRowTile ? 1 : rows <= 2 * kRowTile || dp > 128 ? 2 : 4; }
+// Tiles of rows that share a workgroup's keys and values.  256 rows past 128 (of 4
+// query heads a cache head of 128 columns: 64 new tokens of 16 sequences of 4096 tokens
+// 174 + 16 us, 64 rows a group 278 + 9; 33 of 40 of 500 99 + 17, 134 + 16; of one of 30
+// 33 + 5, 22 + 4).
+inline int tree_row_tiles(int64_t rows, int dp) {
+  return rows <= kRowTile ? 1 : rows <= 2 * kRowTile || dp > 128 ? 2 : rows <= 8 * kRowTile ? 4 : 16;
+}
 
 template <typename T, int DP, int RT, int H, bool TREE>
 void launch_rows(const PagedArgs& a, hipStream_t s) {
   const dim3 grid((uint32_t)device_cu_count());
-  if (a.d == DP) hipLaunchKernelGGL((paged_attention_kernel<T, DP, true, RT, H, TREE>), grid, dim3(64 * H * paged_waves<DP, H>()), 0, s, a);
-  else hipLaunchKernelGGL((paged_attention_kernel<T, DP, false, RT, H, TREE>), grid, dim3(64 * H * paged_waves<DP, H>()), 0, s, a);
+  if (a.d == DP) hipLaunchKernelGGL((paged_attention_kernel<T, DP, true, RT, H, TREE>), grid, dim3(paged_threads<DP, H>()), 0, s, a);
+  else hipLaunchKernelGGL((paged_attention_kernel<T, DP, false, RT, H, TREE>), grid, dim3(paged_threads<DP, H>()), 0, s, a);
 }
 
 // Trees are compiled apart, a type in a file.
 int dispatch_tree_f16(const PagedArgs& a, hipStream_t s);
 int dispatch_tree_bf16(const PagedArgs& a, hipStream_t s);
 
+template <typename T, int DP, int RT, int H>
+void launch_shared(const PagedArgs& a, hipStream_t s) {
+  launch_rows<T, DP, RT, H, true>(a, s);
+  const dim3 grid((uint32_t)(a.batch * a.hkv * a.row_groups), RT * H * kRowTile / join_rows<RT, H>());
+  hipLaunchKernelGGL((paged_join_kernel<T, DP, RT, H>), grid, dim3(128), 0, s, a, device_cu_count());
+}
+
 template <typename T, int DP>
 void launch_tree(const PagedArgs& a, hipStream_t s) {
   const int tiles = tree_row_tiles((int64_t)a.tokens * a.group, DP);
   if (tiles == 1) return launch_rows<T, DP, 1, 1, true>(a, s);
   if constexpr (DP <= 128) {
-    const dim3 grid((uint32_t)(a.batch * a.hkv * a.row_groups), tiles * kRowTile / 4);
-    constexpr int W = paged_waves<DP, 2>();
-    if (tiles == 2) {
-      launch_rows<T, DP, 1, 2, true>(a, s);
-      hipLaunchKernelGGL((paged_join_kernel<T, DP, W, 2 * kRowTile>), grid, dim3(128), 0, s, a, device_cu_count());
-    } else {
-      launch_rows<T, DP, 2, 2, true>(a, s);
-      hipLaunchKernelGGL((paged_join_kernel<T, DP, W, 4 * kRowTile>), grid, dim3(128), 0, s, a, device_cu_count());
-    }
+    if (tiles == 2) launch_shared<T, DP, 1, 2>(a, s);
+    else if (tiles == 4) launch_shared<T, DP, 2, 2>(a, s);
+    else launch_shared<T, DP, 2, 8>(a, s);
   } else {  // (registers and LDS hold no two waves a SIMD)
     launch_rows<T, DP, 2, 1, true>(a, s);
   }
