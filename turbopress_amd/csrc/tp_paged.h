@@ -33,7 +33,7 @@
 // and which of them see a token is asked only in the tiles where they differ.  4
 // flops for each element and row: from 64 rows on the exponentials, products and the
 // waits between them bound it, not HBM (16 new tokens, 32 query heads on 8 of 128
-// columns: 131072 tokens 139 + 8 us of the join = 3.8 TB/s; 13 of 32 sequences of 0 to
+// columns: 131072 tokens 133 + 8 us of the join = 3.8 TB/s; 13 of 32 sequences of 0 to
 // 8191 152 + 10; 64 new tokens of 16 sequences of 4096, 256 rows a group 174 + 16 =
 // 0.40 PFLOP/s, matrix units busy for a third and vector units for half of it).
 #pragma once
@@ -404,6 +404,8 @@ __global__ void __launch_bounds__((paged_threads<DP, H>()), 1) paged_attention_k
     const T* kbase = static_cast<const T*>(a.k) + kvh * a.kc_head;
     const T* vbase = static_cast<const T*>(a.v) + kvh * a.vc_head;
     const T* zeros = reinterpret_cast<const T*>(kZeros);
+    const T* mine_base = half == 0 ? kbase : vbase;  // SHARED
+    const int64_t mine_page = half == 0 ? a.kc_page : a.vc_page, mine_slot = half == 0 ? a.kc_slot : a.vc_slot;
 
     const int unit0 = LEAD ? max(j0 - LEAD, 0) : j0;  // first of tokens
     const int tiles = (LEAD ? max(j1 - LEAD, 0) - unit0 : j1 - j0) * W;
@@ -468,6 +470,11 @@ __global__ void __launch_bounds__((paged_threads<DP, H>()), 1) paged_attention_k
       const int t = first_of(i) + (lane & 31);
       const uint32_t slot = (uint32_t)t % (uint32_t)a.page_size;
       TokenRows r{(uint64_t)zeros, (uint64_t)zeros};
+      if constexpr (SHARED) {  // (a wave loads keys or values: .k is its own row)
+        if (page >= 0 && page < a.n_pages) r.k = (uint64_t)(mine_base + page * mine_page + slot * mine_slot);
+        if (lane < kTile) rows[wave][(i / W) & 1][lane].k = r.k;
+        return;
+      }
       if (page >= 0 && page < a.n_pages)
         r = TokenRows{(uint64_t)(kbase + page * a.kc_page + slot * a.kc_slot), (uint64_t)(vbase + page * a.vc_page + slot * a.vc_slot)};
       if (lane < kTile) rows[wave][(i / W) & 1][lane] = r;
@@ -488,7 +495,7 @@ __global__ void __launch_bounds__((paged_threads<DP, H>()), 1) paged_attention_k
 #pragma unroll
       for (int c = 0; c < VL; ++c) {
         const TokenRows& at = rows[wave][(i / W) & 1][v_token(c)];
-        const T* r = reinterpret_cast<const T*>(SHARED && half == 0 ? at.k : at.v) + 8 * v_piece(c);
+        const T* r = reinterpret_cast<const T*>(SHARED ? at.k : at.v) + 8 * v_piece(c);
         v[c] = load16<!TREE, v8>(EXACT || 8 * v_piece(c) < a.d ? r : zeros);
       }
     };
