@@ -17,6 +17,10 @@
 // k-th largest of 128 groups' largest of those is a bound that the k likeliest
 // reach; the few sets of 128 that reach it are read again, and the logits that
 // reach it are ranked by (value, lower token first) as one whole number.
+//
+// Logits are read once, some 9 vector instructions for each (its type, exponential, two
+// sums, largest): bound by HBM and by issue alike (2047 x 151936 bf16: 119 us = 5.2 TB/s, with
+// the 20 likeliest 159; 4 rows with 5 17 us, a chain of loads, join, sets and ranking).
 #include "tp_ops_common.h"
 
 namespace tp {
@@ -465,8 +469,12 @@ __global__ void __launch_bounds__(256) token_logprobs_kernel(const LogprobArgs a
 
 // (room for the up to 7 places before a row's first logit)
 inline int64_t logprob_pieces(int64_t vocab) { return (vocab + 7 + kPiece - 1) / kPiece; }
-// Pieces of a segment: so few that kWaves waves and more have work.
-constexpr int64_t kWaves = 16384;
+// Pieces of a segment: so few that kWaves waves and more have work, no fewer: a wave's
+// start, its sums' joins and the row's ticket cost as much as several pieces (151936
+// columns, 5 likeliest, 1024 / 2048 / 4096 / 8192 / 16384 waves: 4 rows 17 us all, 100 25 /
+// 26 / 34 / 59, 256 31 / 30 / 34 / 43 / 53, 600 62 / 51 / 54 / 56; 2047 rows, 20 likeliest
+// 160 / 159 / 168 / 173 / 180).
+constexpr int64_t kWaves = 2048;
 inline int64_t logprob_span(int64_t rows, int64_t vocab) {
   const int64_t pieces = logprob_pieces(vocab), want = (kWaves + rows - 1) / rows, most = want < kSegments ? want : kSegments;
   return (pieces + most - 1) / most;

@@ -132,7 +132,8 @@ constexpr int kLine = 64;
 // A wave loads whole lines, 8 lanes each (operands straight from memory would be 64
 // accesses of 16 bytes: 2047 x 9728 of rank 64 30 us), and turns them into operands
 // in LDS of its own: piece c of row r lies at c ^ (r & 7), so that 16 rows' pieces
-// are on distinct banks.
+// are on distinct banks.  Bound by the waits for lines: 2047 x 9728 of rank 64 18.7 us =
+// 2.1 TB/s, matrix units busy for a seventh of it.
 template <typename T, int NT, int RT, int W>
 __global__ void __launch_bounds__(64 * W) lora_shrink_kernel(const LoraArgs p) {
   typedef typename LoraMma<T>::v8 v8;
@@ -258,7 +259,9 @@ __global__ void __launch_bounds__(256) lora_join_kernel(const LoraArgs p) {
   leave_h<T>(p, row, c, sum, p.scales ? p.scales[who] : 1.0f);
 }
 
-// The outputs of 16 NT rows and 256 columns.  PLAIN: a rank that is a
+// The outputs of 16 NT rows and 256 columns (64 rows of 32 adapters of rank 64, 2560 ->
+// 9728 bf16: 15.5 us, of which 45 MB of weights take 7; 2047 rows, 9728 -> 2560 fp16 12.6,
+// y in and out 4.1).  PLAIN: a rank that is a
 // multiple of 8 and 64 columns and more, of which the last wave takes the last 64.
 // Loads that need no other's result are issued together: the ids, then y, h and the
 // first weights; the next step's while one is multiplied.
@@ -385,10 +388,22 @@ struct LoraPlan {
   int64_t parts_bytes, operand_bytes, power_bytes;
 };
 
+// Rows of a workgroup, and over how many its adapters are shared out.  Tiles of 64 rows
+// read an adapter's weights for fewer of them, but go through each adapter that any of
+// the 64 has (fp16, rank 64, rows in order of 4 adapters, 2560 -> 9728: 1024 rows 34 us
+// in tiles of 16, 41 of 64; of 7, 9728 -> 2560: 2047 rows 48 and 39; rank 16, 2560 -> 4096,
+// 32 adapters in no order: 768 rows 51 and 111, 2047 106 and 185).  Slots for some 128
+// workgroups: a tile's adapters in turn are a chain (64 rows of 32 adapters, rank 64,
+// 2560 -> 9728: 16 slots 27 us, 4 36, 1 74; 9728 -> 2560: 26, 40 and 113), slots that find
+// none cost as well (256 rows of 4: 16 slots 27, 8 21, 4 20; of 32: 28, 25, 30).
+//
+// Parts of x A^T's sum: of tiles of 64 rows as many as bring 256 workgroups, of at least
+// 16 lines each; of 16 rows one up to 96 lines (6144 columns), which needs no join (48
+// lines a part: the same).
 inline LoraPlan lora_plan(int64_t rows, int64_t k, int64_t rank) {
   LoraPlan q;
-  q.tiles = rows > 256 ? 4 : 1;
-  q.slots = q.tiles == 1 ? 16 : 1;
+  q.tiles = rows > 1024 ? 4 : 1;
+  q.slots = q.tiles == 1 ? (int)std::min((int64_t)16, 128 / std::max((int64_t)1, (rows + 15) / 16)) : 1;
   q.hr = (int)(rank + 63) / 64 * 64;
   q.lines = (int)((k + kLine - 1) / kLine);
   q.steps = (int)(rank + 31) / 32;
