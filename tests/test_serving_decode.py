@@ -499,3 +499,52 @@ def test_adapters_of_each_sequence(model):
     assert (dec.score(prompts[1], adapter=0, sequence=3).logprobs - base).abs().max() > 0.1
     assert torch.equal(dec.score(prompts[1], sequence=3).logprobs, base)
     assert dec.adapter_of.tolist() == [1, -1, 0, -1]
+
+
+@pytest.mark.gpu
+def test_tensors_on_another_device_than_the_current_one(cuda, monkeypatch):
+    """Each entry point goes to its tensors' device before it looks for a stream."""
+    from test_serving_ops import _gen, _serve
+    from turbopress_amd import logprobs, lora, paged
+    _, run = _serve(_gen(3))
+    want = [t.clone() for t in run()]
+    entered, asked = [], []
+
+    class Device(torch.cuda.device):
+        def __enter__(self):
+            entered.append(self.idx)
+            super().__enter__()
+
+    def elsewhere(index):
+        asked.append(index)
+        return len(asked) > len(entered) * 2  # (once for each call, not again inside)
+
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    for module in (paged, logprobs, lora):
+        monkeypatch.setattr(module, "_elsewhere", elsewhere)
+    got = run()
+    assert len(entered) >= 4 and len(asked) == 2 * len(entered) and set(entered) == {0}
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.gpu
+def test_calls_with_nothing_to_do(cuda):
+    import turbopress_amd as T
+
+    def z(*shape, dtype=torch.float16):
+        return torch.zeros(*shape, dtype=dtype, device=cuda)
+
+    i32 = torch.int32
+    cache = z(3, 4, 2, 8)
+    assert T.paged_tree_attention(z(0, 3, 4, 8), cache, cache, z(0, 2, dtype=i32), z(0, dtype=i32)).shape == (0, 3, 4, 8)
+    # no pages at all, and a table of no columns
+    q = torch.ones(2, 3, 4, 8, dtype=torch.float16, device=cuda)
+    n = torch.tensor([5, 0], dtype=i32, device=cuda)
+    assert not T.paged_tree_attention(q, z(0, 4, 2, 8), z(0, 4, 2, 8), z(2, 2, dtype=i32), n).any()
+    assert not T.paged_tree_attention(q, cache, cache, z(2, 0, dtype=i32), n).any()
+    got = T.token_logprobs(z(0, 9), z(0, dtype=torch.int64), top=2)
+    assert got.logprobs.shape == got.entropy.shape == (0,) and got.top_tokens.shape == (0, 2)
+    assert T.lora_add(z(0, 6), z(0, 5), z(3, 2, 5), z(3, 6, 2), z(0, dtype=i32)).shape == (0, 6)
+    y, ids = torch.rand(4, 6, device=cuda).half(), torch.tensor([0, -1, 2 ** 31 - 1, -2 ** 31], dtype=i32, device=cuda)
+    assert torch.equal(T.lora_add(y, z(4, 5), z(0, 2, 5), z(0, 6, 2), ids), y)
+    assert torch.equal(T.lora_add(y, torch.ones_like(z(4, 5)), z(1, 2, 5), z(1, 6, 2), ids), y)

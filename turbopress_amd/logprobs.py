@@ -14,7 +14,7 @@ from torch import Tensor
 from turbopress_amd import _lib
 from turbopress_amd.hip_kernel import raw_stream as _raw_stream
 from turbopress_amd.norm import DTYPE_CODES
-from turbopress_amd.paged import _workspace
+from turbopress_amd.paged import _elsewhere, _workspace
 
 __all__ = ["token_logprobs", "TokenLogprobs", "MAX_TOP"]
 
@@ -65,6 +65,9 @@ def token_logprobs(logits: Tensor, tokens: Tensor | None = None, top: int = 0) -
             or (tokens is not None and (tokens.dtype is not torch.int64 or tokens.shape != shape[:1]
                                         or tokens.get_device() != index)):
         _refuse(logits, tokens, top)
+    if _elsewhere(index):
+        with torch.cuda.device(index):
+            return token_logprobs(logits, tokens, top)
     rows, vocab = shape
     ld, step = logits.stride()
     if step != 1 and vocab > 1 or ld < 0:

@@ -17,7 +17,7 @@ from torch import Tensor
 from turbopress_amd import _lib
 from turbopress_amd.hip_kernel import raw_stream as _raw_stream
 from turbopress_amd.norm import DTYPE_CODES
-from turbopress_amd.paged import _workspace
+from turbopress_amd.paged import _elsewhere, _workspace
 
 __all__ = ["lora_add", "LoraAdapters", "MAX_RANK"]
 
@@ -83,6 +83,9 @@ def lora_add(y: Tensor, x: Tensor, a: Tensor, b: Tensor, adapters: Tensor, scale
             or (scales is not None and (scales.dtype is not torch.float32 or scales.get_device() != index
                                         or scales.shape != a.shape[:1])):
         _refuse(y, x, a, b, adapters, scales)
+    if _elsewhere(index):
+        with torch.cuda.device(index):
+            return lora_add(y, x, a, b, adapters, scales)
     k, n = x.shape[-1], y.shape[-1]
     count, rank, _ = a.shape
     out = torch.empty_like(y, memory_format=torch.contiguous_format)

@@ -227,7 +227,8 @@ def rotary_append(q: Tensor, k: Tensor, v: Tensor, table: Tensor, positions: Ten
 
     slots (int64 [tokens]): the key and value go to token slots[t] of the
     sequence's cache in place of positions[t], for drafted tokens of a tree, which
-    share positions; a negative one writes nothing."""
+    share positions; a negative one writes nothing (and of two tokens of one slot,
+    any mixture stays)."""
     if k is None or v is None or k_cache is None or v_cache is None or block_table is None:
         raise ValueError("rotary_append needs k, v, k_cache, v_cache and block_table")
     code, index, tokens, hq, d, rd = _turn(q, k, table, positions)
@@ -252,6 +253,9 @@ def rotary_append(q: Tensor, k: Tensor, v: Tensor, table: Tensor, positions: Ten
     k_token, k_head, _ = k.stride()
     v_token, v_head, _ = v.stride()
     if slots is not None:
+        if _elsewhere(index):
+            with torch.cuda.device(index):
+                return rotary_append(q, k, v, table, positions, k_cache, v_cache, block_table, sequences, interleaved, slots)
         if not slots.is_contiguous():
             slots = slots.contiguous()
         st = _lib.lib().tp_rotary_slots(
@@ -285,6 +289,12 @@ def _needs(index: int, batch: int, hq: int, hkv: int, d: int) -> tuple:
     """(workspace bytes, counter bytes) of a call on a device."""
     lib = _lib.lib()
     return (lib.tp_paged_attention_workspace_bytes(batch, hq, hkv, d), lib.tp_paged_attention_counter_bytes(batch, hq, hkv, d))
+
+
+def _elsewhere(index: int) -> bool:
+    """Whether a device is not the current one (whose default stream, and whose number of
+    compute units, a call would take)."""
+    return torch._C._cuda_getDevice() != index
 
 
 def _workspace(index: int, stream: int, need: int, count: int) -> tuple:
@@ -344,6 +354,9 @@ def paged_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, block_table: Te
     need, count = _needs(index, b, hq, hkv, d)
     ws, counters, _held = _workspace(index, stream, need, count)
     if sinks:
+        if _elsewhere(index):
+            with torch.cuda.device(index):
+                return paged_attention(q, k_cache, v_cache, block_table, lengths, scale, window, sinks)
         st = _lib.lib().tp_paged_attention_sinks(
             code, b, hq, hkv, d, qp, q_row, q_head, k_cache.data_ptr(), _strides(k_cache), v_cache.data_ptr(), _strides(v_cache),
             pages, page_size, block_table.data_ptr(), block_table.shape[1], lengths.data_ptr(),
@@ -428,6 +441,9 @@ def paged_tree_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, block_tabl
     pages, page_size, hkv, _ = k_cache.shape
     if d % 8 or not 8 <= d <= 256 or hq < 1 or hkv < 1 or hq % hkv:
         _refuse_tree(q, k_cache, v_cache, block_table, lengths, ancestors)
+    if _elsewhere(index):
+        with torch.cuda.device(index):
+            return paged_tree_attention(q, k_cache, v_cache, block_table, lengths, ancestors, scale, window, sinks)
     q_row, q_token, q_head, q_column = q.stride()
     qp = q.data_ptr()
     if q_column != 1 or (qp | q_row << 1 | q_token << 1 | q_head << 1) & 15:  # (a row of 16-byte pieces)
