@@ -242,7 +242,10 @@ def test_c_entry_points_refuse_on_the_host(built_lib):
     assert sinks(size=one[0] - 1) == sinks(csize=one[1] - 1) == L.TP_ERR_WORKSPACE
 
     need, count = lib.tp_paged_tree_attention_workspace_bytes(2, 5, 4, 2, 64), lib.tp_paged_tree_attention_counter_bytes(2, 5, 4, 2, 64)
-    assert need > 0 and count == 16 and lib.tp_paged_tree_attention_counter_bytes(3, 64, 8, 2, 64) == 3 * 2 * 4 * 4
+    assert need > 0 and count == 16
+    # 256 rows of a cache head: a group of 256, or, of heads of more than 128 columns, of 32 each
+    assert lib.tp_paged_tree_attention_counter_bytes(3, 64, 8, 2, 64) == 3 * 2 * 4
+    assert lib.tp_paged_tree_attention_counter_bytes(3, 64, 8, 2, 256) == 3 * 2 * 8 * 4
 
     def tree(dtype=0, batch=2, tokens=5, hq=4, hkv=2, d=64, q=p, token=256, seen=p, page=16, window=0, sinks=0, size=need, csize=count,
              kc=p, out=p):

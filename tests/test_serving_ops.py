@@ -105,6 +105,22 @@ def test_tree_head_sizes(cuda, d, dtype, count, group):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("d", [8, 64, 72, 96, 104, 128, 136, 256])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("count,group", [(43, 3), (64, 5)])
+def test_tree_rows_of_many_heads(cuda, d, dtype, count, group):
+    """129 rows of a cache head, and 320: more than one group of them."""
+    _check_tree(_gen(d + group), [0, 1, 31, 130, 700], count, 2 * group, 2, d, 16, dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lengths", [[0] * 40, [1] * 90, [0, 1500] * 4, list(range(0, 260, 16)), [6000] + [1] * 20])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (1, 0), (33, 3), (300, 40)])
+def test_tree_rows_of_many_heads_of_uneven_sequences(cuda, lengths, window, sinks):
+    _check_tree(_gen(len(lengths) + window), lengths, 36, 4, 1, 128, 16, F16, window=window, sinks=sinks)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("hq,hkv", [(1, 1), (9, 3), (7, 1), (16, 1), (17, 1), (40, 2)])
 @pytest.mark.parametrize("count", [1, 2, 7, 16])
 def test_tree_head_groups(cuda, hq, hkv, count):
@@ -150,7 +166,7 @@ def test_tree_scales(cuda, scale):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [F16, BF16])
-@pytest.mark.parametrize("count,group", [(6, 1), (20, 1), (20, 4)])
+@pytest.mark.parametrize("count,group", [(6, 1), (20, 1), (20, 4), (36, 4)])
 @pytest.mark.parametrize("window", [0, 9])
 def test_tree_hidden_tokens_do_not_matter(cuda, dtype, count, group, window):
     """NaN and infinity in keys and values of new tokens, and of cached ones that a
