@@ -380,6 +380,7 @@ __global__ void __launch_bounds__((paged_threads<DP, H>()), 1) paged_attention_k
   seq0 = uniform(seq0);
   Span sp = span_of<UNIT, TREE, LEAD>(a, a.lengths[b]);
 
+  const int sinks = (int)min(a.sinks, (int64_t)0x7fffffff);
   // TREE: scores are scaled behind their maximum, so a negative scale's sign goes
   // to the queries (and a scale of 0 is next to it: 0 times a masked -infinity).
   const float scale = TREE ? fmaxf(fabsf(a.scale), 1e-30f) : a.scale;
@@ -529,14 +530,16 @@ __global__ void __launch_bounds__((paged_threads<DP, H>()), 1) paged_attention_k
     auto clean_v = [&](int i) __attribute__((always_inline)) {
       const int t0 = first_of(i);
       if (t0 + kTile <= sp.before && (a.window <= 0 || t0 >= sp.before + a.tokens - a.window || t0 + kTile <= a.sinks)) return;
-      bool found = false;
+      // two values a word: a half of what an exponent lacks is 0 where it is all ones,
+      // else it carries into the half's top bit
+      uint32_t finite = ~0u;
 #pragma unroll
       for (int c = 0; c < VL; ++c) {
-        const i16x8 w = __builtin_bit_cast(i16x8, v[c]);
+        const u32x4 w = __builtin_bit_cast(u32x4, v[c]);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) found |= ((uint32_t)w[e] & Mma<T>::kExponent) == Mma<T>::kExponent;
+        for (int e = 0; e < 4; ++e) finite &= (~w[e] & Mma<T>::kExponent * 0x10001u) + 0x7fff7fffu;
       }
-      if (!__any(found)) return;
+      if (!__any((finite & 0x80008000u) != 0x80008000u)) return;
       wave_lds_fence();
 #pragma unroll 1
       for (int c = lane; c < kTile * DP; c += 64) {
@@ -639,6 +642,7 @@ __global__ void __launch_bounds__((paged_threads<DP, H>()), 1) paged_attention_k
       // the matrix instructions' alone and stay in their registers (64 rows of 128
       // columns: 128 products and 400 copies a tile otherwise).
       int i = first_tile;
+      bool fresh = true;    // nothing is summed yet: there is nothing to scale
       bool staged = false;  // SHARED: W tiles are in LDS, of which a wave takes every G-th
       int seen = first_seen, step = W;
       while (i < tiles) {
@@ -707,9 +711,11 @@ __global__ void __launch_bounds__((paged_threads<DP, H>()), 1) paged_attention_k
               for (int h = 0; h < 2; ++h)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
+                  // (no short cuts: as branches they are 8 RT small blocks, run once or twice a segment)
                   const int t = t0 + 16 * h + 4 * lg + e, j = t - sp.before;
-                  const bool sees = j < 0 ? t >= mine.first || t < a.sinks : j < a.tokens && (mine.bits >> (j & 63) & 1);
-                  if (!sees) s[r][h][e] = -INFINITY;
+                  const int cached = (int)(t >= mine.first) | (int)(t < sinks);
+                  const int drafted = (int)(mine.bits >> (j & 63)) & (int)(j < a.tokens);
+                  s[r][h][e] = (j < 0 ? cached : drafted) & 1 ? s[r][h][e] : -INFINITY;
                 }
             }
           }
@@ -724,10 +730,15 @@ __global__ void __launch_bounds__((paged_threads<DP, H>()), 1) paged_attention_k
             top[r] = combine32<MaxOp>(combine16<MaxOp>(top[r])) * scale;
             above |= top[r] > m[r] + kSlack;
           }
-          if (__any(above)) {  // (the tile is begun again)
-            above = true;
-            break;
+          if (__any(above)) {
+            if (!fresh) {  // (the tile is begun again)
+              above = true;
+              break;
+            }
+#pragma unroll
+            for (int r = 0; r < RT; ++r) m[r] = top[r] > m[r] + kSlack ? top[r] : m[r];
           }
+          above = fresh = false;
           if constexpr (!SHARED) {
             // rows of the next tile, pages of the one after
             put_rows(i + W, page);
