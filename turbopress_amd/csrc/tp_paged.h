@@ -33,9 +33,9 @@
 // and which of them see a token is asked only in the tiles where they differ.  4
 // flops for each element and row: from 64 rows on the exponentials, products and the
 // waits between them bound it, not HBM (16 new tokens, 32 query heads on 8 of 128
-// columns: 131072 tokens 133 + 8 us of the join = 3.8 TB/s; 13 of 32 sequences of 0 to
-// 8191 152 + 10; 64 new tokens of 16 sequences of 4096, 256 rows a group 174 + 16 =
-// 0.40 PFLOP/s, matrix units busy for a third and vector units for half of it).
+// columns: 131072 tokens 131 + 8 us of the join = 3.9 TB/s; 13 of 32 sequences of 0 to
+// 8191 143 + 10; 64 new tokens of 16 sequences of 4096, 256 rows a group 167 + 16 =
+// 0.42 PFLOP/s, matrix units busy for a third and vector units for half of it).
 #pragma once
 
 #include "tp_ops_common.h"
@@ -183,10 +183,10 @@ struct RowSight {
 };
 
 // (13 new tokens of 32 sequences of 0 to 8191 tokens, 8 cache heads of 128: 0 / 1 / 2
-// / 3 / 4 / 6 units 247 / 194 / 173 / 165 / 155 / 156 us, of 61 such 468 / 353 / 351 /
-// 326 / 309 / 303; 32 of 4096 tokens each 139 / 135 / 136 / 137 / 137 / 137.  256 rows,
+// / 3 / 4 / 6 units 207 / 163 / 150 / 141 / 146 / 147 us, of 61 such 401 / 319 / 289 /
+// 294 / 291 / 290; 32 of 4096 tokens each 126 / 129 / 128 / 131 / 129 / 130.  256 rows,
 // whose units take longer: 64 new tokens of 16 sequences of 0 to 8191, 0 / 1 / 2 / 3 / 4
-// units 353 / 222 / 187 / 173 / 172 us, of 16 of 4096 each 167 / 175 / 179 / 174 / 182)
+// units 280 / 183 / 164 / 157 / 166 us, of 16 of 4096 each 157 / 155 / 163 / 163 / 169)
 template <int H>
 constexpr int kLead = H == 1 ? 0 : H == 2 ? 4 : 3;
 
@@ -1045,7 +1045,7 @@ inline int padded_d(int64_t d) { return d <= 64 ? 64 : d <= 96 ? 96 : d <= 128 ?
 // Tiles of rows that share a workgroup's keys and values.  256 rows past 128 (of 4
 // query heads a cache head of 128 columns: 64 new tokens of 16 sequences of 4096 tokens
 // 174 + 16 us, 64 rows a group 278 + 9; 33 of 40 of 500 99 + 17, 134 + 16; of one of 30
-// 33 + 5, 22 + 4).
+// 33 + 5, 22 + 4; each 5 to 10 us less since).
 inline int tree_row_tiles(int64_t rows, int dp) {
   return rows <= kRowTile ? 1 : rows <= 2 * kRowTile || dp > 128 ? 2 : rows <= 8 * kRowTile ? 4 : 16;
 }
