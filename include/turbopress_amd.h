@@ -549,8 +549,9 @@ int64_t tp_paged_tree_attention_counter_bytes(int64_t batch, int64_t tokens, int
  * p = softmax of it: logprobs[r] = log p[tokens[r]] (tokens may be NULL; a
  * negative token gives 0, one >= vocab NaN), entropy[r] = -sum p log p, and the
  * `top` (0..64, at most vocab) largest log probabilities [rows, top] with their
- * tokens, in falling order, of equal ones the lower token first.  Sums are fp32.
- * -infinity has log probability -infinity, also where the whole row is (entropy
+ * tokens, in falling order, of equal ones the lower token first.  Sums are fp32
+ * (what is less than 2^-126 of the largest counts as 0).  Logits may be of any
+ * size that their type holds.  -infinity has log probability -infinity, also where the whole row is (entropy
  * 0).  Where a row holds NaN or +infinity, its log probabilities and entropy are
  * NaN, and its order is NaNs, then +infinity, then the rest.  The workspace
  * (tp_token_logprobs_workspace_bytes, 16-byte aligned) may hold anything; the

@@ -36,8 +36,16 @@ constexpr int kIdBits = 24;        // of a token in an order key
 constexpr int kHeld = 256;         // candidates of a row held at once
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kLn2 = 0.69314718055994530942f;
-constexpr float kLeastPower = -1.0e38f;  // where the power of two begins
-constexpr float kHuge = 1.0e37f;   // largest logits of this size and above: a way of their own
+// Powers of two that sums are about, at most and at least.  An exponent fma(x, log2e,
+// -power) is exact to a rounding of its own size, but the power itself is a rounded
+// product: within 1 of a lane's largest up to 2^24, past that by as much as the
+// product's last bits, and the largest's exponential could overflow (of -1e10 it would
+// be 2^439).  About -kMostPower logits far below it count as 0, as they do beside a
+// row's largest above -kHuge: kMostPower - kHuge log2e = 2.3e6 powers of two.
+// (Rows whose largest is kHuge and above are rare: 64 x 151936 of -1e9 alone, fp32, with
+// 5 likeliest 430 us, of which the ranking of so many equals is 280.)
+constexpr float kMostPower = 8388608.0f;
+constexpr float kHuge = 4194304.0f;  // largest logits of this size and above: a way of their own
 
 // The order of values: NaN above everything, negative zero with zero.
 __device__ __forceinline__ uint32_t order_of(float x) {
@@ -308,8 +316,9 @@ __global__ void __launch_bounds__(256) token_logprobs_kernel(const LogprobArgs a
 
   // The segment.  sum = sum 2^(x log2e - power) and off = sum of those times their
   // exponents, about the lane's own power (a whole number, so that a larger one
-  // scales both exactly); NaN where the lane meets NaN or +infinity.
-  float largest = -INFINITY, power = kLeastPower, sum = 0.0f, off = 0.0f;
+  // scales both exactly); sum is NaN where the lane meets NaN, and may be +infinity
+  // where the row's largest is kHuge and above.
+  float largest = -INFINITY, power = -kMostPower, sum = 0.0f, off = 0.0f;
   const int first = segment * a.span, last = min(first + a.span, a.pieces);
   for (int piece = first; piece < last; ++piece) {
     const int place0 = piece * kPiece + 8 * lane;
@@ -334,7 +343,7 @@ __global__ void __launch_bounds__(256) token_logprobs_kernel(const LogprobArgs a
       if ((lane & 15) < kVectors)
         put_agent(a.sets + (row * a.pieces + piece) * kPieceSets + (lane & 15) * 4 + (lane >> 4), of_set);
     }
-    const float up = fmaxf(ceilf(largest * kLog2e), kLeastPower), scale = __builtin_amdgcn_exp2f(power - up);
+    const float up = fminf(fmaxf(ceilf(largest * kLog2e), -kMostPower), kMostPower), scale = __builtin_amdgcn_exp2f(power - up);
     off = scale * __builtin_fmaf(power - up, sum, off);
     sum *= scale;
     power = up;
@@ -434,7 +443,7 @@ __global__ void __launch_bounds__(256) token_logprobs_kernel(const LogprobArgs a
       }
     }
   } else {
-    // (log2e times such logits overflows: the whole row about its largest)
+    // (their power is no whole number near them: the whole row about its largest)
     for (int place = 8 * lane; place < x.end; place += 512) {
       Eight<T> u;
       u.load(x.base, place, x.end);
