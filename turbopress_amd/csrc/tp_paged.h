@@ -436,7 +436,8 @@ __global__ void __launch_bounds__((paged_threads<DP, H>()), 1) paged_attention_k
         if (a.window > 0) {
           const int depth = __builtin_popcountll(bits);
           first = (int)max((int64_t)sp.before + depth - a.window, (int64_t)0);
-          if (__any(depth > a.window)) {  // a window ends among the new tokens
+          // a window ends among the new tokens (one whose entry is 0 is at the last place before them)
+          if (__any(depth >= a.window)) {
             const int64_t here = (int64_t)sp.before - 1 + depth;
             for (int j = 0; j < a.tokens; ++j) {
               const uint64_t other = (a.ancestors ? (uint64_t)a.ancestors[(int64_t)b * a.tokens + j] : ~0ull >> (63 - j)) & all;
