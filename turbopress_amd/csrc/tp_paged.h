@@ -960,10 +960,12 @@ __global__ void __launch_bounds__((paged_threads<DP, H>()), 1) paged_attention_k
         }
       }
     }
+    // (read ahead of the barrier: behind it a wave may note the next segment's)
+    bool odd = false;
+    if constexpr (TREE) odd = odd_any != 0;
     __syncthreads();
     if constexpr (TREE) {
-      if (odd_any) {  // (the next segment has none yet)
-        __syncthreads();
+      if (odd) {  // (the next segment has none yet)
         for (int x = threadIdx.x; x < ROWS * (DP / 16); x += THREADS) odd_out[x / (DP / 16)][x % (DP / 16)] = 0;
         if (threadIdx.x == 0) odd_any = 0;
         __syncthreads();
