@@ -374,8 +374,13 @@ def paged_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, block_table: Te
 def tree_ancestors(parents: Tensor) -> Tensor:
     """The ``ancestors`` of ``paged_tree_attention`` from the drafted tokens'
     parents: int64 [..., tokens] of indices, each below its own (-1: it follows
-    the cache; -2: there is no token), on the host or the device.  Bit j of
-    token i is set where token j is i or one that it follows."""
+    the cache; -2: there is no token).  Bit j of token i is set where token j is i
+    or one that it follows.
+
+    Parents on the host that are not so, or that are no tokens, raise ValueError.
+    On the device nobody looks (the host would have to wait): there one at or above
+    its own index is taken for the token before, one below -2 for -2, and a token
+    that follows none that is there follows the cache."""
     if parents.dtype != torch.int64 or parents.dim() < 1 or not 1 <= parents.shape[-1] <= TREE_TOKENS:
         raise ValueError(f"parents must be int64 [..., 1 to {TREE_TOKENS} tokens], got {parents.dtype} {list(parents.shape)}")
     out = torch.zeros_like(parents, memory_format=torch.contiguous_format)
@@ -383,6 +388,8 @@ def tree_ancestors(parents: Tensor) -> Tensor:
         own = 1 << i if i < 63 else -1 << 63
         p = parents[..., i:i + 1]
         before = torch.where(p >= 0, out.gather(-1, p.clamp(0, max(0, i - 1))), 0)  # (nothing is in places i and on yet)
+        if not parents.is_cuda and bool(((p < -2) | (p >= i) & (p >= 0) | (p >= 0) & (before == 0)).any()):
+            raise ValueError(f"parents of token {i} must be -2, -1 or tokens below it, got {sorted(set(p.flatten().tolist()))}")
         out[..., i:i + 1] = torch.where(p >= -1, before | own, 0)
     return out
 
