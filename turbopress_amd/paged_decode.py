@@ -508,23 +508,25 @@ class PagedDecoder:
         texts = [p.tolist() + [t] for p, t in zip(prompts, self.tokens.tolist())]
         ends = [len(t) + n_new - 1 for t in texts]
         start, timed, first, passes, idle = None, 0, 0, 0, {}
-        while any(len(t) < e for t, e in zip(texts, ends)):
-            if passes == 1:  # (the first pass may capture)
-                torch.cuda.synchronize()
-                start, first = time.perf_counter(), timed
-            drafts = []
-            for s in range(self.sequences):
-                left = ends[s] - len(texts[s]) if s < count else 0
-                if s < count and not left and s not in idle:
-                    idle[s], self._next[s] = self._next[s], -1  # (it has its tokens: its rows idle)
-                drafts.append(drafter(texts[s], min(self.draft, left - 1)) if left > 1 else None)
-            passes += 1
-            for s, (tokens, _) in enumerate(self.verify(drafts, graph)[:count]):
-                texts[s] += tokens
-                timed += len(tokens)
-        for s, p in idle.items():
-            self._next[s] = self.positions[s] = p
-            self.lengths[s] = p + 1
+        try:
+            while any(len(t) < e for t, e in zip(texts, ends)):
+                if passes == 1:  # (the first pass may capture)
+                    torch.cuda.synchronize()
+                    start, first = time.perf_counter(), timed
+                drafts = []
+                for s in range(self.sequences):
+                    left = ends[s] - len(texts[s]) if s < count else 0
+                    if s < count and not left and s not in idle:
+                        idle[s], self._next[s] = self._next[s], -1  # (it has its tokens: its rows idle)
+                    drafts.append(drafter(texts[s], min(self.draft, left - 1)) if left > 1 else None)
+                passes += 1
+                for s, (tokens, _) in enumerate(self.verify(drafts, graph)[:count]):
+                    texts[s] += tokens
+                    timed += len(tokens)
+        finally:  # (also where a drafter, or verify of what it gave, raises)
+            for s, p in idle.items():
+                self._next[s] = self.positions[s] = p
+                self.lengths[s] = p + 1
         rate = (timed - first) / (time.perf_counter() - start) if timed > first and start else float("inf")
         gain = timed / max(passes * count, 1)
         return [t[len(p):] for t, p in zip(texts, prompts)], rate, gain
