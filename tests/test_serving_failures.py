@@ -42,3 +42,12 @@ def test_finished_sequences_live_on_where_a_drafter_fails(drafting, monkeypatch,
     dec.cache.reserve(0, 32)
     assert dec.verify([([], []), None, None], graph=False) == [([(3 * t + 1) % 64], [-0.5 * t]) for t in last[:2]] + [([], [])]
     assert dec._next == [at[0] + 1, at[1] + 1, -1]
+
+
+def test_a_drafter_that_gives_more_than_is_asked_for(drafting, monkeypatch):  # noqa: F811
+    """Never more than n_new tokens of a prompt: with 4 drafted at each pass, right ones, more would come."""
+    monkeypatch.setattr(torch.cuda, "synchronize", lambda: None)
+    with pytest.raises(ValueError, match="4 tokens, up to [123] were asked for"):
+        drafting.generate_drafted([torch.arange(5)], 9, lambda history, count: _good(history, 4), graph=False)
+    tokens, _, _ = drafting.generate_drafted([torch.arange(5), torch.arange(7)], 9, _good, graph=False)
+    assert [len(t) for t in tokens] == [9, 9]

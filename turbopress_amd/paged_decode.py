@@ -498,7 +498,8 @@ class PagedDecoder:
                          adapters: Sequence | None = None) -> tuple:
         """``generate`` with drafts checked: (greedy tokens, tokens/s, tokens gained
         per pass and sequence).  drafter(history, count): ``(tokens, parents)`` of
-        up to `count` tokens behind a list of ints (``lookup_draft``)."""
+        up to `count` tokens behind a list of ints (``lookup_draft``; ValueError
+        where it gives more).  Where it raises, the sequences stay as they are."""
         if not self.draft:
             raise RuntimeError("this decoder checks no drafts (PagedDecoder(draft=...))")
         return self._decode_drafted(self._begin(prompts, n_new, adapters), prompts, n_new, drafter, graph)
@@ -518,7 +519,10 @@ class PagedDecoder:
                     left = ends[s] - len(texts[s]) if s < count else 0
                     if s < count and not left and s not in idle:
                         idle[s], self._next[s] = self._next[s], -1  # (it has its tokens: its rows idle)
-                    drafts.append(drafter(texts[s], min(self.draft, left - 1)) if left > 1 else None)
+                    asked = min(self.draft, left - 1)
+                    drafts.append(drafter(texts[s], asked) if left > 1 else None)
+                    if drafts[-1] is not None and len(drafts[-1][0]) > asked:  # (more than n_new could come of it)
+                        raise ValueError(f"the drafter gave {len(drafts[-1][0])} tokens, up to {asked} were asked for")
                 passes += 1
                 for s, (tokens, _) in enumerate(self.verify(drafts, graph)[:count]):
                     texts[s] += tokens
