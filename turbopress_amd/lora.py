@@ -149,14 +149,19 @@ class LoraAdapters:
         """From directories of ``adapter_config.json`` (r, lora_alpha, use_rslora)
         and ``adapter_model.safetensors`` (``base_model.model.<module>.lora_A.weight``
         [rank, in] and ``.lora_B.weight`` [out, rank]).  What such an adapter may have
-        beside its two products is refused."""
+        beside its two products is refused, and so are adapters of other weights than
+        the model's own (``init_lora_weights`` of pissa, olora, corda, loftq)."""
         from safetensors.torch import load_file
         adapters, scales = [], []
         for directory in map(Path, directories):
             cfg = json.loads((directory / "adapter_config.json").read_text())
-            for key in ("use_dora", "rank_pattern", "alpha_pattern", "modules_to_save", "fan_in_fan_out"):
+            for key in ("use_dora", "rank_pattern", "alpha_pattern", "modules_to_save", "fan_in_fan_out", "lora_bias", "use_qalora",
+                        "layer_replication", "alora_invocation_tokens", "trainable_token_indices", "target_parameters"):
                 if cfg.get(key):
                     raise ValueError(f"{directory}: {key} = {cfg[key]!r} is not supported")
+            if cfg.get("init_lora_weights", True) not in (True, False, None, "gaussian", "eva", "orthogonal"):
+                # (such a beginning took the two products out of the model's own weights)
+                raise ValueError(f"{directory}: init_lora_weights = {cfg['init_lora_weights']!r}: not an adapter of the model's own weights")
             if cfg.get("bias", "none") != "none" or cfg.get("peft_type", "LORA") != "LORA":
                 raise ValueError(f"{directory}: not a low-rank adapter without biases")
             parts: dict = {}
