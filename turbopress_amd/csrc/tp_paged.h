@@ -165,6 +165,20 @@ constexpr float kSlack = 4.0f;
 template <typename T>
 constexpr float kTreeUnit = __is_same(T, f16_t) ? 11.0f : 0.0f;
 
+// Exponents are one fma(score, scale, unit - m).  m is a rounded product, so that the
+// largest's is off from its unit by up to m's last bit: by an eighth at kFar, which every
+// probability of a row shares and the division takes out, and past that by more than the
+// types hold (scores of 2^27: fp16 probabilities of 2^19).  There the product is rounded
+// first, as m is, and m is taken from it.
+constexpr float kFar = 0x1p20f;
+
+// a b by itself, never a part of an fma.
+__device__ __forceinline__ float product(float a, float b) {
+#pragma clang fp contract(off)
+  const float p = a * b;
+  return p;
+}
+
 // Floats of a state: per row its maximum and sum, then the (unnormalised) outputs.
 template <int DP, int RT>
 __host__ __device__ constexpr int state_floats() {
@@ -644,6 +658,13 @@ __global__ void __launch_bounds__((paged_threads<DP, H>()), 1) paged_attention_k
       // columns: 128 products and 400 copies a tile otherwise).
       int i = first_tile;
       bool fresh = true;    // nothing is summed yet: there is nothing to scale
+      bool far = false;     // of some row of the wave |m| is above kFar
+      auto is_far = [&]() __attribute__((always_inline)) {
+        bool is = false;
+#pragma unroll
+        for (int r = 0; r < RT; ++r) is |= fabsf(m[r]) > kFar && m[r] > kLeastScore;
+        return __any(is) != 0;
+      };
       bool staged = false;  // SHARED: W tiles are in LDS, of which a wave takes every G-th
       int seen = first_seen, step = W;
       while (i < tiles) {
@@ -728,8 +749,8 @@ __global__ void __launch_bounds__((paged_threads<DP, H>()), 1) paged_attention_k
             for (int h = 0; h < 2; ++h)
 #pragma unroll
               for (int e = 0; e < 4; ++e) top[r] = fmaxf(top[r], s[r][h][e]);
-            top[r] = combine32<MaxOp>(combine16<MaxOp>(top[r])) * scale;
-            above |= top[r] > m[r] + kSlack;
+            top[r] = product(combine32<MaxOp>(combine16<MaxOp>(top[r])), scale);
+            above |= top[r] - m[r] > kSlack;
           }
           if (__any(above)) {
             if (!fresh) {  // (the tile is begun again)
@@ -737,7 +758,8 @@ __global__ void __launch_bounds__((paged_threads<DP, H>()), 1) paged_attention_k
               break;
             }
 #pragma unroll
-            for (int r = 0; r < RT; ++r) m[r] = top[r] > m[r] + kSlack ? top[r] : m[r];
+            for (int r = 0; r < RT; ++r) m[r] = top[r] - m[r] > kSlack ? top[r] : m[r];
+            far = is_far();
           }
           above = fresh = false;
           if constexpr (!SHARED) {
@@ -761,16 +783,26 @@ __global__ void __launch_bounds__((paged_threads<DP, H>()), 1) paged_attention_k
             __builtin_amdgcn_sched_barrier(0);
           }
 
+          if (far) {
+#pragma unroll
+            for (int r = 0; r < RT; ++r)
+#pragma unroll
+              for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[r][h][e] = product(s[r][h][e], scale) - m[r];
+          }
+          const float each = far ? 1.0f : scale;
+
           v8 p[RT], rest[RT];
 #pragma unroll
           for (int r = 0; r < RT; ++r) {
-            const float about = kTreeUnit<T> - m[r];
+            const float about = kTreeUnit<T> - (far ? 0.0f : m[r]);
             float x8[8];
 #pragma unroll
             for (int h = 0; h < 2; ++h)
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
-                const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r][h][e], scale, about));
+                const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r][h][e], each, about));
                 l[r] += x;
                 x8[4 * h + e] = x;
               }
@@ -816,12 +848,13 @@ __global__ void __launch_bounds__((paged_threads<DP, H>()), 1) paged_attention_k
         if (!above) break;
 #pragma unroll
         for (int r = 0; r < RT; ++r) {
-          const float to = top[r] > m[r] + kSlack ? top[r] : m[r], keep = __builtin_amdgcn_exp2f(m[r] - to);
+          const float to = top[r] - m[r] > kSlack ? top[r] : m[r], keep = __builtin_amdgcn_exp2f(m[r] - to);
           m[r] = to;
           l[r] *= keep;
 #pragma unroll
           for (int t = 0; t < DT; ++t) o[r][t] *= keep;
         }
+        far = is_far();
       }
     }
 
