@@ -56,3 +56,30 @@ def test_large_scores(cuda, count, group, d, dtype, size, scale):
             few = values[s][[t for t, x in enumerate(at) if x == best]]
             want = few.mean(0)[None].expand(group, -1)
             _within(got[s, i], want, U[dtype] * want.abs() + 2.0 ** -14 * few.abs().mean(0) + LEAST[dtype])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("count,group", [(5, 2), (24, 1), (20, 3), (40, 4)])
+@pytest.mark.parametrize("d,dtype", [(64, F16), (128, BF16), (256, F16)])
+@pytest.mark.parametrize("window", [0, 20])
+def test_rows_of_ordinary_scores_beside_them(cuda, count, group, d, dtype, window):
+    """Every third row's queries are 2^15 times the others', of powers of two: its scores are exact."""
+    from oracle import serving_oracle as O
+    from test_serving_ops import _attention_tol, _trees
+    from turbopress_amd import paged_tree_attention
+    g = _gen(count + d)
+    lengths = [0, 40, 300]
+    k, v, bt = _paged(g, [n + count for n in lengths], 1, d, 16, dtype)
+    k.copy_(torch.where(k.isnan(), k, (k * 4).round() / 4))  # (quarters up to 2^2: sums of products are exact)
+    q = _randn(g, 3, count, group, d, dtype=dtype)
+    far = (torch.arange(count * group, device="cuda") % 3 == 1).view(count, group)
+    q[:, far] = torch.where(torch.rand(3, int(far.sum()), d, generator=g, device="cuda") < 0.5, -2.0 ** 15, 2.0 ** 15).to(dtype)
+    n = torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    ancestors = _trees(g, 3, count)
+    args = dict(scale=2.0 ** -3, window=window, sinks=2)
+    got = paged_tree_attention(q, k, v, bt, n, ancestors=ancestors, **args)
+    want, size, dots = O.paged_tree_attention(q, k, v, bt, n, ancestors, **args)
+    tol = _attention_tol(want, size, torch.where(far, 0, dots), d, dtype)
+    # (exact scores times log2 e, off by 2^-24 of them: two that differ do by 2^10 at least)
+    assert dots[:, far].max() < 2.0 ** 23
+    _within(got, want, tol)
