@@ -530,7 +530,8 @@ int tp_paged_attention_sinks(int dtype, int64_t batch, int64_t hq, int64_t hkv, 
  * whose position is above its own less the window, or below sinks: token t <
  * lengths[b] has position t, new token i lengths[b] - 1 + the number of bits of
  * its ancestors.  What a token does not see does not matter to it (NaN and
- * infinity included); one that sees nothing gives zeros.  Otherwise as
+ * infinity included); one that sees nothing, or all of whose scores are
+ * -infinity, gives zeros.  Otherwise as
  * tp_paged_attention; workspace and counters likewise, of their own sizes. */
 int tp_paged_tree_attention(int dtype, int64_t batch, int64_t tokens, int64_t hq, int64_t hkv, int64_t d,
                             const void* q, int64_t q_batch, int64_t q_token, int64_t q_head, const void* k_cache,

@@ -200,10 +200,11 @@ struct RowSight {
 // / 3 / 4 / 6 units 207 / 163 / 150 / 141 / 146 / 147 us, of 61 such 401 / 319 / 289 /
 // 294 / 291 / 290; 32 of 4096 tokens each 126 / 129 / 128 / 131 / 129 / 130.  256 rows,
 // whose units take longer: 64 new tokens of 16 sequences of 0 to 8191, 0 / 1 / 2 / 3 / 4
-// units 280 / 183 / 164 / 157 / 166 us, of 16 of 4096 each 157 / 155 / 163 / 163 / 169)
+// units 280 / 183 / 164 / 157 / 166 us, of 16 of 4096 each 157 / 155 / 163 / 163 / 169.
+// Of 64 rows 3 and 4 are alike: what 4 loses of the 32 sequences it gains on the 61 and
+// on the even ones.  Of 256 rows 3 is best for uneven sequences and costs even ones 6 us.)
 template <int H>
 constexpr int kLead = H == 1 ? 0 : H == 2 ? 4 : 3;
-
 
 // Tokens of a sequence that attention reads: [0, sinks) and [first, len).  They
 // are counted through in tiles from 0: the first `near` of the count are the
@@ -1078,10 +1079,13 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const PagedArgs a, int 
 // Columns that the kernel's instance for d holds.
 inline int padded_d(int64_t d) { return d <= 64 ? 64 : d <= 96 ? 96 : d <= 128 ? 128 : d <= 192 ? 192 : 256; }
 
-// Tiles of rows that share a workgroup's keys and values.  256 rows past 128 (of 4
-// query heads a cache head of 128 columns: 64 new tokens of 16 sequences of 4096 tokens
-// 174 + 16 us, 64 rows a group 278 + 9; 33 of 40 of 500 99 + 17, 134 + 16; of one of 30
-// 33 + 5, 22 + 4; each 5 to 10 us less since).
+// Tiles of rows that share a workgroup's keys and values.  256 rows past 128 (calls, 4
+// query heads on each of 8 cache heads of 128 columns: 64 new tokens of 16 sequences of
+// 4096 tokens 166 us, 64 rows a group 207; 33 of 40 of 500 92 and 118).  Few or short
+// sequences, whose lengths only the device knows, lose by it: 33 of one of 30 26 and 20,
+// 64 of one of 4096 45 and 32, of 8 of 256 42 and 29.  Wider heads have 32 rows at most,
+// each group of which reads the cache again (256 columns: 64 of 16 of 4096 629 us, 16 of
+// each 165).
 inline int tree_row_tiles(int64_t rows, int dp) {
   return rows <= kRowTile ? 1 : rows <= 2 * kRowTile || dp > 128 ? 2 : rows <= 8 * kRowTile ? 4 : 16;
 }
@@ -1112,7 +1116,9 @@ void launch_tree(const PagedArgs& a, hipStream_t s) {
     if (tiles == 2) launch_shared<T, DP, 1, 2>(a, s);
     else if (tiles == 4) launch_shared<T, DP, 2, 2>(a, s);
     else launch_shared<T, DP, 2, 8>(a, s);
-  } else {  // (registers and LDS hold no two waves a SIMD)
+  } else {
+    // (two sets of waves as above take 136 KB of LDS for their tiles, 8 for addresses and
+    // 16 for the queries of 32 rows, all that a CU has, beside masks and sums)
     launch_rows<T, DP, 2, 1, true>(a, s);
   }
 }

@@ -145,12 +145,12 @@ int launch_rotary(RotaryArgs a, hipStream_t s) {
 using namespace tp;
 
 static int rotary(int dtype, int64_t tokens, int64_t hq, int64_t hk, int64_t d, int64_t rotary_dim,
-                         int interleaved, const void* q, int64_t q_token, int64_t q_head, const void* k,
-                         int64_t k_token, int64_t k_head, const float* table, int64_t n_positions,
-                         const int64_t* positions, void* q_out, void* k_out, const void* v, int64_t v_token,
-                         int64_t v_head, void* k_cache, const int64_t* kc, void* v_cache, const int64_t* vc,
-                         int64_t n_pages, int64_t page_size, const int32_t* block_table, int64_t table_width,
-                         int64_t n_sequences, const int32_t* sequences, const int64_t* slots, void* stream) {
+                  int interleaved, const void* q, int64_t q_token, int64_t q_head, const void* k,
+                  int64_t k_token, int64_t k_head, const float* table, int64_t n_positions,
+                  const int64_t* positions, void* q_out, void* k_out, const void* v, int64_t v_token,
+                  int64_t v_head, void* k_cache, const int64_t* kc, void* v_cache, const int64_t* vc,
+                  int64_t n_pages, int64_t page_size, const int32_t* block_table, int64_t table_width,
+                  int64_t n_sequences, const int32_t* sequences, const int64_t* slots, void* stream) {
   if (!dtype_ok(dtype)) return TP_ERR_BAD_TYPE;
   if (tokens < 0 || hq < 0 || hk < 0 || hq > 65536 || hk > 65536 || d < 2 || d > 65536 || (d & 1) || rotary_dim < 2 ||
       rotary_dim > d || (rotary_dim & 1) || n_positions < 0 || tokens > ((int64_t)1 << 40))

@@ -427,7 +427,8 @@ def paged_tree_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, block_tabl
     tokens], bit j of entry i set where new token i sees new token j, itself among
     them (``tree_ancestors``); None: a chain, each sees those up to itself.  Every
     new token sees the cache before them; an entry of 0 sees only that (rows
-    behind a sequence's last token; with a length of 0 they give zeros).
+    behind a sequence's last token; with a length of 0 they give zeros, as does a
+    token all of whose scores are -infinity).
 
     window: a token at position p sees positions above p - window and the first
     `sinks`; cached token t is at position t, new token i at lengths[s] - 1 + the
